@@ -368,6 +368,44 @@ int sx_inverse_adam_step(int N, int P, float* p, const float* grad, float* m, fl
                          float es_tol, float* best_loss, int* wait, int* active, float* loss_out, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Scaled embedding and its gradient: discrete conditions (machine, scenario, token) as rows of a learned table.
+ * table (rows, dim) and out / dout (n, dim) share `dtype`; ld = row stride in elements of the strided one (table in the
+ * lookup, dout in the gradient), out and dtable are contiguous.  ids: n DEVICE int64 (ids64 != 0) or int32; an id outside
+ * [0, rows) is padding: a row of zeros in the lookup, no gradient.
+ *   sx_embedding_forward  : out[t] = scale * table[ids[t]], computed in fp32, rounded once.
+ *   sx_embedding_backward : dtable[v] = scale * sum_{t: ids[t] = v} dout[t]; every row is written (zeros where no id points);
+ *                           fp32 sums over the tokens in their order, rounded once: the same bits on every run.
+ *                           workspace: sx_embedding_workspace_bytes, 16-byte aligned, contents irrelevant before and after.
+ * rows <= 2^24, n < 2^31 - 1024.  n = 0 is allowed.
+ * --------------------------------------------------------------------------------------------- */
+int64_t sx_embedding_workspace_bytes(int64_t n, int64_t rows, int dim);
+int sx_embedding_forward(int dtype, int64_t n, int64_t rows, int dim, const void* table, int64_t ld, const void* ids, int ids64,
+                         float scale, void* out, void* stream);
+int sx_embedding_backward(int dtype, int64_t n, int64_t rows, int dim, const void* dout, int64_t ld, const void* ids, int ids64,
+                          float scale, void* dtable, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Distillation from a teacher's top logits.  Row t: student logits z (V, `dtype`, row stride ld), K pairs (idx, top) of the
+ * teacher (contiguous; top in top_dtype, idx int64 or int32); a pair whose index is outside [0, V) is ignored.
+ *   p = softmax(top / tau) over the row's valid pairs, q = softmax(z / tau)
+ *   loss_t = tau^2 * weights[t] * sum_k p_k (log p_k - log q_{idx_k});   d loss_t / d z_v = tau * weights[t] * (q_v - sum_{idx_k = v} p_k)
+ * A row of weight 0 or without a valid pair has loss 0 and gradient 0, whatever its logits hold.  weights: [N] fp32, NULL = 1.
+ *   sx_distill_forward  : row_loss[N]; loss (nullable) = sum of row_loss, divided by max(sum weights, 1e-8) if `mean`
+ *                         (den: one float of scratch, required with mean and weights).  dlogits (nullable, row stride ldd) =
+ *                         d loss / d logits (for mean = 0: of the plain sum).  row_stats (nullable) [2][N]: kept for the call below.
+ *   sx_distill_backward : dlogits = g[t * g_stride] * (the same gradient), from the logits and row_stats of the forward call.
+ *                         ready != 0: dlogits still is what that forward call wrote; rows with g = 1 are then left as they are.
+ * 0 < tau < inf; N < 2^22.
+ * --------------------------------------------------------------------------------------------- */
+int sx_distill_forward(int dtype, int64_t N, int V, int K, const void* logits, int64_t ld, int top_dtype, const void* top,
+                       const void* idx, int idx64, float tau, const float* weights, int mean, float* row_loss,
+                       float* row_stats, float* den, float* loss, void* dlogits, int64_t ldd, void* stream);
+int sx_distill_backward(int dtype, int64_t N, int V, int K, const void* logits, int64_t ld, int top_dtype, const void* top,
+                        const void* idx, int idx64, float tau, const float* weights, int mean, const float* row_stats,
+                        const float* den, const float* g, int64_t g_stride, int ready, void* dlogits, int64_t ldd,
+                        void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Whole-network entry points: UNet.encode / UNet.decode (models.py:173-203) and their backward,
  * orchestrated in C++ so that a forward or backward pass is ONE call from the host language.
  *

@@ -1,0 +1,236 @@
+"""GPU: distillation_loss and its gradient against a plain implementation in 64 bits.
+
+Tolerances, u = 2^-24.  With |z - max| / tau <= A and |top - max| / tau <= A, an argument of exp is off by 3 u A (difference, 1 / tau,
+product), an exponential by (3 A + 4) u of itself, a sum of n of them by at most n u more (n = additions in a thread's chain plus the joins,
+<= V / 64 + 32), so q and p are off by E = (6 A + V / 64 + 64) u of themselves and each logarithm by as much in absolute terms plus 2 u of its
+own size <= 2 u (A + log V).  The row's loss, tau^2 sum p (log p - log q), is off by tau^2 * (2 E + E * max|log p - log q| + 8 u (A + log V)),
+the gradient by c (E q + E p) + half a step of its type of itself (plus u for its products, in E)."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}
+
+
+def _inputs(lead, V, K, dtype=torch.float32, tdtype=torch.float32, idt=torch.int64, seed=0, spread=3.0):
+    g = torch.Generator().manual_seed(seed)
+    z = (torch.randn(*lead, V, generator=g) * spread).to(dtype)
+    top = (torch.randn(*lead, K, generator=g) * 2.0 + 5.0).to(tdtype)
+    idx = torch.randint(0, V, (*lead, K), generator=g).to(idt)               # with entries that name the same index
+    return z.cuda().requires_grad_(True), top.cuda(), idx.cuda()
+
+
+def _ref(z, top, idx, tau, weights, reduction, g=None):
+    V = z.shape[-1]
+    z, top, idx = z.detach().double().cpu().reshape(-1, V), top.double().cpu().reshape(-1, top.shape[-1]), idx.long().cpu().reshape(-1, idx.shape[-1])
+    N = z.shape[0]
+    w = torch.ones(N, dtype=torch.float64) if weights is None else weights.double().cpu().reshape(-1)
+    den = max(float(w.sum()), 1e-8) if reduction == "mean" else 1.0
+    ok = (idx >= 0) & (idx < V)
+    loss, grad = torch.zeros(N, dtype=torch.float64), torch.zeros(N, V, dtype=torch.float64)
+    etol, ltol = torch.zeros(N, V, dtype=torch.float64), torch.zeros(N, dtype=torch.float64)
+    up = torch.ones(N, dtype=torch.float64) if g is None else (g.double().cpu().reshape(-1) if g.dim() or reduction == "none" else g.double().cpu().expand(N))
+    for r in range(N):
+        if not ok[r].any() or w[r] == 0:
+            continue
+        logq = torch.log_softmax(z[r] / tau, 0)
+        t, i = top[r][ok[r]] / tau, idx[r][ok[r]]
+        logp = torch.log_softmax(t, 0)
+        p = logp.exp()
+        d = torch.where(p > 0, logp - logq[i], torch.zeros_like(p))
+        loss[r] = tau * tau * w[r] * (p * d).sum()
+        q = logq.exp()
+        sp = torch.zeros(V, dtype=torch.float64).index_add_(0, i, p)
+        c = up[r] * w[r] * tau / den
+        grad[r] = c * (q - sp)
+        zf, tf = z[r][torch.isfinite(z[r])], t[torch.isfinite(t)]
+        A = max(float((zf.max() - zf.min()) / tau), float(tf.max() - tf.min()))
+        A = min(A, 200.0)                                                     # beyond it every exponential is 0 on both sides
+        E = (6 * A + V / 64 + 64) * U
+        etol[r] = abs(c) * E * (q + sp)
+        ltol[r] = tau * tau * abs(w[r]) * (2 * E + E * float(d[torch.isfinite(d)].abs().max() if torch.isfinite(d).any() else 0) + 8 * U * (A + math.log(V)))
+    if reduction != "none":
+        ltol = (ltol.sum() + N * U * loss.abs().sum()) / den
+        loss = loss.sum() / den
+    return loss, grad, ltol, etol
+
+
+def _check(z, top, idx, tau=1.0, weights=None, reduction="mean", g=None):
+    from unet_amd.losses import distillation_loss
+    loss = distillation_loss(z, top, idx, temperature=tau, weights=weights, reduction=reduction)
+    (grad,) = torch.autograd.grad(loss, (z,), g if g is not None else torch.ones_like(loss))
+    rl, rg, lt, gt = _ref(z, top, idx, tau, weights, reduction, g)
+    assert loss.dtype == torch.float32 and grad.dtype == z.dtype and grad.shape == z.shape
+    got = loss.detach().double().cpu().reshape(rl.shape)
+    inf = torch.isinf(rl)
+    assert torch.equal(torch.isinf(got), inf) and ((got - rl).abs() <= lt + U * rl.abs())[~inf].all(), (got - rl).abs().max()
+    gg = grad.double().cpu().reshape(rg.shape)
+    assert ((gg - rg).abs() <= gt + 1.01 * (HALF[z.dtype] + U) * rg.abs() + 1e-38).all(), ((gg - rg).abs() - gt).max()
+    return loss, grad
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lead,V,K", [((1,), 1, 1), ((3,), 2, 5), ((2, 3), 17, 3), ((5,), 255, 16), ((4,), 256, 1), ((3,), 1024, 64), ((2,), 1025, 128),
+                                      ((3,), 4099, 33), ((2,), 8192, 300), ((2,), 33001, 20), ((2,), 65536, 64), ((1,), 131071, 8), ((1,), 140000, 8)])
+def test_loss_and_gradient(lead, V, K, dtype):
+    for i, (tau, red, tdt, idt) in enumerate(((1.0, "mean", torch.float32, torch.int64), (2.0, "sum", torch.bfloat16, torch.int32), (1.5, "none", torch.float32, torch.int32))):
+        z, top, idx = _inputs(lead, V, K, dtype, tdt, idt, seed=i)
+        g = torch.randn(lead, generator=torch.Generator().manual_seed(9)).cuda() if red == "none" else None
+        _check(z, top, idx, tau, None, red, g)
+
+
+def test_upstream_gradients_other_than_one_and_a_second_backward():
+    from unet_amd.losses import distillation_loss
+    for dtype in (torch.float32, torch.bfloat16):
+        z, top, idx = _inputs((6,), 777, 9, dtype)
+        for red, g in (("mean", torch.tensor(0.3)), ("sum", torch.tensor(1.0)), ("none", torch.tensor([1.0, 0.0, -2.0, 1.0, 0.5, 3.0]))):
+            _check(z, top, idx, 2.0, None, red, g.cuda())
+        loss = distillation_loss(z, top, idx)
+        (a,) = torch.autograd.grad(loss, (z,), retain_graph=True)
+        keep = a.clone()
+        (b,) = torch.autograd.grad(loss, (z,), torch.tensor(1.0, device="cuda"), retain_graph=True)
+        assert torch.equal(a, keep) and torch.equal(a, b) and a.data_ptr() != b.data_ptr()
+        loss2 = distillation_loss(z, top, idx)
+        loss2 /= 4                                     # gradient accumulation's usual form
+        (c,) = torch.autograd.grad(loss2, (z,))
+        rg = _ref(z, top, idx, 1.0, None, "mean", torch.tensor(0.25))[1]
+        assert ((c.double().cpu() - rg).abs() <= 1e-5 * rg.abs().max() + HALF[dtype] * 1.01 * rg.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("red", ["mean", "sum", "none"])
+def test_masked_rows_hold_nothing_back(dtype, red):
+    """Rows of weight 0 and rows whose entries are all padding: loss 0 and gradient 0, with NaN and infinities in their logits."""
+    z, top, idx = _inputs((7,), 300, 6, dtype)
+    w = torch.tensor([1.0, 0.0, 2.5, 0.0, 1.0, 1.0, 0.5]).cuda()
+    with torch.no_grad():
+        z[1] = float("nan")
+        z[3, 5] = float("inf")
+        idx[4] = -1
+        z[4, :7] = float("nan")
+        top[4] = float("nan")
+        idx[5, ::2] = 300                              # outside on the other side
+        top[5, ::2] = float("inf")
+        top[1] = float("nan")
+    from unet_amd.losses import distillation_loss
+    loss = distillation_loss(z, top, idx, temperature=1.5, weights=w, reduction=red)
+    g = torch.ones_like(loss)
+    (grad,) = torch.autograd.grad(loss, (z,), g)
+    assert torch.isfinite(loss).all() and torch.isfinite(grad).all()
+    assert not grad[[1, 3, 4]].any()
+    if red == "none":
+        assert not loss.detach()[[1, 3, 4]].any()
+    live = [0, 2, 5, 6]
+    z2, t2 = z.detach().clone(), top.clone()
+    z2[[1, 3, 4]] = 0.0
+    t2[[1, 4]] = 0.0
+    t2[5, ::2] = 0.0
+    rl, rg, lt, gt = _ref(z2, t2, idx, 1.5, w, red)
+    assert ((loss.detach().double().cpu() - rl).abs() <= lt + U * rl.abs()).all()
+    assert ((grad.double().cpu() - rg).abs() <= gt + 1.01 * (HALF[dtype] + U) * rg.abs())[live].all()
+
+
+def test_all_rows_masked():
+    z, top, idx = _inputs((3,), 50, 4)
+    loss, grad = _check(z, top, idx, 1.0, torch.zeros(3).cuda(), "mean")
+    assert float(loss) == 0.0 and not grad.any()
+    from unet_amd.losses import distillation_loss
+    loss, grad = _check(z, top, torch.full_like(idx, -1), 1.0, None, "mean")
+    assert float(loss) == 0.0 and not grad.any()
+    e = torch.empty(0, 50, device="cuda", requires_grad=True)
+    loss = distillation_loss(e, torch.empty(0, 4, device="cuda"), torch.empty(0, 4, dtype=torch.int64, device="cuda"))
+    assert float(loss) == 0.0 and torch.autograd.grad(loss, (e,))[0].shape == (0, 50)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_lowest_values_and_infinities_in_the_vocabulary(dtype):
+    """A masked vocabulary (the type's lowest value or -inf) next to live logits; a teacher entry of -inf has no mass; a teacher entry with
+    mass on a -inf logit makes the loss infinite, its gradient stays finite; far offsets cancel."""
+    low = torch.finfo(dtype).min
+    for fill in (low, float("-inf")):
+        z, top, idx = _inputs((4,), 500, 8, dtype)
+        idx = idx % 250
+        with torch.no_grad():
+            z[:, 250:] = fill
+            top[0, 3] = float("-inf")
+            z[1] += 1000.0
+            idx[2, :] = idx[2, 0]
+        _check(z, top, idx, 1.0)
+    z, top, idx = _inputs((2,), 500, 8, dtype)
+    with torch.no_grad():
+        z[0, idx[0, 2]] = float("-inf")
+    loss, grad = _check(z, top, idx, 1.0, None, "none")
+    assert math.isinf(float(loss[0].detach())) and torch.isfinite(grad).all()
+    z = torch.full((2, 300), low, dtype=dtype, device="cuda", requires_grad=True)
+    _check(z, top, idx % 300, 1.0)
+
+
+def test_strided_and_misaligned_logits():
+    g = torch.Generator().manual_seed(1)
+    for dtype in (torch.float32, torch.bfloat16):
+        wide = (torch.randn(6, 2100, generator=g) * 3).to(dtype).cuda()
+        _, top, idx = _inputs((6,), 2000, 12)
+        for c0 in (0, 1, 3, 8):
+            _check(wide[:, c0:c0 + 2000].detach().requires_grad_(True), top, idx)
+        col = wide.t()[:2000].contiguous().t().detach().requires_grad_(True)       # rows that are not contiguous
+        _check(col, top, idx)
+        _check(wide[::2, :2000].detach().requires_grad_(True), top[:3], idx[:3])
+        odd = wide.reshape(-1)[5:5 + 6 * 1999].view(6, 1999).detach().requires_grad_(True)
+        _check(odd, top, idx % 1999)
+
+
+def test_same_bits_on_every_run_other_stream_and_graph_replays():
+    from unet_amd.losses import distillation_loss
+    z, top, idx = _inputs((50,), 3001, 10, torch.bfloat16)
+    w = (torch.rand(50, generator=torch.Generator().manual_seed(2)) < 0.7).cuda()
+
+    def step():
+        loss = distillation_loss(z, top, idx, temperature=2.0, weights=w)
+        return loss.detach(), torch.autograd.grad(loss, (z,))[0]
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in range(3):
+        z2, top2, idx2 = _inputs((50,), 3001, 10, torch.bfloat16, seed=seed + 20)
+        with torch.no_grad():
+            z.copy_(z2), top.copy_(top2), idx.copy_(idx2)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+def test_gradient_against_differences():
+    """Central differences of the loss in 64 bits would be the reference's own; here the kernel's loss is differenced.  Step 1/16 at an fp32
+    loss of size ~10: the loss's rounding gives 10 * 2^-22 * 8 ~ 2e-5, the third derivative (<= tau^2 / tau^3 = 1) h^2 / 6 = 6.5e-4."""
+    from unet_amd.losses import distillation_loss
+    z, top, idx = _inputs((3,), 40, 5)
+    (grad,) = torch.autograd.grad(distillation_loss(z, top, idx, reduction="sum"), (z,))
+    with torch.no_grad():
+        for r, v in ((0, 0), (1, int(idx[1, 0])), (2, 39)):
+            hi, lo = z.clone(), z.clone()
+            hi[r, v] += 1 / 16
+            lo[r, v] -= 1 / 16
+            d = (float(distillation_loss(hi, top, idx, reduction="sum")) - float(distillation_loss(lo, top, idx, reduction="sum"))) * 8
+            assert abs(d - float(grad[r, v])) <= 8e-4
+
+
+def test_no_gradient_wanted():
+    from unet_amd.losses import distillation_loss
+    z, top, idx = _inputs((5,), 600, 7)
+    a = distillation_loss(z.detach(), top, idx)
+    with torch.no_grad():
+        b = distillation_loss(z, top, idx)
+    assert not a.requires_grad and not b.requires_grad and torch.equal(a, b)
+    assert torch.equal(a, distillation_loss(z, top, idx).detach())

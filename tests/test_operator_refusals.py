@@ -1,0 +1,67 @@
+"""CPU: what the scaled embedding, the distillation loss and their C entry points refuse, before anything reaches a GPU."""
+import ctypes
+
+import pytest
+import torch
+
+
+def test_embedding_refusals():
+    from unet_amd.embedding import scaled_embedding
+    ids = torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        scaled_embedding(ids, torch.zeros(4, 8))
+
+
+def test_distillation_refusals():
+    from unet_amd.losses import distillation_loss
+    z, top, idx = torch.zeros(3, 10), torch.zeros(3, 2), torch.zeros(3, 2, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        distillation_loss(z, top, idx)
+    with pytest.raises(ValueError, match="reduction"):
+        distillation_loss(z, top, idx, reduction="median")
+    for t in (0.0, -1.0, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="temperature"):
+            distillation_loss(z, top, idx, temperature=t)
+
+
+P = ctypes.c_void_p(4096)          # an address that a refused call never reads
+
+
+def _bad(rc):
+    from unet_amd import _lib as L
+    with pytest.raises(ValueError):
+        L.check(rc)
+
+
+def test_embedding_c_entry_refusals():
+    from unet_amd import _lib as L
+    lib = L.lib()
+    need = lib.sx_embedding_workspace_bytes(100, 50, 16)
+    assert need > 0
+    for n, rows, dim in ((-1, 5, 4), (1, 0, 4), (1, 5, 0), (1, (1 << 24) + 1, 4), (1 << 31, 5, 4)):
+        _bad(lib.sx_embedding_workspace_bytes(n, rows, dim))
+    _bad(lib.sx_embedding_forward(7, 10, 5, 4, P, 4, P, 1, 1.0, P, None))
+    _bad(lib.sx_embedding_forward(0, 10, 5, 4, P, 3, P, 1, 1.0, P, None))
+    _bad(lib.sx_embedding_forward(0, 10, 5, 4, None, 4, P, 1, 1.0, P, None))
+    _bad(lib.sx_embedding_forward(0, 10, 5, 4, P, 4, None, 1, 1.0, P, None))
+    _bad(lib.sx_embedding_backward(0, 100, 50, 16, P, 16, P, 1, 1.0, P, P, need - 1, None))
+    _bad(lib.sx_embedding_backward(0, 100, 50, 16, P, 16, P, 1, 1.0, P, ctypes.c_void_p(4100), need, None))
+    _bad(lib.sx_embedding_backward(0, 100, 50, 16, P, 16, P, 1, 1.0, None, P, need, None))
+    _bad(lib.sx_embedding_backward(0, 100, 50, 16, P, 15, P, 1, 1.0, P, P, need, None))
+    assert lib.sx_embedding_forward(0, 0, 5, 4, None, 4, None, 1, 1.0, None, None) == 0
+
+
+def test_distill_c_entry_refusals():
+    from unet_amd import _lib as L
+    lib = L.lib()
+
+    def fwd(dt=0, N=3, V=10, K=2, z=P, ld=10, tdt=0, top=P, idx=P, tau=1.0, w=None, mean=1, rows=P, den=P, d=None, ldd=10):
+        return lib.sx_distill_forward(dt, N, V, K, z, ld, tdt, top, idx, 1, tau, w, mean, rows, None, den, None, d, ldd, None)
+    for kw in (dict(dt=3), dict(tdt=2), dict(N=-1), dict(N=1 << 22), dict(V=0), dict(K=0), dict(ld=9), dict(tau=0.0), dict(tau=float("nan")),
+               dict(tau=float("inf")), dict(z=None), dict(top=None), dict(idx=None), dict(rows=None), dict(d=P, ldd=9), dict(w=P, den=None)):
+        _bad(fwd(**kw))
+
+    def bwd(dt=0, V=10, ld=10, tau=1.0, stats=P, g=P, d=P, ldd=10, w=None, den=None):
+        return lib.sx_distill_backward(dt, 3, V, 2, P, ld, 0, P, P, 1, tau, w, 1, stats, den, g, 0, 0, d, ldd, None)
+    for kw in (dict(dt=5), dict(V=-1), dict(ld=9), dict(tau=-1.0), dict(stats=None), dict(g=None), dict(d=None), dict(ldd=9), dict(w=P)):
+        _bad(bwd(**kw))

@@ -90,6 +90,11 @@ SIGNATURES = {
     "sx_inverse_fit": (_i, [_i, _i, _i, _i, _i, _p, _i, _p, _p, _p, _p, _p, _p, _p, _i, _f, _p]),
     "sx_inverse_adam_step": (_i, [_i, _i, _p, _p, _p, _p, _p, _f, _f, _f, _f, _i, _f, _f, _i, _f, _p, _p, _p, _p, _p]),
     "sx_adamw_step": (_i, [_p, _p, _p, _p, _l, _f, _f, _f, _f, _f, _i, _f, _p, _f, _p, _p, _p]),
+    "sx_embedding_workspace_bytes": (_l, [_l, _l, _i]),
+    "sx_embedding_forward": (_i, [_i, _l, _l, _i, _p, _l, _p, _i, _f, _p, _p]),
+    "sx_embedding_backward": (_i, [_i, _l, _l, _i, _p, _l, _p, _i, _f, _p, _p, _l, _p]),
+    "sx_distill_forward": (_i, [_i, _l, _i, _i, _p, _l, _i, _p, _p, _i, _f, _p, _i, _p, _p, _p, _p, _p, _l, _p]),
+    "sx_distill_backward": (_i, [_i, _l, _i, _i, _p, _l, _i, _p, _p, _i, _f, _p, _i, _p, _p, _p, _l, _i, _p, _l, _p]),
     "sx_unet_num_params": (_i, [_D]),
     "sx_unet_wpack_bytes": (_l, [_D]),
     "sx_unet_workspace_bytes": (_l, [_D]),
@@ -142,6 +147,32 @@ def ptr(t):
 def stream_ptr():
     import torch
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def dtype_code(t, who):
+    """sx dtype of a floating tensor the kernels read (float32 or bfloat16), ValueError otherwise."""
+    import torch
+    if t.dtype == torch.float32:
+        return SX_F32
+    if t.dtype == torch.bfloat16:
+        return SX_BF16
+    raise ValueError(f"{who}: expected float32 or bfloat16, got {t.dtype}")
+
+
+def ids_flag(t, who):
+    """1 for int64 ids, 0 for int32, ValueError otherwise."""
+    import torch
+    if t.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"{who}: ids must be int64 or int32, got {t.dtype}")
+    return 1 if t.dtype == torch.int64 else 0
+
+
+def rows_2d(t, width):
+    """(..., width) tensor -> ((rows, width) tensor whose last dimension is contiguous, row stride); a copy only if it must be."""
+    t = t.reshape(-1, width) if width else t.reshape(0, 0)
+    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < width):
+        t = t.contiguous()
+    return t, (int(t.stride(0)) if t.shape[0] > 1 else width)
 
 
 def ptr_table(tensors):

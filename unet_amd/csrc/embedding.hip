@@ -1,0 +1,240 @@
+// Scaled embedding lookup, out[t] = scale * table[ids[t]], and its gradient, dtable[v] = scale * sum_{t: ids[t] = v} dout[t].
+//
+// Ids outside [0, rows) are padding: a row of zeros, no gradient.  Both directions are bound by memory: the lookup reads and
+// writes each row once; the gradient reads dout once and writes every row of the table once.  The sums run in fp32 over the
+// entries sorted by id (sort_ids.hip), each row summed by one group of threads in the order of its tokens, so the result does
+// not depend on the run.  A row with more than kRun tokens would keep its group busy long after the others: its entries are cut
+// into runs of kRun, summed by groups of their own into partial rows, and joined in order by a second launch.
+#include "sort_ids.h"
+#include <algorithm>
+
+namespace sx {
+
+constexpr int kRun = 64;
+constexpr int64_t kMaxRows = 1 << 24;      // the gradient's grid gives every row of the table up to 128 threads of a 2^32 limit
+
+template <typename T, typename I, bool VEC>
+__global__ __launch_bounds__(256) void embed_fwd_kernel(const T* __restrict__ table, int64_t ld, const I* __restrict__ ids, int64_t n,
+                                                        int64_t rows, int dim, float scale, T* __restrict__ out) {
+  constexpr int E = VEC ? 16 / (int)sizeof(T) : 1;
+  const int pieces = dim / E;
+  const int64_t total = n * pieces;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    const int64_t t = i / pieces;
+    const int c = (int)(i - t * pieces) * E;
+    const int64_t id = (int64_t)ids[t];
+    const bool ok = id >= 0 && id < rows;
+    const T* src = table + (ok ? id : 0) * ld + c;
+    T* dst = out + t * dim + c;
+    if constexpr (VEC) {
+      typename Elem<T>::Vec v = {};
+      if (ok) v = *reinterpret_cast<const typename Elem<T>::Vec*>(src);
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = from_f32<T>(to_f32(v[e]) * scale);
+      *reinterpret_cast<typename Elem<T>::Vec*>(dst) = v;
+    } else {
+      *dst = ok ? from_f32<T>(to_f32(*src) * scale) : from_f32<T>(0.f);
+    }
+  }
+}
+
+struct EmbedBwdArgs {
+  const void* dout; int64_t ld;
+  const int* perm; const int* key; const int* start;
+  int64_t rows; int dim; int64_t n;
+  float scale;
+  void* dtable;
+  float* part;              // [runs][2][dim]: the first and the last long row that a run of entries holds part of
+  int64_t run_blocks;       // blocks behind those of the rows
+  int64_t row_groups;
+};
+
+template <typename T, int E>
+__device__ __forceinline__ void add_row(const T* __restrict__ p, float (&acc)[E]) {
+  if constexpr (E == 1) acc[0] += to_f32(*p);
+  else {
+    typename Elem<T>::Vec v = *reinterpret_cast<const typename Elem<T>::Vec*>(p);
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] += to_f32(v[e]);
+  }
+}
+
+// sum of dout rows perm[a .. b) at column c
+template <typename T, int E>
+__device__ __forceinline__ void sum_rows(const EmbedBwdArgs& q, int a, int b, int c, float (&acc)[E]) {
+  const T* dout = (const T*)q.dout + c;
+  for (int i = a; i < b; ++i) add_row<T, E>(dout + (int64_t)q.perm[i] * q.ld, acc);
+}
+
+template <typename T, int E>
+__device__ __forceinline__ void put_row(const EmbedBwdArgs& q, int64_t v, int c, const float (&acc)[E]) {
+  T* dst = (T*)q.dtable + v * q.dim + c;
+  if constexpr (E == 1) *dst = from_f32<T>(acc[0] * q.scale);
+  else {
+    typename Elem<T>::Vec o;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = from_f32<T>(acc[e] * q.scale);
+    *reinterpret_cast<typename Elem<T>::Vec*>(dst) = o;
+  }
+}
+
+// GROUP threads share a row (or a run of a long row); blocks [0, gridDim.x - run_blocks) take the rows
+template <typename T, bool VEC, int GROUP>
+__global__ __launch_bounds__(256) void embed_bwd_kernel(EmbedBwdArgs q) {
+  constexpr int E = VEC ? 16 / (int)sizeof(T) : 1;
+  const int sub = threadIdx.x / GROUP, li = threadIdx.x % GROUP;
+  const int64_t row_blocks = gridDim.x - q.run_blocks;
+  if ((int64_t)blockIdx.x < row_blocks) {
+    const int64_t v = blockIdx.x * (int64_t)(256 / GROUP) + sub;
+    if (v >= q.rows) return;
+    const int a = q.start[v], b = q.start[v + 1];
+    if (b - a > kRun) return;
+    for (int c = li * E; c < q.dim; c += GROUP * E) {
+      float acc[E] = {};
+      sum_rows<T, E>(q, a, b, c, acc);
+      put_row<T, E>(q, v, c, acc);
+    }
+  } else {
+    const int64_t run = (blockIdx.x - row_blocks) * (int64_t)(256 / GROUP) + sub;
+    const int64_t e0 = run * kRun, e1 = std::min<int64_t>(q.n, e0 + kRun);
+    if (e0 >= q.n) return;
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      const int v = q.key[side ? e1 - 1 : e0];
+      if (v >= q.rows) continue;
+      const int a = q.start[v], b = q.start[v + 1];
+      if (b - a <= kRun) continue;
+      if (side && a < e0) continue;                      // one long row fills the run: it is its first
+      const int f = (int)std::max<int64_t>(a, e0), t = (int)std::min<int64_t>(b, e1);
+      if (!side && a >= e0 && t == e1) continue;         // it begins in this run and goes on: it is its last
+      for (int c = li * E; c < q.dim; c += GROUP * E) {
+        float acc[E] = {};
+        sum_rows<T, E>(q, f, t, c, acc);
+        float* dst = q.part + (run * 2 + side) * q.dim + c;
+#pragma unroll
+        for (int e = 0; e < E; ++e) dst[e] = acc[e];
+      }
+    }
+  }
+}
+
+// the long row that begins in a run (its last one) = that run's last part + the first parts of the runs it goes on into
+template <typename T, bool VEC, int GROUP>
+__global__ __launch_bounds__(256) void embed_join_kernel(EmbedBwdArgs q) {
+  constexpr int E = VEC ? 16 / (int)sizeof(T) : 1;
+  const int sub = threadIdx.x / GROUP, li = threadIdx.x % GROUP;
+  const int64_t run = blockIdx.x * (int64_t)(256 / GROUP) + sub;
+  const int64_t e0 = run * kRun, e1 = std::min<int64_t>(q.n, e0 + kRun);
+  if (e0 >= q.n) return;
+  const int v = q.key[e1 - 1];
+  if (v >= q.rows) return;
+  const int a = q.start[v], b = q.start[v + 1];
+  if (b - a <= kRun || a < e0) return;
+  const int64_t last = (b - 1) / kRun;
+  for (int c = li * E; c < q.dim; c += GROUP * E) {
+    float acc[E] = {};
+    for (int64_t r = run; r <= last; ++r) {
+      const float* p = q.part + (r * 2 + (r == run ? 1 : 0)) * q.dim + c;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] += p[e];
+    }
+    put_row<T, E>(q, v, c, acc);
+  }
+}
+
+struct EmbedWs { size_t perm, key, start, part, total; };
+static EmbedWs embed_ws(int64_t n, int64_t rows, int dim) {
+  EmbedWs w;
+  size_t o = 0;
+  w.perm = o; o = align_up(o + (size_t)n * 4, 256);
+  w.key = o; o = align_up(o + (size_t)n * 4, 256);
+  w.start = o; o = align_up(o + (size_t)(rows + 2) * 4, 256);
+  w.part = o; o = align_up(o + (n > kRun ? (size_t)cdiv64(n, kRun) * 2 * (size_t)dim * 4 : 0), 256);
+  w.total = o;
+  return w;
+}
+
+template <typename T, bool VEC, int GROUP>
+static int embed_bwd_launch(EmbedBwdArgs q, hipStream_t st) {
+  const int per = 256 / GROUP;
+  const int64_t runs = q.n > kRun ? cdiv64(q.n, kRun) : 0;
+  q.run_blocks = cdiv64(runs, per);
+  const int64_t blocks = cdiv64(q.rows, per) + q.run_blocks;
+  hipLaunchKernelGGL((embed_bwd_kernel<T, VEC, GROUP>), dim3((unsigned)blocks), dim3(256), 0, st, q);
+  SX_LAUNCH_CHECK("embed_bwd");
+  if (runs) {
+    hipLaunchKernelGGL((embed_join_kernel<T, VEC, GROUP>), dim3((unsigned)q.run_blocks), dim3(256), 0, st, q);
+    SX_LAUNCH_CHECK("embed_join");
+  }
+  return SX_OK;
+}
+
+template <typename T, bool VEC>
+static int embed_bwd_pick(const EmbedBwdArgs& q, hipStream_t st) {
+  const int pieces = q.dim / (VEC ? 16 / (int)sizeof(T) : 1);
+  if (pieces <= 16) return embed_bwd_launch<T, VEC, 16>(q, st);
+  if (pieces <= 64) return embed_bwd_launch<T, VEC, 64>(q, st);
+  return embed_bwd_launch<T, VEC, 128>(q, st);
+}
+
+template <typename T>
+static int embed_bwd(const EmbedBwdArgs& q, hipStream_t st) {
+  constexpr int E = 16 / (int)sizeof(T);
+  const bool vec = q.dim % E == 0 && q.ld % E == 0 && (uintptr_t)q.dout % 16 == 0 && (uintptr_t)q.dtable % 16 == 0;
+  return vec ? embed_bwd_pick<T, true>(q, st) : embed_bwd_pick<T, false>(q, st);
+}
+
+template <typename T, typename I>
+static int embed_fwd(const void* table, int64_t ld, const void* ids, int64_t n, int64_t rows, int dim, float scale, void* out, hipStream_t st) {
+  constexpr int E = 16 / (int)sizeof(T);
+  const bool vec = dim % E == 0 && ld % E == 0 && (uintptr_t)table % 16 == 0 && (uintptr_t)out % 16 == 0;
+  const int64_t total = n * (vec ? dim / E : dim);
+  const unsigned blocks = (unsigned)std::max<int64_t>(1, std::min<int64_t>(cdiv64(total, 256), 256 * 32));
+  if (vec) hipLaunchKernelGGL((embed_fwd_kernel<T, I, true>), dim3(blocks), dim3(256), 0, st, (const T*)table, ld, (const I*)ids, n, rows, dim, scale, (T*)out);
+  else hipLaunchKernelGGL((embed_fwd_kernel<T, I, false>), dim3(blocks), dim3(256), 0, st, (const T*)table, ld, (const I*)ids, n, rows, dim, scale, (T*)out);
+  SX_LAUNCH_CHECK("embed_fwd");
+  return SX_OK;
+}
+
+static int embed_check(const char* who, int dtype, int64_t n, int64_t rows, int dim, int64_t ld) {
+  SX_REQUIRE(dtype == SX_F32 || dtype == SX_BF16, "%s: dtype %d is neither fp32 nor bf16", who, dtype);
+  SX_REQUIRE(n >= 0 && n < (1ll << 31) - 1024 && rows > 0 && rows <= kMaxRows && dim > 0 && ld >= dim, "%s: bad sizes n=%lld rows=%lld dim=%d ld=%lld", who,
+             (long long)n, (long long)rows, dim, (long long)ld);
+  return SX_OK;
+}
+
+}  // namespace sx
+
+using namespace sx;
+
+extern "C" int64_t sx_embedding_workspace_bytes(int64_t n, int64_t rows, int dim) {
+  SX_TRY(embed_check("sx_embedding_workspace_bytes", SX_F32, n, rows, dim, dim));
+  return (int64_t)embed_ws(n, rows, dim).total;
+}
+
+extern "C" int sx_embedding_forward(int dtype, int64_t n, int64_t rows, int dim, const void* table, int64_t ld, const void* ids, int ids64,
+                                    float scale, void* out, void* stream) {
+  SX_TRY(embed_check("sx_embedding_forward", dtype, n, rows, dim, ld));
+  if (n == 0) return SX_OK;
+  SX_REQUIRE(table && ids && out, "sx_embedding_forward: null pointer");
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == SX_BF16)
+    return ids64 ? embed_fwd<bf16, int64_t>(table, ld, ids, n, rows, dim, scale, out, st) : embed_fwd<bf16, int32_t>(table, ld, ids, n, rows, dim, scale, out, st);
+  return ids64 ? embed_fwd<float, int64_t>(table, ld, ids, n, rows, dim, scale, out, st) : embed_fwd<float, int32_t>(table, ld, ids, n, rows, dim, scale, out, st);
+}
+
+extern "C" int sx_embedding_backward(int dtype, int64_t n, int64_t rows, int dim, const void* dout, int64_t ld, const void* ids, int ids64,
+                                     float scale, void* dtable, void* workspace, int64_t workspace_bytes, void* stream) {
+  SX_TRY(embed_check("sx_embedding_backward", dtype, n, rows, dim, ld));
+  SX_REQUIRE(dtable && workspace && (n == 0 || (dout && ids)), "sx_embedding_backward: null pointer");
+  const EmbedWs w = embed_ws(n, rows, dim);
+  SX_REQUIRE(workspace_bytes >= (int64_t)w.total && (uintptr_t)workspace % 16 == 0, "sx_embedding_backward: workspace of %lld bytes, %lld needed, 16-byte aligned",
+             (long long)workspace_bytes, (long long)w.total);
+  char* ws = (char*)workspace;
+  EmbedBwdArgs q = {};
+  q.dout = dout; q.ld = ld; q.rows = rows; q.dim = dim; q.n = n; q.scale = scale; q.dtable = dtable;
+  q.perm = (int*)(ws + w.perm); q.key = (int*)(ws + w.key); q.start = (int*)(ws + w.start); q.part = (float*)(ws + w.part);
+  hipStream_t st = (hipStream_t)stream;
+  SX_TRY(launch_sort_ids(ids, ids64, n, rows, (int*)q.perm, (int*)q.key, (int*)q.start, st));
+  return dtype == SX_BF16 ? embed_bwd<bf16>(q, st) : embed_bwd<float>(q, st);
+}

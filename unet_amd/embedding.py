@@ -1,0 +1,74 @@
+"""Learned rows for discrete conditions (machine, scenario, parameter bin): a scaled table lookup and its gradient on the HIP
+kernels of `csrc/embedding.hip`.  No counterpart in the reference, whose conditions are all continuous (`params`); the rows
+feed the same places, e.g. `UNet(..., P=dim)(x, params=scaled_embedding(ids, table))`.  No CPU fallback."""
+from __future__ import annotations
+
+import torch
+from torch import nn
+
+from . import _lib as L
+
+
+class _EmbeddingFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, table, scale):
+        dt = L.dtype_code(table, "scaled_embedding")
+        V, D = table.shape
+        i = ids.contiguous().view(-1)
+        t = table.detach()
+        t, ld = L.rows_2d(t, D)
+        out = torch.empty(*ids.shape, D, dtype=table.dtype, device=table.device)
+        with torch.cuda.device(table.device):
+            L.check(L.lib().sx_embedding_forward(dt, i.numel(), V, D, L.ptr(t), ld, L.ptr(i), L.ids_flag(ids, "scaled_embedding"),
+                                                 float(scale), L.ptr(out), L.stream_ptr()), "sx_embedding_forward")
+        ctx.save_for_backward(i)
+        ctx.meta = (dt, V, D, float(scale), table.dtype)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        (i,) = ctx.saved_tensors
+        dt, V, D, scale, dtype = ctx.meta
+        if not ctx.needs_input_grad[1]:
+            return None, None, None
+        lib = L.lib()
+        d, ld = L.rows_2d(dout, D)
+        grad = torch.empty(V, D, dtype=dtype, device=dout.device)
+        nb = L.check(lib.sx_embedding_workspace_bytes(i.numel(), V, D), "sx_embedding_workspace_bytes")
+        ws = torch.empty(nb, dtype=torch.uint8, device=dout.device)
+        with torch.cuda.device(dout.device):
+            L.check(lib.sx_embedding_backward(dt, i.numel(), V, D, L.ptr(d), ld, L.ptr(i), 1 if i.dtype == torch.int64 else 0, scale,
+                                              L.ptr(grad), L.ptr(ws), nb, L.stream_ptr()), "sx_embedding_backward")
+        return None, grad, None
+
+
+def scaled_embedding(ids, table, scale=1.0):
+    """out[..., :] = scale * table[ids[...], :] in the table's dtype (fp32 or bf16; one rounding).
+
+    ids: int64 / int32 of any shape, on the table's device.  An id outside [0, rows) -- -1 by convention -- is padding: a row of
+    zeros, no gradient.  The table's gradient sums the tokens of a row in their order, in fp32: the same bits on every run.
+    Not differentiable twice.  `scale` is a number."""
+    who = "scaled_embedding"
+    if not table.is_cuda or not ids.is_cuda:
+        raise RuntimeError(f"{who}: the HIP path needs CUDA (ROCm) tensors; this build has no CPU path")
+    if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
+        raise ValueError(f"{who}: table must be (rows, dim) with at least one of each, got {tuple(table.shape)}")
+    if ids.device != table.device:
+        raise ValueError(f"{who}: ids are on {ids.device}, the table on {table.device}")
+    L.ids_flag(ids, who)
+    L.dtype_code(table, who)
+    return _EmbeddingFn.apply(ids, table, float(scale))
+
+
+class ScaledEmbedding(nn.Module):
+    """`scaled_embedding` with its table as the parameter `weight` (num, dim), initialised N(0, 1) / scale."""
+
+    def __init__(self, num, dim, scale=1.0):
+        super().__init__()
+        self.scale = float(scale)
+        self.weight = nn.Parameter(torch.empty(num, dim))
+        nn.init.normal_(self.weight, std=1.0 / abs(self.scale) if self.scale else 1.0)
+
+    def forward(self, ids):
+        return scaled_embedding(ids, self.weight, self.scale)

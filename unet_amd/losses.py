@@ -155,6 +155,80 @@ def masked_weighted_loss(pred, target, mask, *, w=None, lam_grad=0.2, lam_w=1.0,
     return _LossFn.apply(pred, tgt, m, wt, cw, opts)
 
 
+class _DistillFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, top, idx, weights, tau, reduction):
+        V, K = logits.shape[-1], top.shape[-1]
+        z, ld = L.rows_2d(logits.detach(), V)
+        N = z.shape[0]
+        dev = logits.device
+        dt, tdt, i64 = L.dtype_code(logits, "distillation_loss"), L.dtype_code(top, "distillation_loss"), L.ids_flag(idx, "distillation_loss")
+        need = ctx.needs_input_grad[0]
+        d = torch.empty(N, V, dtype=logits.dtype, device=dev) if need else None
+        rows = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
+        loss = None if reduction == "none" else torch.empty((), dtype=torch.float32, device=dev)
+        keep = torch.empty(1 + 2 * N, dtype=torch.float32, device=dev)         # sum of the weights, row statistics
+        mean = 1 if reduction == "mean" else 0
+        with torch.cuda.device(dev):
+            L.check(L.lib().sx_distill_forward(dt, N, V, K, L.ptr(z), ld, tdt, L.ptr(top), L.ptr(idx), i64, tau, L.ptr(weights), mean,
+                                               L.ptr(rows), L.ptr(keep[1:]) if need else None, L.ptr(keep), L.ptr(loss), L.ptr(d), V,
+                                               L.stream_ptr()), "sx_distill_forward")
+        if need:
+            ctx.save_for_backward(logits, top, idx, weights, keep)
+            ctx.d, ctx.meta = d, (dt, tdt, i64, N, V, K, tau, mean, reduction)
+        return rows if reduction == "none" else loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        """The forward pass left the gradient for an upstream gradient of 1; rows with another one are computed again from the
+        logits (one rounding), not scaled after theirs."""
+        logits, top, idx, weights, keep = ctx.saved_tensors
+        dt, tdt, i64, N, V, K, tau, mean, reduction = ctx.meta
+        d, ctx.d = ctx.d, None                     # the buffer is the caller's now: a second backward pass fills one of its own
+        ready = d is not None
+        if not ready:
+            d = torch.empty(N, V, dtype=logits.dtype, device=logits.device)
+        z, ld = L.rows_2d(logits.detach(), V)
+        g = g.float().contiguous()
+        with torch.cuda.device(logits.device):
+            L.check(L.lib().sx_distill_backward(dt, N, V, K, L.ptr(z), ld, tdt, L.ptr(top), L.ptr(idx), i64, tau, L.ptr(weights), mean,
+                                                L.ptr(keep[1:]), L.ptr(keep), L.ptr(g), 1 if reduction == "none" else 0,
+                                                1 if ready else 0, L.ptr(d), V, L.stream_ptr()), "sx_distill_backward")
+        return d.view(logits.shape), None, None, None, None, None
+
+
+def distillation_loss(logits, top_logits, top_idx, *, temperature=1.0, weights=None, reduction="mean"):
+    """Distillation of `logits` (..., V) from a teacher's top logits: `top_logits` (..., K) at the indices `top_idx` (..., K).
+
+    loss = tau^2 * sum_k p_k (log p_k - log q_k) with p = softmax(top_logits / tau) over the row's K entries and q = softmax(logits /
+    tau) over all V.  An entry whose index is outside [0, V) (-1 by convention) is ignored; a row without any entry left or of
+    weight 0 has loss 0 and gradient 0, whatever its logits hold.  `weights` (...): per row, or a mask.  reduction: "mean" =
+    sum / max(sum weights, 1e-8), "sum", or "none" (a loss per row, weights included).  fp32 / bf16 logits, fp32 arithmetic, an fp32
+    loss; the gradient has the logits' dtype and only goes to the logits.  Not differentiable twice."""
+    who = "distillation_loss"
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"Unknown reduction={reduction}")
+    tau = float(temperature)
+    if not 0.0 < tau < float("inf"):
+        raise ValueError(f"{who}: temperature must be positive and finite, got {temperature}")
+    for t in (logits, top_logits, top_idx):
+        _require_cuda(t, who)
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"{who}: logits must be (..., V), got {tuple(logits.shape)}")
+    lead = tuple(logits.shape[:-1])
+    if top_logits.dim() < 1 or top_logits.shape[-1] < 1 or tuple(top_logits.shape) != tuple(top_idx.shape) or tuple(top_logits.shape[:-1]) != lead:
+        raise ValueError(f"{who}: top_logits and top_idx must both be {lead + ('K',)}, got {tuple(top_logits.shape)} / {tuple(top_idx.shape)}")
+    if top_logits.device != logits.device or top_idx.device != logits.device:
+        raise ValueError(f"{who}: logits, top_logits and top_idx must be on one device")
+    L.dtype_code(logits, who), L.dtype_code(top_logits, who), L.ids_flag(top_idx, who)
+    if weights is not None:
+        if tuple(weights.shape) != lead:
+            raise ValueError(f"{who}: weights must be {lead}, got {tuple(weights.shape)}")
+        weights = weights.detach().to(device=logits.device, dtype=torch.float32).contiguous()
+    return _DistillFn.apply(logits, top_logits.detach().contiguous(), top_idx.contiguous(), weights, tau, reduction)
+
+
 def edge_weights(mask_np: np.ndarray, sigma_px: float = 3.0) -> np.ndarray:
     """Reference: solpex/losses.py:215-224.  Host-side (scipy), once per run."""
     from scipy.ndimage import binary_erosion, distance_transform_edt
