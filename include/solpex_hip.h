@@ -385,6 +385,27 @@ int sx_embedding_backward(int dtype, int64_t n, int64_t rows, int dim, const voi
                           float scale, void* dtable, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Low-rank adapters of many requests beside one shared projection.  Row t belongs to adapter a = ids[t] (outside [0, G): none).
+ *   y[t] = W x[t] + bias + scales[a] * B_a (A_a x[t]);  gradients with respect to x, A and B (W, bias and scales are constants)
+ * x (T, K), w (N, K), y / dy (T, N) with row strides in elements; A (G, r, K), B (G, N, r), dx (T, K), dA, dB contiguous; all of
+ * `dtype`.  bias [N] and scales [G] (fp32) may be NULL.  Sums in fp32, one rounding; the same bits on every run.
+ *   kept      : sx_adapter_kept_bytes, written by the forward call (rows in the order of their adapter, A x), read by the backward call.
+ *   workspace : sx_adapter_workspace_bytes, contents irrelevant before and after either call.  Both 16-byte aligned.
+ *   sx_adapter_backward: dx, dA, dB may each be NULL (not wanted); dA and dB are written whole (zeros where no row names the adapter).
+ * 1 <= r <= 128, 1 <= G <= 65535, T <= 2^24, K and N <= 2^20.
+ * --------------------------------------------------------------------------------------------- */
+int64_t sx_adapter_kept_bytes(int64_t T, int r, int G);
+int64_t sx_adapter_workspace_bytes(int dtype, int64_t T, int K, int N, int r, int G);
+int sx_adapter_forward(int dtype, int64_t T, int K, int N, int r, int G, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                       const void* bias, const void* A, const void* B, const float* scales, const void* ids, int ids64,
+                       void* y, int64_t ldy, void* kept, int64_t kept_bytes, void* workspace, int64_t workspace_bytes,
+                       void* stream);
+int sx_adapter_backward(int dtype, int64_t T, int K, int N, int r, int G, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                        const void* A, const void* B, const float* scales, const void* dy, int64_t lddy, const void* kept,
+                        int64_t kept_bytes, void* dx, void* dA, void* dB, void* workspace, int64_t workspace_bytes,
+                        void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Distillation from a teacher's top logits.  Row t: student logits z (V, `dtype`, row stride ld), K pairs (idx, top) of the
  * teacher (contiguous; top in top_dtype, idx int64 or int32); a pair whose index is outside [0, V) is ignored.
  *   p = softmax(top / tau) over the row's valid pairs, q = softmax(z / tau)

@@ -1,4 +1,4 @@
-"""CPU: what the scaled embedding, the distillation loss and their C entry points refuse, before anything reaches a GPU."""
+"""CPU: what the scaled embedding, the adapter projection, the distillation loss and their C entry points refuse, before anything reaches a GPU."""
 import ctypes
 
 import pytest
@@ -64,4 +64,37 @@ def test_distill_c_entry_refusals():
     def bwd(dt=0, V=10, ld=10, tau=1.0, stats=P, g=P, d=P, ldd=10, w=None, den=None):
         return lib.sx_distill_backward(dt, 3, V, 2, P, ld, 0, P, P, 1, tau, w, 1, stats, den, g, 0, 0, d, ldd, None)
     for kw in (dict(dt=5), dict(V=-1), dict(ld=9), dict(tau=-1.0), dict(stats=None), dict(g=None), dict(d=None), dict(ldd=9), dict(w=P)):
+        _bad(bwd(**kw))
+
+
+def test_adapter_refusals():
+    from unet_amd.adapters import adapter_linear
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        adapter_linear(torch.zeros(2, 8), torch.zeros(4, 8), None, torch.zeros(1, 2, 8), torch.zeros(1, 4, 2), torch.zeros(2, dtype=torch.int64))
+
+
+def test_adapter_c_entry_refusals():
+    from unet_amd import _lib as L
+    lib = L.lib()
+    nk, nw = lib.sx_adapter_kept_bytes(10, 4, 3), lib.sx_adapter_workspace_bytes(0, 10, 16, 8, 4, 3)
+    assert nk > 0 and nw > 0
+    for T, r, G in ((-1, 4, 3), ((1 << 24) + 1, 4, 3), (1, 0, 3), (1, 129, 3), (1, 4, 0), (1, 4, 65536)):
+        _bad(lib.sx_adapter_kept_bytes(T, r, G))
+        _bad(lib.sx_adapter_workspace_bytes(0, T, 16, 8, r, G))
+    for dt, K, N in ((2, 16, 8), (0, 0, 8), (0, 16, 0), (0, (1 << 20) + 1, 8), (1, 16, (1 << 20) + 1)):
+        _bad(lib.sx_adapter_workspace_bytes(dt, 10, K, N, 4, 3))
+
+    def fwd(dt=0, T=10, r=4, G=3, x=P, ldx=16, w=P, ldw=16, A=P, B=P, ids=P, y=P, ldy=8, kept=P, nk=nk, ws=P, nw=nw):
+        return lib.sx_adapter_forward(dt, T, 16, 8, r, G, x, ldx, w, ldw, None, A, B, None, ids, 1, y, ldy, kept, nk, ws, nw, None)
+    odd = ctypes.c_void_p(4100)
+    for kw in (dict(dt=9), dict(T=-5), dict(r=0), dict(r=200), dict(G=0), dict(x=None), dict(w=None), dict(A=None), dict(B=None), dict(ids=None),
+               dict(y=None), dict(kept=None), dict(ws=None), dict(ldx=15), dict(ldw=15), dict(ldy=7), dict(nk=nk - 1), dict(nw=nw - 1), dict(kept=odd),
+               dict(ws=odd)):
+        _bad(fwd(**kw))
+    assert fwd(T=0) == 0
+
+    def bwd(dt=0, T=10, x=P, ldx=16, w=P, ldw=16, A=P, B=P, dy=P, ldd=8, kept=P, nk=nk, ws=P, nw=nw):
+        return lib.sx_adapter_backward(dt, T, 16, 8, 4, 3, x, ldx, w, ldw, A, B, None, dy, ldd, kept, nk, P, P, P, ws, nw, None)
+    for kw in (dict(dt=9), dict(T=0), dict(x=None), dict(w=None), dict(A=None), dict(B=None), dict(dy=None), dict(kept=None), dict(ws=None), dict(ldx=15),
+               dict(ldw=15), dict(ldd=7), dict(nk=nk - 1), dict(nw=nw - 1), dict(kept=odd), dict(ws=odd)):
         _bad(bwd(**kw))

@@ -9,6 +9,7 @@ from .data import (MaskedLogStandardizer, MaskedLinearStandardizer, MaskedSymLog
 from .models import UNet, ParamToZ, bottleneck_to_z, z_to_bottleneck
 from .losses import edge_weights, masked_weighted_loss, mae_norm, batch_error_sums_ev, distillation_loss
 from .embedding import scaled_embedding, ScaledEmbedding
+from .adapters import adapter_linear, AdapterLinear
 from .train import train_unet, TrainEngine
 from .predict import load_checkpoint, predict_fields, predict_te, predict_fields_batch, scale_params
 from .utils import (pick_device, sample_from_loader, eval_param2z_one, nearest_neighbor_in_Z, scale_params_for_inference,
@@ -24,5 +25,6 @@ __all__ = [
     "masked_weighted_loss", "mae_norm", "batch_error_sums_ev", "train_unet", "TrainEngine", "load_checkpoint",
     "predict_fields", "predict_te", "predict_fields_batch", "scale_params", "pick_device", "sample_from_loader", "eval_param2z_one",
     "nearest_neighbor_in_Z", "scale_params_for_inference", "save_geometry_h5", "extract_z_dataset", "ZToParam", "train_param2z", "train_z2param",
-    "train_cycle_consistent", "ResidentLoader", "fp32_exact", "distillation_loss", "scaled_embedding", "ScaledEmbedding",
+    "train_cycle_consistent", "ResidentLoader", "fp32_exact", "distillation_loss", "scaled_embedding", "ScaledEmbedding", "adapter_linear",
+    "AdapterLinear",
 ]

@@ -93,6 +93,10 @@ SIGNATURES = {
     "sx_embedding_workspace_bytes": (_l, [_l, _l, _i]),
     "sx_embedding_forward": (_i, [_i, _l, _l, _i, _p, _l, _p, _i, _f, _p, _p]),
     "sx_embedding_backward": (_i, [_i, _l, _l, _i, _p, _l, _p, _i, _f, _p, _p, _l, _p]),
+    "sx_adapter_kept_bytes": (_l, [_l, _i, _i]),
+    "sx_adapter_workspace_bytes": (_l, [_i, _l, _i, _i, _i, _i]),
+    "sx_adapter_forward": (_i, [_i, _l, _i, _i, _i, _i, _p, _l, _p, _l, _p, _p, _p, _p, _p, _i, _p, _l, _p, _l, _p, _l, _p]),
+    "sx_adapter_backward": (_i, [_i, _l, _i, _i, _i, _i, _p, _l, _p, _l, _p, _p, _p, _p, _l, _p, _l, _p, _p, _p, _p, _l, _p]),
     "sx_distill_forward": (_i, [_i, _l, _i, _i, _p, _l, _i, _p, _p, _i, _f, _p, _i, _p, _p, _p, _p, _p, _l, _p]),
     "sx_distill_backward": (_i, [_i, _l, _i, _i, _p, _l, _i, _p, _p, _i, _f, _p, _i, _p, _p, _p, _l, _i, _p, _l, _p]),
     "sx_unet_num_params": (_i, [_D]),
