@@ -93,6 +93,12 @@ def test_larger_tiles(T, K, N, r, G, kind, dtype):
     _check(_inputs(T, K, N, r, G, dtype, kind))
 
 
+@pytest.mark.parametrize("T,K,N,r,G,kind", [(4100, 72, 4096, 20, 3, "random"), (4100, 4096, 72, 20, 3, "segments"), (4100, 264, 2048, 8, 40, "random"),
+                                            (4100, 2048, 264, 8, 40, "segments"), (4100, 328, 4096, 128, 2, "segments")])
+def test_largest_tiles(T, K, N, r, G, kind):
+    _check(_inputs(T, K, N, r, G, torch.bfloat16, kind))
+
+
 def test_rows_without_an_adapter():
     for dtype in (torch.float32, torch.bfloat16):
         y, dx, dA, dB = _check(_inputs(70, 40, 33, 6, 4, dtype, "none"))

@@ -76,25 +76,27 @@ def test_adapter_refusals():
 def test_adapter_c_entry_refusals():
     from unet_amd import _lib as L
     lib = L.lib()
-    nk, nw = lib.sx_adapter_kept_bytes(10, 4, 3), lib.sx_adapter_workspace_bytes(0, 10, 16, 8, 4, 3)
-    assert nk > 0 and nw > 0
+    nk, nw, nb = lib.sx_adapter_kept_bytes(0, 10, 4, 3), lib.sx_adapter_workspace_bytes(0, 10, 16, 8, 4, 3, 0), lib.sx_adapter_workspace_bytes(0, 10, 16, 8, 4, 3, 1)
+    assert nk > 0 and nw > 0 and nb > 0
     for T, r, G in ((-1, 4, 3), ((1 << 24) + 1, 4, 3), (1, 0, 3), (1, 129, 3), (1, 4, 0), (1, 4, 65536)):
-        _bad(lib.sx_adapter_kept_bytes(T, r, G))
-        _bad(lib.sx_adapter_workspace_bytes(0, T, 16, 8, r, G))
+        _bad(lib.sx_adapter_kept_bytes(0, T, r, G))
+        _bad(lib.sx_adapter_workspace_bytes(0, T, 16, 8, r, G, 0))
+    _bad(lib.sx_adapter_kept_bytes(4, 10, 4, 3))
+    _bad(lib.sx_adapter_workspace_bytes(1, 10, 1 << 20, 8, 4, 1000, 1))
     for dt, K, N in ((2, 16, 8), (0, 0, 8), (0, 16, 0), (0, (1 << 20) + 1, 8), (1, 16, (1 << 20) + 1)):
-        _bad(lib.sx_adapter_workspace_bytes(dt, 10, K, N, 4, 3))
+        _bad(lib.sx_adapter_workspace_bytes(dt, 10, K, N, 4, 3, 1))
 
     def fwd(dt=0, T=10, r=4, G=3, x=P, ldx=16, w=P, ldw=16, A=P, B=P, ids=P, y=P, ldy=8, kept=P, nk=nk, ws=P, nw=nw):
         return lib.sx_adapter_forward(dt, T, 16, 8, r, G, x, ldx, w, ldw, None, A, B, None, ids, 1, y, ldy, kept, nk, ws, nw, None)
     odd = ctypes.c_void_p(4100)
     for kw in (dict(dt=9), dict(T=-5), dict(r=0), dict(r=200), dict(G=0), dict(x=None), dict(w=None), dict(A=None), dict(B=None), dict(ids=None),
                dict(y=None), dict(kept=None), dict(ws=None), dict(ldx=15), dict(ldw=15), dict(ldy=7), dict(nk=nk - 1), dict(nw=nw - 1), dict(kept=odd),
-               dict(ws=odd)):
+               dict(ws=odd), dict(x=odd), dict(w=odd), dict(A=odd), dict(B=odd), dict(ldx=18), dict(ldw=17)):
         _bad(fwd(**kw))
     assert fwd(T=0) == 0
 
-    def bwd(dt=0, T=10, x=P, ldx=16, w=P, ldw=16, A=P, B=P, dy=P, ldd=8, kept=P, nk=nk, ws=P, nw=nw):
+    def bwd(dt=0, T=10, x=P, ldx=16, w=P, ldw=16, A=P, B=P, dy=P, ldd=8, kept=P, nk=nk, ws=P, nw=nb):
         return lib.sx_adapter_backward(dt, T, 16, 8, 4, 3, x, ldx, w, ldw, A, B, None, dy, ldd, kept, nk, P, P, P, ws, nw, None)
     for kw in (dict(dt=9), dict(T=0), dict(x=None), dict(w=None), dict(A=None), dict(B=None), dict(dy=None), dict(kept=None), dict(ws=None), dict(ldx=15),
-               dict(ldw=15), dict(ldd=7), dict(nk=nk - 1), dict(nw=nw - 1), dict(kept=odd), dict(ws=odd)):
+               dict(ldw=15), dict(ldd=7), dict(ldd=9), dict(dy=odd), dict(nk=nk - 1), dict(nw=nb - 1), dict(kept=odd), dict(ws=odd)):
         _bad(bwd(**kw))

@@ -93,8 +93,8 @@ SIGNATURES = {
     "sx_embedding_workspace_bytes": (_l, [_l, _l, _i]),
     "sx_embedding_forward": (_i, [_i, _l, _l, _i, _p, _l, _p, _i, _f, _p, _p]),
     "sx_embedding_backward": (_i, [_i, _l, _l, _i, _p, _l, _p, _i, _f, _p, _p, _l, _p]),
-    "sx_adapter_kept_bytes": (_l, [_l, _i, _i]),
-    "sx_adapter_workspace_bytes": (_l, [_i, _l, _i, _i, _i, _i]),
+    "sx_adapter_kept_bytes": (_l, [_i, _l, _i, _i]),
+    "sx_adapter_workspace_bytes": (_l, [_i, _l, _i, _i, _i, _i, _i]),
     "sx_adapter_forward": (_i, [_i, _l, _i, _i, _i, _i, _p, _l, _p, _l, _p, _p, _p, _p, _p, _i, _p, _l, _p, _l, _p, _l, _p]),
     "sx_adapter_backward": (_i, [_i, _l, _i, _i, _i, _i, _p, _l, _p, _l, _p, _p, _p, _p, _l, _p, _l, _p, _p, _p, _p, _l, _p]),
     "sx_distill_forward": (_i, [_i, _l, _i, _i, _p, _l, _i, _p, _p, _i, _f, _p, _i, _p, _p, _p, _p, _p, _l, _p]),
@@ -171,12 +171,23 @@ def ids_flag(t, who):
     return 1 if t.dtype == torch.int64 else 0
 
 
-def rows_2d(t, width):
-    """(..., width) tensor -> ((rows, width) tensor whose last dimension is contiguous, row stride); a copy only if it must be."""
-    t = t.reshape(-1, width) if width else t.reshape(0, 0)
+def rows_2d(t, width, aligned=False):
+    """(..., width) tensor -> ((rows, width) tensor whose last dimension is contiguous, row stride); a copy only if it must be.
+    aligned: rows of a whole number of 16-byte pieces also start on 16 bytes."""
+    t = t.reshape(-1, width)
     if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < width):
         t = t.contiguous()
-    return t, (int(t.stride(0)) if t.shape[0] > 1 else width)
+    ld = int(t.stride(0)) if t.shape[0] > 1 else width
+    if aligned:
+        e = 16 // t.element_size()
+        if width % e == 0 and (ld % e or t.data_ptr() % 16):
+            t, ld = torch_clone(t), width
+    return t, ld
+
+
+def torch_clone(t):
+    import torch
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def ptr_table(tensors):

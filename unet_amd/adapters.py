@@ -23,14 +23,14 @@ class _AdapterFn(torch.autograd.Function):
         N, K = weight.shape
         G, r = A.shape[:2]
         dt = L.dtype_code(x, "adapter_linear")
-        x2, ldx = L.rows_2d(x.detach(), K)
-        w, ldw = L.rows_2d(weight.detach(), K)
+        x2, ldx = L.rows_2d(x.detach(), K, aligned=True)
+        w, ldw = L.rows_2d(weight.detach(), K, aligned=True)
         T, dev = x2.shape[0], x.device
         i64 = L.ids_flag(ids, "adapter_linear")
-        Ad, Bd = A.detach().contiguous(), B.detach().contiguous()
+        Ad, Bd = L.rows_2d(A.detach().contiguous(), K, aligned=True)[0], L.rows_2d(B.detach().contiguous(), r, aligned=True)[0]
         y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=dev)
-        nk = L.check(lib.sx_adapter_kept_bytes(T, r, G), "sx_adapter_kept_bytes")
-        nw = L.check(lib.sx_adapter_workspace_bytes(dt, T, K, N, r, G), "sx_adapter_workspace_bytes")
+        nk = L.check(lib.sx_adapter_kept_bytes(dt, T, r, G), "sx_adapter_kept_bytes")
+        nw = L.check(lib.sx_adapter_workspace_bytes(dt, T, K, N, r, G, 0), "sx_adapter_workspace_bytes")
         kept = torch.empty(nk, dtype=torch.uint8, device=dev)
         ws = torch.empty(nw, dtype=torch.uint8, device=dev)
         with torch.cuda.device(dev):
@@ -59,9 +59,9 @@ class _AdapterFn(torch.autograd.Function):
             return dx, None, None, dA, dB, None, None
         x2, ldx = L.rows_2d(x.detach(), K)
         w, ldw = L.rows_2d(weight.detach(), K)
-        d2, ldd = L.rows_2d(dy, N)
+        d2, ldd = L.rows_2d(dy, N, aligned=True)
         Ad, Bd = A.detach().contiguous(), B.detach().contiguous()
-        nw = L.check(lib.sx_adapter_workspace_bytes(dt, T, K, N, r, G), "sx_adapter_workspace_bytes")
+        nw = L.check(lib.sx_adapter_workspace_bytes(dt, T, K, N, r, G, 1), "sx_adapter_workspace_bytes")
         ws = torch.empty(nw, dtype=torch.uint8, device=dev)
         with torch.cuda.device(dev):
             L.check(lib.sx_adapter_backward(dt, T, K, N, r, G, L.ptr(x2), ldx, L.ptr(w), ldw, L.ptr(Ad), L.ptr(Bd), L.ptr(scales), L.ptr(d2), ldd,

@@ -1,0 +1,49 @@
+// Shared by the kernels of the adapter projection (adapters.hip, adapter_tiles.hip, adapter_tokens.hip).
+#pragma once
+#include "sx_common.h"
+
+namespace sx {
+
+template <typename T> struct Mma;
+template <> struct Mma<bf16> {
+  static __device__ __forceinline__ f32x4 run(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mma<float> {      // lane (n, g) feeds k = 4 g + i in MFMA i, on both sides
+  static __device__ __forceinline__ f32x4 run(f32x4 a, f32x4 b, f32x4 c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// 16 bytes of a row from column c on, zeros from column C on (C a multiple of the piece, rows 16-byte aligned)
+template <typename T>
+__device__ __forceinline__ typename Elem<T>::Vec load_piece(const T* __restrict__ row, int c, int C) {
+  typename Elem<T>::Vec v = {};
+  if (c < C) v = *reinterpret_cast<const typename Elem<T>::Vec*>(row + c);
+  return v;
+}
+
+// h in fp32 as the MFMA's operand.  fp32: as it is.  bf16: 16 ranks are 16 hi parts, then 16 lo parts (h - hi): one K block of 32, whose
+// other side holds the 16 factors twice.  h loses 2^-17 of itself where one bf16 would cost 2^-9.
+__device__ __forceinline__ bf16 h_lo(float v) {
+  const float hi = (float)(bf16)v;
+  return fabsf(hi) == INFINITY ? (bf16)0.f : (bf16)(v - hi);
+}
+
+struct ProjectArgs {
+  const void* x; int64_t ldx;                 // T rows of K elements, by perm
+  const void* w; int64_t ldw;                 // N rows of K elements
+  const void* bias;                           // [N] or null
+  const void* q; int64_t q_g; int q_ld;       // Q(g, n, j) = q[g * q_g + n * q_ld + j], the adapter's second factor; zeros for j in [r, q_ld)
+  const void* h; int rp;                      // sorted rows: fp32 [T][rp], or bf16 [T][rp / 16][16 hi, 16 lo]
+  const int* perm; const int* key; const int* start;
+  int64_t T; int K, N, r, G;
+  void* y; int64_t ldy;
+};
+
+// the shared product on large bf16 tiles (adapter_tiles.hip); false: not for this kernel
+bool project_tiles_ok(const ProjectArgs& a);
+int project_tiles_launch(const ProjectArgs& a, hipStream_t st);
+
+}  // namespace sx

@@ -5,13 +5,15 @@
 //   dA_a  = sum_t dh[t] x[t]^T             dB_a = sum_t dy[t] h[t]^T          (W and b are frozen)
 //
 // The rows are taken in the order of their adapter (sort_ids.hip), so that a tile of rows meets few adapters and an adapter's
-// gradient is a sum over consecutive rows.  Three kernels serve both directions:
-//   shrink  h and dh: skinny products over the long dimension, kept in fp32, in sorted order
+// gradient is a sum over consecutive rows.  Four kernels serve both directions:
+//   pack    operands whose rows cannot be read 16 bytes at a time, and the transposed factors that the gradients multiply by, as
+//           rows of whole 16-byte pieces
+//   shrink  h and dh: skinny products over the long dimension, summed in fp32, in sorted order
 //   project y and dx: the shared product by tiles, and behind its last K step one more short step per adapter that the tile
-//           meets, with h (dh) as the left operand: the adapter's share goes through the same accumulators and is rounded
-//           once, with the product.  bf16 MFMA takes h as two bf16 parts, hi + lo, side by side in one K block of 32: an error of
-//           2^-17 of h where rounding h to bf16 alone would cost 2^-9.
+//           meets, with h (dh) as an operand: the adapter's share goes through the same accumulators and is rounded once, with
+//           the product.  bf16 MFMA takes h as two bf16 parts (adapters.h).
 //   outer   dA and dB: sums over an adapter's rows
+#include "adapters.h"
 #include "sort_ids.h"
 #include <algorithm>
 
@@ -19,120 +21,203 @@ namespace sx {
 
 constexpr int kMaxRank = 128;
 
-template <typename T> struct Mma;
-template <> struct Mma<bf16> {
-  static __device__ __forceinline__ f32x4 run(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+// ------------------------------------------------------------------ pack
+// dst[b][i][j] (row length ld, rows * ld elements per b) = src[b * s_b + i * s_i + j * s_j] for j < cols, 0 up to ld; one of s_i, s_j is 1
+struct PackJob {
+  const void* src; int64_t s_b, s_i, s_j;
+  void* dst; int ld, rows, cols, batch;
+  int ti, tj; int64_t first;                  // 64 x 64 tiles along i and j; the job's first tile
 };
-template <> struct Mma<float> {      // lane (n, g) feeds k = 4 g + i in MFMA i, on both sides
-  static __device__ __forceinline__ f32x4 run(f32x4 a, f32x4 b, f32x4 c) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
-    return c;
-  }
-};
+constexpr int kMaxJobs = 5;
+struct PackArgs { PackJob job[kMaxJobs]; int n; int64_t tiles; };
 
-// 16 bytes of a row from column c on, zeros from column C on; `vec`: 16-byte loads are possible and C is a multiple of them
-template <typename T, bool VEC>
-__device__ __forceinline__ typename Elem<T>::Vec load_piece(const T* __restrict__ row, int c, int C) {
-  typename Elem<T>::Vec v = {};
-  if constexpr (VEC) {
-    if (c < C) v = *reinterpret_cast<const typename Elem<T>::Vec*>(row + c);
-  } else {
-#pragma unroll
-    for (int i = 0; i < Elem<T>::EPL; ++i)
-      if (c + i < C) v[i] = row[c + i];
-  }
-  return v;
-}
-// the same from elements `stride` apart
 template <typename T>
-__device__ __forceinline__ typename Elem<T>::Vec gather_piece(const T* __restrict__ p, int64_t stride, int c, int C) {
-  typename Elem<T>::Vec v = {};
+__global__ __launch_bounds__(256) void adapter_pack_kernel(PackArgs a) {
+  typedef __attribute__((ext_vector_type(4))) T T4;
+  __shared__ __align__(16) T tile[64][64 + 2];
+  const int lx = threadIdx.x & 15, ly = threadIdx.x >> 4;
+  for (int64_t at = blockIdx.x; at < a.tiles; at += gridDim.x) {
+    PackJob j = a.job[0];
+    for (int k = 1; k < a.n; ++k)
+      if (at >= a.job[k].first) j = a.job[k];
+    int64_t t = at - j.first;
+    const int j0 = (int)(t % j.tj) * 64;
+    t /= j.tj;
+    const int i0 = (int)(t % j.ti) * 64;
+    const int64_t b = t / j.ti;
+    const T* src = (const T*)j.src + b * j.s_b;
+    T* dst = (T*)j.dst + b * j.rows * j.ld;
+    if (j.s_j != 1 || j.s_i == 1) {           // transposed: i runs along memory
+      const bool vec = j.s_j % 4 == 0 && j.s_b % 4 == 0 && (uintptr_t)j.src % (4 * sizeof(T)) == 0;
+      __syncthreads();                        // the tile before has been read
 #pragma unroll
-  for (int i = 0; i < Elem<T>::EPL; ++i)
-    if (c + i < C) v[i] = p[(c + i) * stride];
-  return v;
+      for (int k = 0; k < 4; ++k) {
+        const int jj = j0 + ly + 16 * k, i = i0 + lx * 4;
+        T4 v = {};
+        if (jj < j.cols) {
+          if (vec && i + 3 < j.rows) v = *reinterpret_cast<const T4*>(src + jj * j.s_j + i);
+          else
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (i + e < j.rows) v[e] = src[jj * j.s_j + i + e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) tile[ly + 16 * k][lx * 4 + e] = v[e];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = i0 + ly + 16 * k, jj = j0 + lx * 4;
+        T4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = tile[lx * 4 + e][ly + 16 * k];
+        if (i < j.rows && jj < j.ld) *reinterpret_cast<T4*>(dst + (int64_t)i * j.ld + jj) = v;      // ld is a multiple of 4
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = i0 + ly + 16 * k, jj = j0 + lx * 4;
+        if (i >= j.rows || jj >= j.ld) continue;
+        T4 v = {};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (jj + e < j.cols) v[e] = src[i * j.s_i + jj + e];
+        *reinterpret_cast<T4*>(dst + (int64_t)i * j.ld + jj) = v;
+      }
+    }
+  }
 }
+
+struct Packer {
+  PackArgs a = {};
+  void add(const void* src, int64_t s_b, int64_t s_i, int64_t s_j, void* dst, int ld, int rows, int cols, int batch) {
+    PackJob& j = a.job[a.n++];
+    j.src = src; j.s_b = s_b; j.s_i = s_i; j.s_j = s_j; j.dst = dst; j.ld = ld; j.rows = rows; j.cols = cols; j.batch = batch;
+    j.ti = cdiv(rows, 64); j.tj = cdiv(ld, 64); j.first = a.tiles;
+    a.tiles += (int64_t)j.ti * j.tj * batch;
+  }
+  template <typename T> int launch(hipStream_t st) {
+    if (!a.n) return SX_OK;
+    hipLaunchKernelGGL(adapter_pack_kernel<T>, dim3((unsigned)std::min<int64_t>(a.tiles, 1 << 16)), dim3(256), 0, st, a);
+    SX_LAUNCH_CHECK("adapter_pack");
+    return SX_OK;
+  }
+};
 
 // ------------------------------------------------------------------ shrink
 struct ShrinkArgs {
   const void* x; int64_t ldx;                 // rows of C elements
-  const void* p; int64_t p_g, p_j, p_c;       // P(g, j, c) = p[g * p_g + j * p_j + c * p_c]
+  const void* p; int64_t p_g; int p_ld;       // P(g, j, c) = p[g * p_g + j * p_ld + c]
   const float* scales;
   const int* perm; const int* key; const int* start;
   int64_t T; int C, r, G, rp;
-  float* h;                                   // [T][rp]
+  void* h;                                    // see ProjectArgs
+  bf16* ht; int64_t ldt;                      // bf16: [2][rp][ldt], hi and lo parts with the rows along memory; or null
 };
 
-// 16 sorted rows and 64 ranks per block; the four waves split the columns
-template <typename T, bool VEC, bool PC>
-__global__ __launch_bounds__(256) void adapter_shrink_kernel(ShrinkArgs a) {
-  constexpr int EPL = Elem<T>::EPL, CK = Elem<T>::CK;
+// MT * 16 sorted rows and RT * 16 ranks per block; its NW waves split the columns
+template <typename T, int MT, int RT, int NW>
+__global__ __launch_bounds__(64 * NW) void adapter_shrink_kernel(ShrinkArgs a) {
+  constexpr int EPL = Elem<T>::EPL, CK = Elem<T>::CK, RJ = RT * 16, U = 4;
   typedef typename Elem<T>::Vec Vec;
-  __shared__ float red[4][16][64 + 1];
+  __shared__ float red[NW][MT * 16][RJ + 1];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, n = lane & 15, gq = lane >> 4;
-  const int64_t m0 = blockIdx.x * 16ll;
-  const int j0 = blockIdx.y * 64;
-  const int rows = (int)std::min<int64_t>(16, a.T - m0);
-  const T* xr = (const T*)a.x + (int64_t)a.perm[m0 + std::min(n, rows - 1)] * a.ldx;
-  f32x4 tot[4] = {};
+  const int64_t m0 = blockIdx.x * (int64_t)(MT * 16);
+  const int j0 = blockIdx.y * RJ;
+  const int rows = (int)std::min<int64_t>(MT * 16, a.T - m0);
+  const T* xr[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) xr[i] = (const T*)a.x + (int64_t)a.perm[m0 + std::min(i * 16 + n, rows - 1)] * a.ldx + gq * EPL;
+  f32x4 tot[MT][RT] = {};
   for (int at = 0; at < rows;) {
     const int g = a.key[m0 + at];
     const int end = (int)std::min<int64_t>(rows, a.start[g + 1] - m0);
     if (g < a.G) {
-      const T* pg = (const T*)a.p + g * a.p_g;
-      f32x4 acc[4] = {};
-      for (int c0 = wid * CK; c0 < a.C; c0 += 4 * CK) {
-        const int c = c0 + gq * EPL;
-        const Vec xv = load_piece<T, VEC>(xr, c, a.C);
+      const T* pr[RT];                        // ranks past the last one read it again: their products are not stored
 #pragma unroll
-        for (int rt = 0; rt < 4; ++rt) {
-          const int j = j0 + rt * 16 + n;
-          if (j0 + rt * 16 >= a.r) continue;
-          Vec pv = {};
-          if (j < a.r) {
-            if constexpr (PC) pv = load_piece<T, VEC>(pg + j * a.p_j, c, a.C);
-            else pv = gather_piece<T>(pg + j * a.p_j, a.p_c, c, a.C);
-          }
-          acc[rt] = Mma<T>::run(xv, pv, acc[rt]);
+      for (int t = 0; t < RT; ++t) pr[t] = (const T*)a.p + g * a.p_g + (int64_t)std::min(j0 + t * 16 + n, a.r - 1) * a.p_ld + gq * EPL;
+      f32x4 acc[MT][RT] = {};
+      int c0 = wid * CK;
+      for (; c0 + (U - 1) * NW * CK + CK <= a.C; c0 += U * NW * CK) {
+        Vec xv[U][MT], pv[U][RT];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+          for (int i = 0; i < MT; ++i) xv[u][i] = *reinterpret_cast<const Vec*>(xr[i] + c0 + u * NW * CK);
+#pragma unroll
+          for (int t = 0; t < RT; ++t) pv[u][t] = *reinterpret_cast<const Vec*>(pr[t] + c0 + u * NW * CK);
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int t = 0; t < RT; ++t) acc[i][t] = Mma<T>::run(xv[u][i], pv[u][t], acc[i][t]);
+      }
+      for (; c0 < a.C; c0 += NW * CK) {
+        Vec xv[MT], pv[RT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) xv[i] = load_piece<T>(xr[i] - gq * EPL, c0 + gq * EPL, a.C);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) pv[t] = load_piece<T>(pr[t] - gq * EPL, c0 + gq * EPL, a.C);
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int t = 0; t < RT; ++t) acc[i][t] = Mma<T>::run(xv[i], pv[t], acc[i][t]);
       }
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (4 * gq + q >= at && 4 * gq + q < end)
+      for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int rt = 0; rt < 4; ++rt) tot[rt][q] = acc[rt][q];
+        for (int q = 0; q < 4; ++q)
+          if (i * 16 + 4 * gq + q >= at && i * 16 + 4 * gq + q < end)
+#pragma unroll
+            for (int t = 0; t < RT; ++t) tot[i][t][q] = acc[i][t][q];
     }
     at = end;
   }
 #pragma unroll
-  for (int rt = 0; rt < 4; ++rt)
+  for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) red[wid][4 * gq + q][rt * 16 + n] = tot[rt][q];
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) red[wid][i * 16 + 4 * gq + q][t * 16 + n] = tot[i][t][q];
   __syncthreads();
-  for (int i = tid; i < rows * 64; i += 256) {
-    const int m = i >> 6, j = i & 63;
-    if (j0 + j >= a.rp) continue;
+  auto value = [&](int m, int j) {
     const int g = a.key[m0 + m];
-    const float s = g < a.G ? (a.scales ? a.scales[g] : 1.f) : 0.f;
-    a.h[(m0 + m) * a.rp + j0 + j] = g < a.G ? s * (red[0][m][j] + red[1][m][j] + red[2][m][j] + red[3][m][j]) : 0.f;
+    if (g >= a.G || j0 + j >= a.r) return 0.f;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) v += red[w][m][j];
+    return a.scales ? a.scales[g] * v : v;
+  };
+  for (int i = tid; i < MT * 16 * RJ; i += 64 * NW) {
+    const int m = i / RJ, j = i % RJ;
+    if (m >= rows || j0 + j >= a.rp) continue;
+    const float v = value(m, j);
+    if constexpr (sizeof(T) == 2) {
+      bf16* h = (bf16*)a.h + (m0 + m) * (2 * a.rp) + (j0 + j) / 16 * 32 + (j & 15);
+      h[0] = (bf16)v;
+      h[16] = h_lo(v);
+    } else {
+      ((float*)a.h)[(m0 + m) * a.rp + j0 + j] = v;
+    }
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (!a.ht) return;
+    for (int i = tid; i < MT * 16 * RJ; i += 64 * NW) {
+      const int m = i % (MT * 16), j = i / (MT * 16);
+      if (m >= rows || j0 + j >= a.rp) continue;
+      const float v = value(m, j);
+      bf16* h = a.ht + (int64_t)(j0 + j) * a.ldt + m0 + m;
+      h[0] = (bf16)v;
+      h[a.rp * a.ldt] = h_lo(v);
+    }
   }
 }
 
-// ------------------------------------------------------------------ project
-struct ProjectArgs {
-  const void* x; int64_t ldx;                 // T rows of K elements, by perm
-  const void* w; int64_t ldw;                 // WT = false: N rows of K elements; true: K rows of N elements
-  const void* bias;                           // [N] or null
-  const void* q; int64_t q_g, q_n, q_j;       // Q(g, n, j), the adapter's second factor
-  const float* h; int rp;                     // [T][rp], sorted order
-  const int* perm; const int* key; const int* start;
-  int64_t T; int K, N, r, G;
-  void* y; int64_t ldy;
-};
-
+// ------------------------------------------------------------------ project (fp32, and bf16 operands of 2 GiB and more)
 // A block's tile is BM sorted rows x BN columns: four waves of (BM / 2) x (BN / 2), K steps of 128 bytes through LDS
-template <typename T, bool VEC, bool WT, int BM, int BN>
+template <typename T, int BM, int BN>
 __global__ __launch_bounds__(256) void adapter_project_kernel(ProjectArgs a) {
   constexpr int EPL = Elem<T>::EPL, CK = Elem<T>::CK, BK = 2 * CK, LD = BK + EPL;
   typedef typename Elem<T>::Vec Vec;
@@ -147,86 +232,62 @@ __global__ __launch_bounds__(256) void adapter_project_kernel(ProjectArgs a) {
   const T* w = (const T*)a.w;
   f32x4 acc[MI][NI] = {};
   constexpr int PA = BM * 8 / 256, PB = BN * 8 / 256;
-  const T* xrow[PA];
+  const T *xrow[PA], *wrow[PB];
 #pragma unroll
-  for (int i = 0; i < PA; ++i) {
-    const int64_t m = std::min<int64_t>(m0 + (i * 256 + tid) / 8, a.T - 1);
-    xrow[i] = x + (int64_t)a.perm[m] * a.ldx;
-  }
-  auto product = [&](int half) {
-    Vec av[MI], bv[NI];
+  for (int i = 0; i < PA; ++i) xrow[i] = x + (int64_t)a.perm[std::min<int64_t>(m0 + (i * 256 + tid) / 8, a.T - 1)] * a.ldx;
 #pragma unroll
-    for (int i = 0; i < MI; ++i) av[i] = *reinterpret_cast<const Vec*>(&As[wm + i * 16 + n][half * CK + gq * EPL]);
-#pragma unroll
-    for (int i = 0; i < NI; ++i) bv[i] = *reinterpret_cast<const Vec*>(&Bs[wn + i * 16 + n][half * CK + gq * EPL]);
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-      for (int j = 0; j < NI; ++j) acc[i][j] = Mma<T>::run(av[i], bv[j], acc[i][j]);
-  };
+  for (int i = 0; i < PB; ++i) wrow[i] = w + (int64_t)std::min(n0 + (i * 256 + tid) / 8, a.N - 1) * a.ldw;
   for (int k0 = 0; k0 < a.K; k0 += BK) {
     Vec ra[PA], rb[PB];
 #pragma unroll
-    for (int i = 0; i < PA; ++i) ra[i] = load_piece<T, VEC>(xrow[i], k0 + (tid & 7) * EPL, a.K);
+    for (int i = 0; i < PA; ++i) ra[i] = load_piece<T>(xrow[i], k0 + (tid & 7) * EPL, a.K);
 #pragma unroll
-    for (int i = 0; i < PB; ++i) {
-      const int p = i * 256 + tid;
-      if constexpr (WT) {
-        const int nn = std::min(n0 + p % BN, a.N - 1);
-        rb[i] = gather_piece<T>(w + nn, a.ldw, k0 + p / BN * EPL, a.K);
-      } else {
-        rb[i] = load_piece<T, VEC>(w + (int64_t)std::min(n0 + p / 8, a.N - 1) * a.ldw, k0 + (p & 7) * EPL, a.K);
-      }
-    }
+    for (int i = 0; i < PB; ++i) rb[i] = load_piece<T>(wrow[i], k0 + (tid & 7) * EPL, a.K);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < PA; ++i) *reinterpret_cast<Vec*>(&As[(i * 256 + tid) / 8][(tid & 7) * EPL]) = ra[i];
 #pragma unroll
-    for (int i = 0; i < PB; ++i) {
-      const int p = i * 256 + tid;
-      if constexpr (WT) *reinterpret_cast<Vec*>(&Bs[p % BN][p / BN * EPL]) = rb[i];
-      else *reinterpret_cast<Vec*>(&Bs[p / 8][(p & 7) * EPL]) = rb[i];
-    }
+    for (int i = 0; i < PB; ++i) *reinterpret_cast<Vec*>(&Bs[(i * 256 + tid) / 8][(tid & 7) * EPL]) = rb[i];
     __syncthreads();
-    product(0);
-    product(1);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      Vec av[MI], bv[NI];
+#pragma unroll
+      for (int i = 0; i < MI; ++i) av[i] = *reinterpret_cast<const Vec*>(&As[wm + i * 16 + n][half * CK + gq * EPL]);
+#pragma unroll
+      for (int i = 0; i < NI; ++i) bv[i] = *reinterpret_cast<const Vec*>(&Bs[wn + i * 16 + n][half * CK + gq * EPL]);
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) acc[i][j] = Mma<T>::run(av[i], bv[j], acc[i][j]);
+    }
   }
-  // the adapters that this tile's rows meet, 16 ranks at a time: fp32 one K block of 16; bf16 one of 32, 16 hi then 16 lo
+  // the adapters that this tile's rows meet, 16 ranks at a time
   const int rows = (int)std::min<int64_t>(BM, a.T - m0);
   for (int at = 0; at < rows;) {
     const int g = a.key[m0 + at];
     if (g >= a.G) break;                                  // the rows without an adapter come last
     const int end = (int)std::min<int64_t>(rows, a.start[g + 1] - m0);
+    const T* qg = (const T*)a.q + g * a.q_g;
     for (int j0 = 0; j0 < a.r; j0 += 16) {
-      __syncthreads();
-      for (int i = tid; i < BM * 16; i += 256) {
-        const int m = i >> 4, j = i & 15;
-        const float h = (m >= at && m < end) ? a.h[(m0 + m) * a.rp + j0 + j] : 0.f;
-        const T hi = from_f32<T>(h);
-        As[m][j] = hi;
-        if constexpr (CK == 32) As[m][16 + j] = from_f32<T>(fabsf(to_f32(hi)) == INFINITY ? 0.f : h - to_f32(hi));
-      }
-      for (int i = tid; i < BN * 16; i += 256) {
-        const int nn = a.q_n == 1 ? i % BN : i >> 4, j = a.q_n == 1 ? i / BN : i & 15;
-        const T v = (n0 + nn < a.N && j0 + j < a.r) ? ((const T*)a.q)[g * a.q_g + (n0 + nn) * a.q_n + (j0 + j) * a.q_j] : from_f32<T>(0.f);
-        Bs[nn][j] = v;
-        if constexpr (CK == 32) Bs[nn][16 + j] = v;
-      }
-      __syncthreads();
-      // only this adapter's rows take the product: a NaN or an infinity in its factors must not reach the others as 0 * NaN
+      const int jr = j0 + (sizeof(T) == 2 ? (gq & 1) * 8 : gq * 4);
+      Vec bv[NI];
+#pragma unroll
+      for (int j = 0; j < NI; ++j) bv[j] = load_piece<T>(qg + (int64_t)std::min(n0 + wn + j * 16 + n, a.N - 1) * a.q_ld, jr, a.q_ld);
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
         const int f = wm + i * 16;
         if (f >= end || f + 16 <= at) continue;
-        const Vec av = *reinterpret_cast<const Vec*>(&As[f + n][gq * EPL]);
+        const int64_t m = m0 + std::min(f + n, rows - 1);
+        const T* h = (const T*)a.h + (sizeof(T) == 2 ? m * (2 * a.rp) + j0 * 2 + gq * 8 : m * a.rp + j0 + gq * 4);
+        const Vec av = *reinterpret_cast<const Vec*>(h);
 #pragma unroll
-        for (int jj = 0; jj < NI; ++jj) {
-          const Vec bv = *reinterpret_cast<const Vec*>(&Bs[wn + jj * 16 + n][gq * EPL]);
+        for (int j = 0; j < NI; ++j) {
           const f32x4 z = {0.f, 0.f, 0.f, 0.f};
-          const f32x4 d = Mma<T>::run(av, bv, z);
+          const f32x4 d = Mma<T>::run(av, bv[j], z);
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (f + 4 * gq + q >= at && f + 4 * gq + q < end) acc[i][jj][q] += d[q];
+          for (int q = 0; q < 4; ++q)                     // only this adapter's rows: 0 * NaN must not reach the others
+            if (f + 4 * gq + q >= at && f + 4 * gq + q < end) acc[i][j][q] += d[q];
         }
       }
     }
@@ -248,188 +309,366 @@ __global__ __launch_bounds__(256) void adapter_project_kernel(ProjectArgs a) {
 }
 
 // ------------------------------------------------------------------ outer
+// out(g, j, c) = sum over the rows of adapter g of h[t][j] x[t][c]
+struct OuterJob {
+  const void* x; int64_t ldx; int C;          // rows of C elements, by perm
+  const void* h;                              // fp32: [T][rp]; bf16: the transposed parts [2][rp][ldt]; sorted rows
+  void* out; int64_t o_g, o_j, o_c;           // one of o_j and o_c is 1
+  int vec;                                    // 4 columns can be read at once
+  int cols, first;                            // 64-column blocks; the job's first block
+};
 struct OuterArgs {
-  const void* x; int64_t ldx;                 // rows of C elements, by perm
-  const float* h; int rp;                     // [T][rp], sorted order
+  OuterJob job[2]; int n;
   const int* perm; const int* start;
-  int C, r;
-  void* out; int64_t o_g, o_j, o_c;           // out(g, j, c)
+  int r, rp, G; int64_t ldt;
 };
 
-// out(g, j, c) = sum over the rows of adapter g of h[t][j] x[t][c]; 64 columns and 16 ranks per block, its waves split the rows
-template <typename T>
-__global__ __launch_bounds__(256) void adapter_outer_kernel(OuterArgs a) {
+__device__ __forceinline__ void outer_block(const OuterArgs& a, OuterJob& j, int& c0, int& g) {
+  j = a.n > 1 && (int)blockIdx.x >= a.job[1].first ? a.job[1] : a.job[0];
+  const int t = blockIdx.x - j.first;
+  c0 = t % j.cols * 64;
+  g = t / j.cols;
+}
+
+// fp32: 64 columns and 16 ranks per block, its waves split the rows
+__global__ __launch_bounds__(256) void adapter_outer_f32_kernel(OuterArgs a) {
   __shared__ float red[4][16][64];
+  OuterJob j;
+  int c0, g;
+  outer_block(a, j, c0, g);
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-  const int c = blockIdx.x * 64 + lane, j0 = blockIdx.y * 16, g = blockIdx.z;
+  const int c = c0 + lane, j0 = blockIdx.y * 16;
   const int t0 = a.start[g], t1 = a.start[g + 1];
   float acc[16] = {};
   for (int t = t0 + wid; t < t1; t += 4) {
-    const float xv = c < a.C ? to_f32(((const T*)a.x)[(int64_t)a.perm[t] * a.ldx + c]) : 0.f;
-    const float* h = a.h + (int64_t)t * a.rp + j0;
+    const float xv = c < j.C ? ((const float*)j.x)[(int64_t)a.perm[t] * j.ldx + c] : 0.f;
+    const float* h = (const float*)j.h + (int64_t)t * a.rp + j0;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) acc[j] = fmaf(h[j], xv, acc[j]);
+    for (int k = 0; k < 16; ++k) acc[k] = fmaf(h[k], xv, acc[k]);
   }
 #pragma unroll
-  for (int j = 0; j < 16; ++j) red[wid][j][lane] = acc[j];
+  for (int k = 0; k < 16; ++k) red[wid][k][lane] = acc[k];
   __syncthreads();
   for (int i = threadIdx.x; i < 16 * 64; i += 256) {
-    const int j = a.o_j == 1 ? i & 15 : i >> 6, cc = a.o_j == 1 ? i >> 4 : i & 63;
-    if (j0 + j < a.r && (int)blockIdx.x * 64 + cc < a.C)
-      ((T*)a.out)[g * a.o_g + (j0 + j) * a.o_j + ((int64_t)blockIdx.x * 64 + cc) * a.o_c] =
-          from_f32<T>(red[0][j][cc] + red[1][j][cc] + red[2][j][cc] + red[3][j][cc]);
+    const int k = j.o_j == 1 ? i & 15 : i >> 6, cc = j.o_j == 1 ? i >> 4 : i & 63;
+    if (j0 + k < a.r && c0 + cc < j.C)
+      ((float*)j.out)[g * j.o_g + (j0 + k) * j.o_j + (int64_t)(c0 + cc) * j.o_c] = red[0][k][cc] + red[1][k][cc] + red[2][k][cc] + red[3][k][cc];
+  }
+}
+
+// bf16: 64 columns and RT * 16 ranks per block; a wave takes every fourth block of 32 rows.  h comes with the rows along memory (16 bytes
+// = 8 rows of one rank); x comes as it lies, 4 columns of 8 rows per lane, and is turned in registers: fragment f holds columns 4 n + f.
+// 32-row blocks are aligned, so that h's 16-byte reads are: rows of other adapters in the first and last one are cleared on both
+// sides.
+template <int RT>
+__global__ __launch_bounds__(256) void adapter_outer_kernel(OuterArgs a) {
+  __shared__ float red[4][RT * 16][64 + 1];
+  OuterJob j;
+  int c0, g;
+  outer_block(a, j, c0, g);
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, n = lane & 15, gq = lane >> 4;
+  const int j0 = blockIdx.y * (RT * 16), c = c0 + 4 * n;
+  const int t0 = a.start[g], t1 = a.start[g + 1];
+  const bf16* x = (const bf16*)j.x;
+  const bf16* ht = (const bf16*)j.h;
+  f32x4 acc[RT][4] = {};
+  for (int tb = (t0 & ~31) + wid * 32; tb < t1; tb += 128) {
+    const int t = tb + gq * 8;
+    u32x4 lo, hi;                             // columns (0, 1) and (2, 3) of rows t + 2 e, t + 2 e + 1
+    uint32_t v[8][2];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[e][0] = v[e][1] = 0;
+      if (t + e >= t0 && t + e < t1) {
+        const bf16* p = x + (int64_t)a.perm[t + e] * j.ldx + c;
+        if (j.vec) {
+          if (c < j.C) {
+            const uint64_t q = *reinterpret_cast<const uint64_t*>(p);
+            v[e][0] = (uint32_t)q;
+            v[e][1] = (uint32_t)(q >> 32);
+          }
+        } else {
+          const uint16_t* p16 = reinterpret_cast<const uint16_t*>(p);
+          if (c < j.C) v[e][0] = p16[0];
+          if (c + 1 < j.C) v[e][0] |= (uint32_t)p16[1] << 16;
+          if (c + 2 < j.C) v[e][1] = p16[2];
+          if (c + 3 < j.C) v[e][1] |= (uint32_t)p16[3] << 16;
+        }
+      }
+    }
+    bf16x8 xf[4];
+#pragma unroll
+    for (int f = 0; f < 4; ++f) {
+      union { uint32_t u[4]; bf16x8 b; } w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t p = v[2 * e][f >> 1], q = v[2 * e + 1][f >> 1];
+        w.u[e] = f & 1 ? (p >> 16) | (q & 0xffff0000u) : (p & 0xffffu) | (q << 16);
+      }
+      xf[f] = w.b;
+    }
+    const bool whole = tb >= t0 && tb + 32 <= t1;
+#pragma unroll
+    for (int k = 0; k < RT; ++k) {
+      const bf16* h = ht + (int64_t)std::min(j0 + k * 16 + n, a.rp - 1) * a.ldt + t;
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        bf16x8 hv = *reinterpret_cast<const bf16x8*>(h + part * (int64_t)a.rp * a.ldt);
+        if (!whole)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (t + e < t0 || t + e >= t1) hv[e] = (bf16)0.f;
+#pragma unroll
+        for (int f = 0; f < 4; ++f) acc[k][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hv, xf[f], acc[k][f], 0, 0, 0);
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < RT; ++k)
+#pragma unroll
+    for (int f = 0; f < 4; ++f)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) red[wid][k * 16 + 4 * gq + q][4 * n + f] = acc[k][f][q];
+  __syncthreads();
+  for (int i = tid; i < RT * 16 * 64; i += 256) {
+    const int k = j.o_j == 1 ? i % (RT * 16) : i >> 6, cc = j.o_j == 1 ? i / (RT * 16) : i & 63;
+    if (j0 + k < a.r && c0 + cc < j.C)
+      ((bf16*)j.out)[g * j.o_g + (j0 + k) * j.o_j + (int64_t)(c0 + cc) * j.o_c] = (bf16)(red[0][k][cc] + red[1][k][cc] + red[2][k][cc] + red[3][k][cc]);
   }
 }
 
 // ------------------------------------------------------------------ host
-struct AdapterWs { size_t perm, key, start, h, total; };
-static AdapterWs adapter_ws(int64_t T, int r, int G) {
-  AdapterWs w;
+// kept: what a backward call needs of the forward one
+struct AdapterKept { size_t perm, key, start, h, ht, total; int rp; int64_t ldt; };
+static AdapterKept adapter_kept(int dtype, int64_t T, int r, int G) {
+  AdapterKept w;
   size_t o = 0;
+  w.rp = round_up(r, 16);
+  w.ldt = (int64_t)align_up((size_t)T, 64);
   w.perm = o; o = align_up(o + (size_t)T * 4, 256);
   w.key = o; o = align_up(o + (size_t)T * 4, 256);
   w.start = o; o = align_up(o + (size_t)(G + 2) * 4, 256);
-  w.h = o; o = align_up(o + (size_t)T * round_up(r, 16) * 4, 256);
+  w.h = o; o = align_up(o + (size_t)T * w.rp * 4, 256);
+  w.ht = o; o = align_up(o + (dtype == SX_BF16 ? (size_t)w.rp * w.ldt * 4 : 0), 256);
   w.total = o;
   return w;
 }
-static size_t adapter_dh_bytes(int64_t T, int r) { return align_up((size_t)T * round_up(r, 16) * 4, 256); }
+// sizes that rows of K elements lie in whole 16-byte pieces for; other ones are packed into rows that do
+static int padded(int dtype, int n) { return round_up(n, dtype == SX_BF16 ? 8 : 4); }
 
-template <typename T>
-static bool rows_vec(const void* p, int64_t ld, int C) {
-  constexpr int E = Elem<T>::EPL;
-  return C % E == 0 && ld % E == 0 && (uintptr_t)p % 16 == 0;
+struct AdapterWs { size_t x, w, A, B, dy, wt, at, bt, dh, dht, total; };
+static AdapterWs adapter_ws(int dtype, int64_t T, int K, int N, int r, int G, bool backward) {
+  const size_t e = dtype_size(dtype);
+  const int Kp = padded(dtype, K), Np = padded(dtype, N), r8 = padded(dtype, r);
+  AdapterWs w = {};
+  size_t o = 0;
+  auto take = [&](size_t& at, size_t elems, size_t size) { at = o; o = align_up(o + elems * size, 256); };
+  if (!backward) {
+    if (Kp != K) { take(w.x, (size_t)T * Kp, e); take(w.w, (size_t)N * Kp, e); take(w.A, (size_t)G * r * Kp, e); }
+    if (r8 != r) take(w.B, (size_t)G * N * r8, e);
+  } else {
+    const AdapterKept k = adapter_kept(dtype, T, r, G);
+    if (Np != N) take(w.dy, (size_t)T * Np, e);
+    take(w.wt, (size_t)K * Np, e);
+    take(w.at, (size_t)G * K * r8, e);
+    take(w.bt, (size_t)G * r * Np, e);
+    take(w.dh, (size_t)T * k.rp, 4);
+    if (dtype == SX_BF16) take(w.dht, (size_t)k.rp * k.ldt, 4);
+  }
+  w.total = std::max<size_t>(o, 256);
+  return w;
 }
 
 template <typename T>
 static int shrink_launch(const ShrinkArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)cdiv64(a.T, 16), cdiv(a.rp, 64));
-  const bool pc = a.p_c == 1;
-  const bool vec = rows_vec<T>(a.x, a.ldx, a.C) && (!pc || (rows_vec<T>(a.p, a.p_j, a.C) && a.p_g % Elem<T>::EPL == 0));
-  if (vec && pc) hipLaunchKernelGGL((adapter_shrink_kernel<T, true, true>), grid, dim3(256), 0, st, a);
-  else if (vec) hipLaunchKernelGGL((adapter_shrink_kernel<T, true, false>), grid, dim3(256), 0, st, a);
-  else if (pc) hipLaunchKernelGGL((adapter_shrink_kernel<T, false, true>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((adapter_shrink_kernel<T, false, false>), grid, dim3(256), 0, st, a);
+  // 32 rows share an adapter's factor once there are rows enough for two such blocks a CU; below, 16 rows and twice the waves
+  const bool big = a.T >= 32 * 512;
+  const int rt = a.rp <= 16 ? 1 : a.rp <= 32 ? 2 : 4;
+  const dim3 grid((unsigned)cdiv64(a.T, big ? 32 : 16), cdiv(a.rp, rt * 16));
+  if (big) {
+    if (rt == 1) hipLaunchKernelGGL((adapter_shrink_kernel<T, 2, 1, 4>), grid, dim3(256), 0, st, a);
+    else if (rt == 2) hipLaunchKernelGGL((adapter_shrink_kernel<T, 2, 2, 4>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((adapter_shrink_kernel<T, 2, 4, 4>), grid, dim3(256), 0, st, a);
+  } else {
+    if (rt == 1) hipLaunchKernelGGL((adapter_shrink_kernel<T, 1, 1, 8>), grid, dim3(512), 0, st, a);
+    else if (rt == 2) hipLaunchKernelGGL((adapter_shrink_kernel<T, 1, 2, 8>), grid, dim3(512), 0, st, a);
+    else hipLaunchKernelGGL((adapter_shrink_kernel<T, 1, 4, 8>), grid, dim3(512), 0, st, a);
+  }
   SX_LAUNCH_CHECK("adapter_shrink");
   return SX_OK;
 }
 
-template <typename T, bool WT>
+template <typename T>
 static int project_launch(const ProjectArgs& a, hipStream_t st) {
-  const bool vec = rows_vec<T>(a.x, a.ldx, a.K) && (WT || rows_vec<T>(a.w, a.ldw, a.K));
-  const bool big = a.T >= 512 && a.N >= 512;
-  const int b = big ? 128 : 64;
-  const dim3 grid((unsigned)cdiv64(a.T, b), cdiv(a.N, b));
-  if (big && vec) hipLaunchKernelGGL((adapter_project_kernel<T, true, WT, 128, 128>), grid, dim3(256), 0, st, a);
-  else if (big) hipLaunchKernelGGL((adapter_project_kernel<T, false, WT, 128, 128>), grid, dim3(256), 0, st, a);
-  else if (vec) hipLaunchKernelGGL((adapter_project_kernel<T, true, WT, 64, 64>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((adapter_project_kernel<T, false, WT, 64, 64>), grid, dim3(256), 0, st, a);
+  if (sizeof(T) == 2 && project_tiles_ok(a)) return project_tiles_launch(a, st);
+  if (cdiv64(a.T, 128) * cdiv(a.N, 128) >= 256) {
+    hipLaunchKernelGGL((adapter_project_kernel<T, 128, 128>), dim3((unsigned)cdiv64(a.T, 128), cdiv(a.N, 128)), dim3(256), 0, st, a);
+  } else {
+    hipLaunchKernelGGL((adapter_project_kernel<T, 64, 64>), dim3((unsigned)cdiv64(a.T, 64), cdiv(a.N, 64)), dim3(256), 0, st, a);
+  }
   SX_LAUNCH_CHECK("adapter_project");
   return SX_OK;
 }
 
 template <typename T>
-static int outer_launch(const OuterArgs& a, int G, hipStream_t st) {
-  hipLaunchKernelGGL(adapter_outer_kernel<T>, dim3(cdiv(a.C, 64), cdiv(a.r, 16), G), dim3(256), 0, st, a);
+static int outer_launch(OuterArgs a, hipStream_t st) {
+  int blocks = 0;
+  for (int i = 0; i < a.n; ++i) {
+    a.job[i].cols = cdiv(a.job[i].C, 64);
+    a.job[i].first = blocks;
+    a.job[i].vec = a.job[i].C % 4 == 0 && a.job[i].ldx % 4 == 0 && (uintptr_t)a.job[i].x % 8 == 0;
+    blocks += a.job[i].cols * a.G;
+  }
+  if (!blocks) return SX_OK;
+  if (sizeof(T) == 4) hipLaunchKernelGGL(adapter_outer_f32_kernel, dim3(blocks, cdiv(a.r, 16)), dim3(256), 0, st, a);
+  else if (a.rp <= 16) hipLaunchKernelGGL(adapter_outer_kernel<1>, dim3(blocks, 1), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL(adapter_outer_kernel<2>, dim3(blocks, cdiv(a.rp, 32)), dim3(256), 0, st, a);
   SX_LAUNCH_CHECK("adapter_outer");
   return SX_OK;
 }
 
+struct AdapterCall {
+  int dtype; int64_t T; int K, N, r, G;
+  const void* x; int64_t ldx;
+  const void* w; int64_t ldw;
+  const void *bias, *A, *B;
+  const float* scales;
+};
+
 template <typename T>
-static int adapter_forward(int64_t Tn, int K, int N, int r, int G, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
-                           const void* A, const void* B, const float* scales, const void* ids, int ids64, void* y, int64_t ldy, char* ws, hipStream_t st) {
-  const AdapterWs o = adapter_ws(Tn, r, G);
-  int *perm = (int*)(ws + o.perm), *key = (int*)(ws + o.key), *start = (int*)(ws + o.start);
-  float* h = (float*)(ws + o.h);
-  SX_TRY(launch_sort_ids(ids, ids64, Tn, G, perm, key, start, st));
+static int adapter_forward(const AdapterCall& c, const void* ids, int ids64, void* y, int64_t ldy, char* kept, char* ws, hipStream_t st) {
+  const AdapterKept k = adapter_kept(c.dtype, c.T, c.r, c.G);
+  const AdapterWs o = adapter_ws(c.dtype, c.T, c.K, c.N, c.r, c.G, false);
+  const int Kp = padded(c.dtype, c.K), r8 = padded(c.dtype, c.r);
+  int *perm = (int*)(kept + k.perm), *key = (int*)(kept + k.key), *start = (int*)(kept + k.start);
+  const void *x = c.x, *w = c.w, *A = c.A, *B = c.B;
+  int64_t ldx = c.ldx, ldw = c.ldw;
+  Packer pk;
+  if (Kp != c.K) {
+    pk.add(c.x, 0, c.ldx, 1, ws + o.x, Kp, (int)c.T, c.K, 1);
+    pk.add(c.w, 0, c.ldw, 1, ws + o.w, Kp, c.N, c.K, 1);
+    pk.add(c.A, 0, c.K, 1, ws + o.A, Kp, c.G * c.r, c.K, 1);
+    x = ws + o.x; w = ws + o.w; A = ws + o.A; ldx = ldw = Kp;
+  }
+  if (r8 != c.r) {
+    pk.add(c.B, (int64_t)c.N * c.r, c.r, 1, ws + o.B, r8, c.N, c.r, c.G);
+    B = ws + o.B;
+  }
+  SX_TRY(pk.launch<T>(st));
+  SX_TRY(launch_sort_ids(ids, ids64, c.T, c.G, perm, key, start, st));
   ShrinkArgs s = {};
-  s.x = x; s.ldx = ldx; s.p = A; s.p_g = (int64_t)r * K; s.p_j = K; s.p_c = 1; s.scales = scales; s.perm = perm; s.key = key; s.start = start;
-  s.T = Tn; s.C = K; s.r = r; s.G = G; s.rp = round_up(r, 16); s.h = h;
+  s.x = x; s.ldx = ldx; s.p = A; s.p_g = (int64_t)c.r * Kp; s.p_ld = Kp; s.scales = c.scales; s.perm = perm; s.key = key; s.start = start;
+  s.T = c.T; s.C = Kp; s.r = c.r; s.G = c.G; s.rp = k.rp; s.h = kept + k.h; s.ht = sizeof(T) == 2 ? (bf16*)(kept + k.ht) : nullptr; s.ldt = k.ldt;
   SX_TRY(shrink_launch<T>(s, st));
   ProjectArgs p = {};
-  p.x = x; p.ldx = ldx; p.w = w; p.ldw = ldw; p.bias = bias; p.q = B; p.q_g = (int64_t)N * r; p.q_n = r; p.q_j = 1; p.h = h; p.rp = s.rp;
-  p.perm = perm; p.key = key; p.start = start; p.T = Tn; p.K = K; p.N = N; p.r = r; p.G = G; p.y = y; p.ldy = ldy;
-  return project_launch<T, false>(p, st);
+  p.x = x; p.ldx = ldx; p.w = w; p.ldw = ldw; p.bias = c.bias; p.q = B; p.q_g = (int64_t)c.N * r8; p.q_ld = r8; p.h = kept + k.h; p.rp = k.rp;
+  p.perm = perm; p.key = key; p.start = start; p.T = c.T; p.K = Kp; p.N = c.N; p.r = c.r; p.G = c.G; p.y = y; p.ldy = ldy;
+  return project_launch<T>(p, st);
 }
 
 template <typename T>
-static int adapter_backward(int64_t Tn, int K, int N, int r, int G, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* A, const void* B,
-                            const float* scales, const void* dy, int64_t lddy, const char* kept, void* dx, void* dA, void* dB, char* ws, hipStream_t st) {
-  const AdapterWs o = adapter_ws(Tn, r, G);
-  const int *perm = (const int*)(kept + o.perm), *key = (const int*)(kept + o.key), *start = (const int*)(kept + o.start);
-  const float* h = (const float*)(kept + o.h);
-  float* dh = (float*)ws;
-  const int rp = round_up(r, 16);
+static int adapter_backward(const AdapterCall& c, const void* dy, int64_t lddy, const char* kept, void* dx, void* dA, void* dB, char* ws, hipStream_t st) {
+  const AdapterKept k = adapter_kept(c.dtype, c.T, c.r, c.G);
+  const AdapterWs o = adapter_ws(c.dtype, c.T, c.K, c.N, c.r, c.G, true);
+  const int Np = padded(c.dtype, c.N), r8 = padded(c.dtype, c.r);
+  const int *perm = (const int*)(kept + k.perm), *key = (const int*)(kept + k.key), *start = (const int*)(kept + k.start);
+  Packer pk;
+  const void* d = dy;
+  int64_t ldd = lddy;
+  if (Np != c.N) {
+    pk.add(dy, 0, lddy, 1, ws + o.dy, Np, (int)c.T, c.N, 1);
+    d = ws + o.dy;
+    ldd = Np;
+  }
+  if (dx || dA) pk.add(c.B, (int64_t)c.N * c.r, 1, c.r, ws + o.bt, Np, c.r, c.N, c.G);
+  if (dx) {
+    pk.add(c.w, 0, 1, c.ldw, ws + o.wt, Np, c.K, c.N, 1);
+    pk.add(c.A, (int64_t)c.r * c.K, 1, c.K, ws + o.at, r8, c.K, c.r, c.G);
+  }
+  SX_TRY(pk.launch<T>(st));
+  bf16* dht = sizeof(T) == 2 ? (bf16*)(ws + o.dht) : nullptr;
   if (dx || dA) {
     ShrinkArgs s = {};
-    s.x = dy; s.ldx = lddy; s.p = B; s.p_g = (int64_t)N * r; s.p_j = 1; s.p_c = r; s.scales = scales; s.perm = perm; s.key = key; s.start = start;
-    s.T = Tn; s.C = N; s.r = r; s.G = G; s.rp = rp; s.h = dh;
+    s.x = d; s.ldx = ldd; s.p = ws + o.bt; s.p_g = (int64_t)c.r * Np; s.p_ld = Np; s.scales = c.scales; s.perm = perm; s.key = key; s.start = start;
+    s.T = c.T; s.C = Np; s.r = c.r; s.G = c.G; s.rp = k.rp; s.h = ws + o.dh; s.ht = dht; s.ldt = k.ldt;
     SX_TRY(shrink_launch<T>(s, st));
   }
   if (dx) {
     ProjectArgs p = {};
-    p.x = dy; p.ldx = lddy; p.w = w; p.ldw = ldw; p.q = A; p.q_g = (int64_t)r * K; p.q_n = 1; p.q_j = K; p.h = dh; p.rp = rp;
-    p.perm = perm; p.key = key; p.start = start; p.T = Tn; p.K = N; p.N = K; p.r = r; p.G = G; p.y = dx; p.ldy = K;
-    SX_TRY((project_launch<T, true>(p, st)));
+    p.x = d; p.ldx = ldd; p.w = ws + o.wt; p.ldw = Np; p.q = ws + o.at; p.q_g = (int64_t)c.K * r8; p.q_ld = r8; p.h = ws + o.dh; p.rp = k.rp;
+    p.perm = perm; p.key = key; p.start = start; p.T = c.T; p.K = Np; p.N = c.K; p.r = c.r; p.G = c.G; p.y = dx; p.ldy = c.K;
+    SX_TRY(project_launch<T>(p, st));
   }
   OuterArgs q = {};
-  q.perm = perm; q.start = start; q.r = r; q.rp = rp;
+  q.perm = perm; q.start = start; q.r = c.r; q.rp = k.rp; q.G = c.G; q.ldt = k.ldt;
   if (dA) {
-    q.x = x; q.ldx = ldx; q.h = dh; q.C = K; q.out = dA; q.o_g = (int64_t)r * K; q.o_j = K; q.o_c = 1;
-    SX_TRY(outer_launch<T>(q, G, st));
+    OuterJob& j = q.job[q.n++];
+    j.x = c.x; j.ldx = c.ldx; j.C = c.K; j.h = sizeof(T) == 2 ? (const void*)dht : ws + o.dh; j.out = dA; j.o_g = (int64_t)c.r * c.K; j.o_j = c.K; j.o_c = 1;
   }
   if (dB) {
-    q.x = dy; q.ldx = lddy; q.h = h; q.C = N; q.out = dB; q.o_g = (int64_t)N * r; q.o_j = 1; q.o_c = r;
-    SX_TRY(outer_launch<T>(q, G, st));
+    OuterJob& j = q.job[q.n++];
+    j.x = d; j.ldx = ldd; j.C = c.N; j.h = kept + (sizeof(T) == 2 ? k.ht : k.h); j.out = dB; j.o_g = (int64_t)c.N * c.r; j.o_j = 1; j.o_c = c.r;
   }
-  return SX_OK;
+  return outer_launch<T>(q, st);
 }
 
 static int adapter_check(const char* who, int dtype, int64_t T, int K, int N, int r, int G) {
   SX_REQUIRE(dtype == SX_F32 || dtype == SX_BF16, "%s: dtype %d is neither fp32 nor bf16", who, dtype);
   SX_REQUIRE(T >= 0 && T <= (1 << 24) && K > 0 && N > 0 && K <= (1 << 20) && N <= (1 << 20), "%s: bad sizes T=%lld K=%d N=%d", who, (long long)T, K, N);
+  SX_REQUIRE((int64_t)G * std::max(K, N) <= (1 << 29), "%s: %d adapters of K=%d, N=%d: more than 2^29 rows", who, G, K, N);
   SX_REQUIRE(r >= 1 && r <= kMaxRank && G >= 1 && G <= 65535, "%s: rank %d must be 1..%d and the adapters %d 1..65535", who, r, kMaxRank, G);
   return SX_OK;
+}
+
+// rows of C elements that are read 16 bytes at a time; where C is no multiple of that, they are packed first and may lie anywhere
+static bool rows_ok(int dtype, const void* p, int64_t ld, int C) {
+  const int e = dtype == SX_BF16 ? 8 : 4;
+  return ld >= C && (C % e != 0 || (ld % e == 0 && (uintptr_t)p % 16 == 0));
 }
 
 }  // namespace sx
 
 using namespace sx;
 
-extern "C" int64_t sx_adapter_kept_bytes(int64_t T, int r, int G) {
-  SX_TRY(adapter_check("sx_adapter_kept_bytes", SX_F32, T, 1, 1, r, G));
-  return (int64_t)adapter_ws(T, r, G).total;
+extern "C" int64_t sx_adapter_kept_bytes(int dtype, int64_t T, int r, int G) {
+  SX_TRY(adapter_check("sx_adapter_kept_bytes", dtype, T, 1, 1, r, G));
+  return (int64_t)adapter_kept(dtype, T, r, G).total;
 }
 
-extern "C" int64_t sx_adapter_workspace_bytes(int dtype, int64_t T, int K, int N, int r, int G) {
+extern "C" int64_t sx_adapter_workspace_bytes(int dtype, int64_t T, int K, int N, int r, int G, int backward) {
   SX_TRY(adapter_check("sx_adapter_workspace_bytes", dtype, T, K, N, r, G));
-  return (int64_t)std::max<size_t>(adapter_dh_bytes(T, r), 256);
+  return (int64_t)adapter_ws(dtype, T, K, N, r, G, backward != 0).total;
 }
 
 extern "C" int sx_adapter_forward(int dtype, int64_t T, int K, int N, int r, int G, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
                                   const void* A, const void* B, const float* scales, const void* ids, int ids64, void* y, int64_t ldy, void* kept,
                                   int64_t kept_bytes, void* workspace, int64_t workspace_bytes, void* stream) {
   SX_TRY(adapter_check("sx_adapter_forward", dtype, T, K, N, r, G));
-  SX_REQUIRE(ldx >= K && ldw >= K && ldy >= N, "sx_adapter_forward: row strides %lld, %lld, %lld for K=%d, N=%d", (long long)ldx, (long long)ldw, (long long)ldy, K, N);
   if (T == 0) return SX_OK;
   SX_REQUIRE(x && w && A && B && ids && y && kept && workspace, "sx_adapter_forward: null pointer");
-  SX_REQUIRE(kept_bytes >= (int64_t)adapter_ws(T, r, G).total && (uintptr_t)kept % 16 == 0 && workspace_bytes >= sx_adapter_workspace_bytes(dtype, T, K, N, r, G) &&
-                 (uintptr_t)workspace % 16 == 0, "sx_adapter_forward: kept or workspace too small or not 16-byte aligned");
-  hipStream_t st = (hipStream_t)stream;
-  if (dtype == SX_BF16) return adapter_forward<bf16>(T, K, N, r, G, x, ldx, w, ldw, bias, A, B, scales, ids, ids64, y, ldy, (char*)kept, st);
-  return adapter_forward<float>(T, K, N, r, G, x, ldx, w, ldw, bias, A, B, scales, ids, ids64, y, ldy, (char*)kept, st);
+  SX_REQUIRE(rows_ok(dtype, x, ldx, K) && rows_ok(dtype, w, ldw, K) && rows_ok(dtype, A, K, K) && rows_ok(dtype, B, r, r) && ldy >= N,
+             "sx_adapter_forward: rows of x, w, A (K=%d) or B (r=%d) shorter than that or not 16-byte aligned (ldx=%lld ldw=%lld ldy=%lld)", K, r,
+             (long long)ldx, (long long)ldw, (long long)ldy);
+  SX_REQUIRE(kept_bytes >= (int64_t)adapter_kept(dtype, T, r, G).total && (uintptr_t)kept % 16 == 0 &&
+                 workspace_bytes >= (int64_t)adapter_ws(dtype, T, K, N, r, G, false).total && (uintptr_t)workspace % 16 == 0,
+             "sx_adapter_forward: kept or workspace too small or not 16-byte aligned");
+  const AdapterCall c = {dtype, T, K, N, r, G, x, ldx, w, ldw, bias, A, B, scales};
+  return dtype == SX_BF16 ? adapter_forward<bf16>(c, ids, ids64, y, ldy, (char*)kept, (char*)workspace, (hipStream_t)stream)
+                          : adapter_forward<float>(c, ids, ids64, y, ldy, (char*)kept, (char*)workspace, (hipStream_t)stream);
 }
 
 extern "C" int sx_adapter_backward(int dtype, int64_t T, int K, int N, int r, int G, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* A,
                                    const void* B, const float* scales, const void* dy, int64_t lddy, const void* kept, int64_t kept_bytes, void* dx, void* dA,
                                    void* dB, void* workspace, int64_t workspace_bytes, void* stream) {
   SX_TRY(adapter_check("sx_adapter_backward", dtype, T, K, N, r, G));
-  SX_REQUIRE(ldx >= K && ldw >= K && lddy >= N, "sx_adapter_backward: row strides %lld, %lld, %lld for K=%d, N=%d", (long long)ldx, (long long)ldw, (long long)lddy, K, N);
   SX_REQUIRE(T > 0, "sx_adapter_backward: T must be positive");
   SX_REQUIRE(x && w && A && B && dy && kept && workspace, "sx_adapter_backward: null pointer");
-  SX_REQUIRE(kept_bytes >= (int64_t)adapter_ws(T, r, G).total && (uintptr_t)kept % 16 == 0 && workspace_bytes >= sx_adapter_workspace_bytes(dtype, T, K, N, r, G) &&
-                 (uintptr_t)workspace % 16 == 0, "sx_adapter_backward: kept or workspace too small or not 16-byte aligned");
-  hipStream_t st = (hipStream_t)stream;
-  if (dtype == SX_BF16) return adapter_backward<bf16>(T, K, N, r, G, x, ldx, w, ldw, A, B, scales, dy, lddy, (const char*)kept, dx, dA, dB, (char*)workspace, st);
-  return adapter_backward<float>(T, K, N, r, G, x, ldx, w, ldw, A, B, scales, dy, lddy, (const char*)kept, dx, dA, dB, (char*)workspace, st);
+  SX_REQUIRE(ldx >= K && ldw >= K && rows_ok(dtype, dy, lddy, N), "sx_adapter_backward: rows of x, w (K=%d) or dy (N=%d) shorter than that or dy not 16-byte aligned (ldx=%lld ldw=%lld lddy=%lld)",
+             K, N, (long long)ldx, (long long)ldw, (long long)lddy);
+  SX_REQUIRE(kept_bytes >= (int64_t)adapter_kept(dtype, T, r, G).total && (uintptr_t)kept % 16 == 0 &&
+                 workspace_bytes >= (int64_t)adapter_ws(dtype, T, K, N, r, G, true).total && (uintptr_t)workspace % 16 == 0,
+             "sx_adapter_backward: kept or workspace too small or not 16-byte aligned");
+  const AdapterCall c = {dtype, T, K, N, r, G, x, ldx, w, ldw, nullptr, A, B, scales};
+  return dtype == SX_BF16 ? adapter_backward<bf16>(c, dy, lddy, (const char*)kept, dx, dA, dB, (char*)workspace, (hipStream_t)stream)
+                          : adapter_backward<float>(c, dy, lddy, (const char*)kept, dx, dA, dB, (char*)workspace, (hipStream_t)stream);
 }
