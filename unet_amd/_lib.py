@@ -174,10 +174,13 @@ def ids_flag(t, who):
 def rows_2d(t, width, aligned=False):
     """(..., width) tensor -> ((rows, width) tensor whose last dimension is contiguous, row stride); a copy only if it must be.
     aligned: rows of a whole number of 16-byte pieces also start on 16 bytes."""
-    t = t.reshape(-1, width)
-    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < width):
-        t = t.contiguous()
-    ld = int(t.stride(0)) if t.shape[0] > 1 else width
+    if t.dim() != 2:
+        t = t.reshape(-1, width)
+    rows, (ld, last) = t.shape[0], t.stride()
+    if (last != 1 and width > 1) or (rows > 1 and ld < width):
+        t, ld = t.contiguous(), width
+    elif rows <= 1:
+        ld = width
     if aligned:
         e = 16 // t.element_size()
         if width % e == 0 and (ld % e or t.data_ptr() % 16):
@@ -188,6 +191,29 @@ def rows_2d(t, width, aligned=False):
 def torch_clone(t):
     import torch
     return t.clone(memory_format=torch.contiguous_format)
+
+
+def addr(t):
+    """Device address of a tensor as an int (None stays None): what a c_void_p argument takes without an object around it."""
+    return None if t is None else t.data_ptr()
+
+
+def launch(name, device, *args):
+    """Call the entry point `name` with `args` and, behind them, the current stream of `device`, with that device current."""
+    import torch
+    fn = getattr(_lib or lib(), name)
+    i = device.index
+    if torch._C._cuda_getDevice() == i:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    else:
+        with torch.cuda.device(i):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    return rc if rc >= 0 else check(rc, name)
+
+
+def wants_grad(*tensors):
+    import torch
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def ptr_table(tensors):

@@ -16,57 +16,62 @@ from . import _lib as L
 MAX_RANK = 128
 
 
+def _factors(A, B):
+    return L.rows_2d(A.contiguous(), A.shape[2], aligned=True)[0], L.rows_2d(B.contiguous(), B.shape[2], aligned=True)[0]
+
+
+def _project(x, weight, bias, A, B, ids, scales):
+    """(y, what the backward pass needs of it)"""
+    lib = L.lib()
+    N, K = weight.shape
+    G, r = A.shape[:2]
+    dt, dev = L.dtype_code(x, "adapter_linear"), x.device
+    x2, ldx = L.rows_2d(x, K, aligned=True)
+    w, ldw = L.rows_2d(weight, K, aligned=True)
+    T = x2.shape[0]
+    Ad, Bd = _factors(A, B)
+    y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=dev)
+    nk = L.check(lib.sx_adapter_kept_bytes(dt, T, r, G), "sx_adapter_kept_bytes")
+    nw = L.check(lib.sx_adapter_workspace_bytes(dt, T, K, N, r, G, 0), "sx_adapter_workspace_bytes")
+    kept = torch.empty(nk, dtype=torch.uint8, device=dev)
+    ws = torch.empty(nw, dtype=torch.uint8, device=dev)
+    L.launch("sx_adapter_forward", dev, dt, T, K, N, r, G, L.addr(x2), ldx, L.addr(w), ldw, L.addr(bias), L.addr(Ad), L.addr(Bd), L.addr(scales),
+             L.addr(ids), L.ids_flag(ids, "adapter_linear"), L.addr(y), N, L.addr(kept), nk, L.addr(ws), nw)
+    return y, kept
+
+
 class _AdapterFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, A, B, ids, scales):
-        lib = L.lib()
-        N, K = weight.shape
-        G, r = A.shape[:2]
-        dt = L.dtype_code(x, "adapter_linear")
-        x2, ldx = L.rows_2d(x.detach(), K, aligned=True)
-        w, ldw = L.rows_2d(weight.detach(), K, aligned=True)
-        T, dev = x2.shape[0], x.device
-        i64 = L.ids_flag(ids, "adapter_linear")
-        Ad, Bd = L.rows_2d(A.detach().contiguous(), K, aligned=True)[0], L.rows_2d(B.detach().contiguous(), r, aligned=True)[0]
-        y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=dev)
-        nk = L.check(lib.sx_adapter_kept_bytes(dt, T, r, G), "sx_adapter_kept_bytes")
-        nw = L.check(lib.sx_adapter_workspace_bytes(dt, T, K, N, r, G, 0), "sx_adapter_workspace_bytes")
-        kept = torch.empty(nk, dtype=torch.uint8, device=dev)
-        ws = torch.empty(nw, dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev):
-            L.check(lib.sx_adapter_forward(dt, T, K, N, r, G, L.ptr(x2), ldx, L.ptr(w), ldw, L.ptr(bias), L.ptr(Ad), L.ptr(Bd), L.ptr(scales),
-                                           L.ptr(ids), i64, L.ptr(y), N, L.ptr(kept), nk, L.ptr(ws), nw, L.stream_ptr()), "sx_adapter_forward")
-        if any(ctx.needs_input_grad):
-            ctx.save_for_backward(x, weight, A, B, scales, kept)
-            ctx.meta = (dt, T, K, N, r, G)
+        y, kept = _project(x.detach(), weight, bias, A.detach(), B.detach(), ids, scales)
+        ctx.save_for_backward(x, weight, A, B, scales, kept)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        lib = L.lib()
         x, weight, A, B, scales, kept = ctx.saved_tensors
-        dt, T, K, N, r, G = ctx.meta
-        need_x, need_a, need_b = ctx.needs_input_grad[0], ctx.needs_input_grad[3], ctx.needs_input_grad[4]
-        dev = x.device
+        need_x, _, _, need_a, need_b = ctx.needs_input_grad[:5]
+        N, K = weight.shape
+        G, r = A.shape[:2]
+        dt, dev = L.dtype_code(x, "adapter_linear"), x.device
         dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
         dA = torch.empty(A.shape, dtype=A.dtype, device=dev) if need_a else None
         dB = torch.empty(B.shape, dtype=B.dtype, device=dev) if need_b else None
+        x2, ldx = L.rows_2d(x, K)
+        T = x2.shape[0]
         if T == 0:
             for g in (dA, dB):
                 if g is not None:
                     g.zero_()
             return dx, None, None, dA, dB, None, None
-        x2, ldx = L.rows_2d(x.detach(), K)
-        w, ldw = L.rows_2d(weight.detach(), K)
+        w, ldw = L.rows_2d(weight, K)
         d2, ldd = L.rows_2d(dy, N, aligned=True)
-        Ad, Bd = A.detach().contiguous(), B.detach().contiguous()
-        nw = L.check(lib.sx_adapter_workspace_bytes(dt, T, K, N, r, G, 1), "sx_adapter_workspace_bytes")
+        Ad, Bd = A.contiguous(), B.contiguous()
+        nw = L.check(L.lib().sx_adapter_workspace_bytes(dt, T, K, N, r, G, 1), "sx_adapter_workspace_bytes")
         ws = torch.empty(nw, dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev):
-            L.check(lib.sx_adapter_backward(dt, T, K, N, r, G, L.ptr(x2), ldx, L.ptr(w), ldw, L.ptr(Ad), L.ptr(Bd), L.ptr(scales), L.ptr(d2), ldd,
-                                            L.ptr(kept), kept.numel(), L.ptr(dx), L.ptr(dA), L.ptr(dB), L.ptr(ws), nw, L.stream_ptr()),
-                    "sx_adapter_backward")
+        L.launch("sx_adapter_backward", dev, dt, T, K, N, r, G, L.addr(x2), ldx, L.addr(w), ldw, L.addr(Ad), L.addr(Bd), L.addr(scales), L.addr(d2), ldd,
+                 L.addr(kept), kept.numel(), L.addr(dx), L.addr(dA), L.addr(dB), L.addr(ws), nw)
         return dx, None, None, dA, dB, None, None
 
 
@@ -79,9 +84,8 @@ def adapter_linear(x, weight, bias, A, B, ids, *, scales=None):
     outside [0, G) -- -1 by convention -- means the shared projection alone.  Sums in fp32, one rounding at the end; the same bits on every
     run.  Gradients go to x, A and B (zeros for an adapter no row names).  Not differentiable twice."""
     who = "adapter_linear"
-    for t in (x, weight, A, B, ids):
-        if not t.is_cuda:
-            raise RuntimeError(f"{who}: the HIP path needs CUDA (ROCm) tensors; this build has no CPU path")
+    if not (x.is_cuda and weight.is_cuda and A.is_cuda and B.is_cuda and ids.is_cuda):
+        raise RuntimeError(f"{who}: the HIP path needs CUDA (ROCm) tensors; this build has no CPU path")
     if weight.dim() != 2 or x.dim() < 1 or weight.shape[1] < 1 or weight.shape[0] < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"{who}: x must be (..., K) and weight (N, K), got {tuple(x.shape)} / {tuple(weight.shape)}")
     N, K = weight.shape
@@ -95,13 +99,12 @@ def adapter_linear(x, weight, bias, A, B, ids, *, scales=None):
     if scales is not None and tuple(scales.shape) != (G,):
         raise ValueError(f"{who}: scales must be ({G},), got {tuple(scales.shape)}")
     L.dtype_code(x, who), L.ids_flag(ids, who)
-    for t in (weight, A, B) + (() if bias is None else (bias,)):
-        if t.dtype != x.dtype:
-            raise ValueError(f"{who}: weight, bias, A and B must have x's dtype {x.dtype}, got {t.dtype}")
-    for t in (weight, A, B, ids) + tuple(t for t in (bias, scales) if t is not None):
-        if t.device != x.device:
-            raise ValueError(f"{who}: all tensors must be on {x.device}, got one on {t.device}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (weight, bias, scales)):
+    dtype, dev = x.dtype, x.device
+    if not (weight.dtype == A.dtype == B.dtype == dtype and (bias is None or bias.dtype == dtype)):
+        raise ValueError(f"{who}: weight, bias, A and B must have x's dtype {dtype}")
+    if not (weight.device == A.device == B.device == ids.device == dev and (bias is None or bias.device == dev) and (scales is None or scales.device == dev)):
+        raise ValueError(f"{who}: all tensors must be on x's device {dev}")
+    if L.wants_grad(weight, bias, scales):
         raise ValueError(f"{who}: the shared projection and the scales are frozen; pass them without requires_grad")
     lead = tuple(x.shape[:-1])
     if ids.dim() < (1 if lead else 0) or tuple(ids.shape) != lead[:ids.dim()]:
@@ -110,7 +113,8 @@ def adapter_linear(x, weight, bias, A, B, ids, *, scales=None):
         ids = ids.reshape(tuple(ids.shape) + (1,) * (len(lead) - ids.dim())).expand(lead)
     if scales is not None:
         scales = scales.detach().float().contiguous()
-    return _AdapterFn.apply(x, weight, None if bias is None else bias.contiguous(), A, B, ids.contiguous(), scales)
+    args = (x, weight, None if bias is None else bias.contiguous(), A, B, ids.contiguous(), scales)
+    return _AdapterFn.apply(*args) if L.wants_grad(x, A, B) else _project(*args)[0]
 
 
 class AdapterLinear(nn.Module):

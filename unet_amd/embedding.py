@@ -9,37 +9,37 @@ from torch import nn
 from . import _lib as L
 
 
+def _lookup(ids, table, scale):
+    """(flat ids, output)"""
+    V, D = table.shape
+    i = ids.contiguous()
+    t, ld = L.rows_2d(table, D)
+    out = torch.empty(*ids.shape, D, dtype=table.dtype, device=table.device)
+    L.launch("sx_embedding_forward", table.device, L.dtype_code(table, "scaled_embedding"), i.numel(), V, D, L.addr(t), ld, L.addr(i),
+             L.ids_flag(i, "scaled_embedding"), scale, L.addr(out))
+    return i, out
+
+
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, table, scale):
-        dt = L.dtype_code(table, "scaled_embedding")
-        V, D = table.shape
-        i = ids.contiguous().view(-1)
-        t = table.detach()
-        t, ld = L.rows_2d(t, D)
-        out = torch.empty(*ids.shape, D, dtype=table.dtype, device=table.device)
-        with torch.cuda.device(table.device):
-            L.check(L.lib().sx_embedding_forward(dt, i.numel(), V, D, L.ptr(t), ld, L.ptr(i), L.ids_flag(ids, "scaled_embedding"),
-                                                 float(scale), L.ptr(out), L.stream_ptr()), "sx_embedding_forward")
+        i, out = _lookup(ids, table.detach(), scale)
         ctx.save_for_backward(i)
-        ctx.meta = (dt, V, D, float(scale), table.dtype)
+        ctx.meta = (*table.shape, scale, table.dtype)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         (i,) = ctx.saved_tensors
-        dt, V, D, scale, dtype = ctx.meta
-        if not ctx.needs_input_grad[1]:
-            return None, None, None
-        lib = L.lib()
+        V, D, scale, dtype = ctx.meta
+        n, dev = i.numel(), dout.device
         d, ld = L.rows_2d(dout, D)
-        grad = torch.empty(V, D, dtype=dtype, device=dout.device)
-        nb = L.check(lib.sx_embedding_workspace_bytes(i.numel(), V, D), "sx_embedding_workspace_bytes")
-        ws = torch.empty(nb, dtype=torch.uint8, device=dout.device)
-        with torch.cuda.device(dout.device):
-            L.check(lib.sx_embedding_backward(dt, i.numel(), V, D, L.ptr(d), ld, L.ptr(i), 1 if i.dtype == torch.int64 else 0, scale,
-                                              L.ptr(grad), L.ptr(ws), nb, L.stream_ptr()), "sx_embedding_backward")
+        grad = torch.empty(V, D, dtype=dtype, device=dev)
+        nb = L.check(L.lib().sx_embedding_workspace_bytes(n, V, D), "sx_embedding_workspace_bytes")
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+        L.launch("sx_embedding_backward", dev, L.dtype_code(grad, "scaled_embedding"), n, V, D, L.addr(d), ld, L.addr(i),
+                 L.ids_flag(i, "scaled_embedding"), scale, L.addr(grad), L.addr(ws), nb)
         return None, grad, None
 
 
@@ -58,7 +58,7 @@ def scaled_embedding(ids, table, scale=1.0):
         raise ValueError(f"{who}: ids are on {ids.device}, the table on {table.device}")
     L.ids_flag(ids, who)
     L.dtype_code(table, who)
-    return _EmbeddingFn.apply(ids, table, float(scale))
+    return _EmbeddingFn.apply(ids, table, float(scale)) if L.wants_grad(table) else _lookup(ids, table, float(scale))[1]
 
 
 class ScaledEmbedding(nn.Module):

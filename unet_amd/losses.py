@@ -155,47 +155,49 @@ def masked_weighted_loss(pred, target, mask, *, w=None, lam_grad=0.2, lam_w=1.0,
     return _LossFn.apply(pred, tgt, m, wt, cw, opts)
 
 
+def _distill(logits, top, idx, weights, tau, reduction, need):
+    """(loss, sum of the weights and row statistics, d loss / d logits), the last two only if `need`"""
+    who = "distillation_loss"
+    V, K = logits.shape[-1], top.shape[-1]
+    z, ld = L.rows_2d(logits, V)
+    N, dev = z.shape[0], logits.device
+    rows = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
+    loss = None if reduction == "none" else torch.empty((), dtype=torch.float32, device=dev)
+    keep = torch.empty(1 + (2 * N if need else 0), dtype=torch.float32, device=dev)
+    d = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if need else None
+    L.launch("sx_distill_forward", dev, L.dtype_code(logits, who), N, V, K, L.addr(z), ld, L.dtype_code(top, who), L.addr(top), L.addr(idx),
+             L.ids_flag(idx, who), tau, L.addr(weights), 1 if reduction == "mean" else 0, L.addr(rows), L.addr(keep) + 4 if need else None, L.addr(keep),
+             L.addr(loss), L.addr(d), V)
+    return (rows if loss is None else loss), keep, d
+
+
 class _DistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, top, idx, weights, tau, reduction):
-        V, K = logits.shape[-1], top.shape[-1]
-        z, ld = L.rows_2d(logits.detach(), V)
-        N = z.shape[0]
-        dev = logits.device
-        dt, tdt, i64 = L.dtype_code(logits, "distillation_loss"), L.dtype_code(top, "distillation_loss"), L.ids_flag(idx, "distillation_loss")
-        need = ctx.needs_input_grad[0]
-        d = torch.empty(N, V, dtype=logits.dtype, device=dev) if need else None
-        rows = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
-        loss = None if reduction == "none" else torch.empty((), dtype=torch.float32, device=dev)
-        keep = torch.empty(1 + 2 * N, dtype=torch.float32, device=dev)         # sum of the weights, row statistics
-        mean = 1 if reduction == "mean" else 0
-        with torch.cuda.device(dev):
-            L.check(L.lib().sx_distill_forward(dt, N, V, K, L.ptr(z), ld, tdt, L.ptr(top), L.ptr(idx), i64, tau, L.ptr(weights), mean,
-                                               L.ptr(rows), L.ptr(keep[1:]) if need else None, L.ptr(keep), L.ptr(loss), L.ptr(d), V,
-                                               L.stream_ptr()), "sx_distill_forward")
-        if need:
-            ctx.save_for_backward(logits, top, idx, weights, keep)
-            ctx.d, ctx.meta = d, (dt, tdt, i64, N, V, K, tau, mean, reduction)
-        return rows if reduction == "none" else loss
+        loss, keep, ctx.d = _distill(logits.detach(), top, idx, weights, tau, reduction, True)
+        ctx.save_for_backward(logits, top, idx, weights, keep)
+        ctx.meta = (tau, reduction)
+        return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         """The forward pass left the gradient for an upstream gradient of 1; rows with another one are computed again from the
         logits (one rounding), not scaled after theirs."""
+        who = "distillation_loss"
         logits, top, idx, weights, keep = ctx.saved_tensors
-        dt, tdt, i64, N, V, K, tau, mean, reduction = ctx.meta
+        tau, reduction = ctx.meta
+        V, K = logits.shape[-1], top.shape[-1]
         d, ctx.d = ctx.d, None                     # the buffer is the caller's now: a second backward pass fills one of its own
         ready = d is not None
         if not ready:
-            d = torch.empty(N, V, dtype=logits.dtype, device=logits.device)
-        z, ld = L.rows_2d(logits.detach(), V)
+            d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        z, ld = L.rows_2d(logits, V)
         g = g.float().contiguous()
-        with torch.cuda.device(logits.device):
-            L.check(L.lib().sx_distill_backward(dt, N, V, K, L.ptr(z), ld, tdt, L.ptr(top), L.ptr(idx), i64, tau, L.ptr(weights), mean,
-                                                L.ptr(keep[1:]), L.ptr(keep), L.ptr(g), 1 if reduction == "none" else 0,
-                                                1 if ready else 0, L.ptr(d), V, L.stream_ptr()), "sx_distill_backward")
-        return d.view(logits.shape), None, None, None, None, None
+        L.launch("sx_distill_backward", logits.device, L.dtype_code(logits, who), z.shape[0], V, K, L.addr(z), ld, L.dtype_code(top, who), L.addr(top),
+                 L.addr(idx), L.ids_flag(idx, who), tau, L.addr(weights), 1 if reduction == "mean" else 0, L.addr(keep) + 4, L.addr(keep), L.addr(g),
+                 1 if reduction == "none" else 0, 1 if ready else 0, L.addr(d), V)
+        return d, None, None, None, None, None
 
 
 def distillation_loss(logits, top_logits, top_idx, *, temperature=1.0, weights=None, reduction="mean"):
@@ -226,7 +228,10 @@ def distillation_loss(logits, top_logits, top_idx, *, temperature=1.0, weights=N
         if tuple(weights.shape) != lead:
             raise ValueError(f"{who}: weights must be {lead}, got {tuple(weights.shape)}")
         weights = weights.detach().to(device=logits.device, dtype=torch.float32).contiguous()
-    return _DistillFn.apply(logits, top_logits.detach().contiguous(), top_idx.contiguous(), weights, tau, reduction)
+    top = top_logits.detach().contiguous()
+    if L.wants_grad(logits):
+        return _DistillFn.apply(logits, top, top_idx.contiguous(), weights, tau, reduction)
+    return _distill(logits, top, top_idx.contiguous(), weights, tau, reduction, False)[0]
 
 
 def edge_weights(mask_np: np.ndarray, sigma_px: float = 3.0) -> np.ndarray:
