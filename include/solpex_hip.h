@@ -416,7 +416,7 @@ int sx_adapter_backward(int dtype, int64_t T, int K, int N, int r, int G, const 
  * A row of weight 0 or without a valid pair has loss 0 and gradient 0, whatever its logits hold.  weights: [N] fp32, NULL = 1.
  *   sx_distill_forward  : row_loss[N]; loss (nullable) = sum of row_loss, divided by max(sum weights, 1e-8) if `mean`
  *                         (den: one float of scratch, required with mean and weights).  dlogits (nullable, row stride ldd) =
- *                         d loss / d logits (for mean = 0: of the plain sum).  row_stats (nullable) [2][N]: kept for the call below.
+ *                         d loss / d logits (for mean = 0: of the plain sum).  row_stats (nullable) [4][N]: kept for the call below.
  *   sx_distill_backward : dlogits = g[t * g_stride] * (the same gradient), from the logits and row_stats of the forward call.
  *                         ready != 0: dlogits still is what that forward call wrote; rows with g = 1 are then left as they are.
  * 0 < tau < inf; N < 2^22.

@@ -6,8 +6,15 @@
 //   dz_v   = c * (q_v - sum_{k: idx_k = v} p_k),   c = tau * weight / den
 //
 // A row of weight 0 or without a valid pair has loss 0 and gradient 0, whatever its logits hold.
+//
+// Both directions are bound by memory: what a pass cannot do without is one read of the logits and one write of the gradient.  A
+// block therefore keeps its row in registers between the two (rows_kernel): 16 threads-waves hold up to 128 Ki bf16 or 64 Ki fp32
+// logits.  Maximum and sum run in one pass (a thread rescales its sum when its maximum grows).  Blocks are persistent, and as soon as
+// a register's gradient is stored the register takes the next row's logits: the loads of a row run under the stores of the one
+// before.  Longer rows, and gradients for another upstream factor than 1, read the logits twice (wide_kernel).
 #include "sx_common.h"
 #include <algorithm>
+#include <type_traits>
 
 namespace sx {
 
@@ -21,9 +28,9 @@ struct DistillArgs {
   const float* den;           // device scalar or null (then den_host)
   float den_host;
   float* row_loss;            // [N]: weight * loss (not divided by den)
-  float* row_max;             // [N] max of z, [N] log2 of the sum (what a later gradient pass needs); null: not kept
-  float* row_sum;
+  float* row_stats;           // [4][N]: maximum and sum of the logits and of the teacher's (what a later gradient pass needs); null: not kept
   void* dz; int64_t lddz;
+  float* den_out;             // sum of the weights, taken and stored by the kernel itself; or null (then den / den_host)
   int ready;                  // gradient pass: dz is as the forward pass left it
   const float* g; int64_t g_stride;      // gradient pass: upstream gradient per row (stride 0: one for all)
 };
@@ -67,21 +74,259 @@ __device__ __forceinline__ float pair_top(const DistillArgs& a, int64_t at) {
   return a.top_bf16 ? to_f32(((const bf16*)a.top)[at]) : ((const float*)a.top)[at];
 }
 
-// fmaxf drops a NaN; the sum that follows brings it back, as exp(NaN - max) is NaN
+// a * b rounded, never fused into a neighbouring addition
+__device__ __forceinline__ float mul_rn(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+
+// exponent of 2 of a logit relative to the row's maximum.  z * c - m * c in one fma: m * c is rounded, but alike for all of the row (and
+// sums move from one maximum to another by the difference of the rounded products).
+// Beyond 1e30 (a row whose every logit is the type's lowest value) m * c could overflow: the difference is taken first.
+struct Expo {
+  float c, m, mc;
+  bool far;
+  __device__ __forceinline__ Expo(float m_, float c_) : c(c_), m(m_), mc(mul_rn(m_, c_)), far(fabsf(m_) > 1e30f) {}
+  __device__ __forceinline__ float at(float z) const { return far ? (z - m) * c : fmaf(z, c, -mc); }
+};
+
+__device__ __forceinline__ void keep_stats(const DistillArgs& a, int64_t row, float m, float s, float tm, float ts) {
+  a.row_stats[row] = m;
+  a.row_stats[a.N + row] = s;
+  a.row_stats[2 * a.N + row] = tm;
+  a.row_stats[3 * a.N + row] = ts;
+}
+
+constexpr int kKeptPairs = 256;        // pairs per row that rows_kernel takes: one per thread of its smallest block
+
+// E logits of a row as they lie in memory, 16 bytes from 16-byte boundaries: element e of vector v is the row's element v * E + e - off,
+// off being the row's start behind a boundary.  Elements before and behind the row read as -inf and are not stored.
+template <typename T>
+__device__ __forceinline__ typename Elem<T>::Vec load_row_vec(const T* __restrict__ z, int off, int V, int v) {
+  constexpr int E = Elem<T>::EPL;
+  const int i = v * E - off;
+  typename Elem<T>::Vec r;
+  if (i >= 0 && i + E <= V) return *reinterpret_cast<const typename Elem<T>::Vec*>(z + i);
+#pragma unroll
+  for (int e = 0; e < E; ++e) r[e] = (i + e >= 0 && i + e < V) ? z[i + e] : from_f32<T>(-INFINITY);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void store_row_vec(T* __restrict__ d, int off, int V, int v, bool whole, typename Elem<T>::Vec r) {
+  constexpr int E = Elem<T>::EPL;
+  const int i = v * E - off;
+  if (whole && i >= 0 && i + E <= V) { *reinterpret_cast<typename Elem<T>::Vec*>(d + i) = r; return; }
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (i + e >= 0 && i + e < V) d[i + e] = r[e];
+}
+template <typename T>
+__device__ __forceinline__ int row_off(const T* z) { return (int)(((uintptr_t)z & 15) / sizeof(T)); }
+
+// a thread's maximum never goes below this, so that a set without a live logit joins the others as a sum of 0
+constexpr float kFloor = -1e30f;
+
+// Row = nh elements up to the first 16-byte boundary, nb whole vectors, the rest.  Vector v belongs to thread v % NT, register v / NT; the
+// elements before and behind the vectors to threads 0, 1, ... one each.  Pair k belongs to thread k; the gradient at its index is
+// stored once more, over the plain q of the row's other elements, behind the next barrier that the block meets anyway.
+template <typename T, int NT, int NV>
+__global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
+  constexpr int E = Elem<T>::EPL, NW = NT / 64;
+  typedef typename Elem<T>::Vec Vec;
+  __shared__ float red[5][NW];                          // per wave: maximum and sum of the logits and of the teacher's, any pair
+  __shared__ float red_kl[NW];
+  __shared__ float pair_p[kKeptPairs];
+  __shared__ int pair_i[kKeptPairs];
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const float it = 1.f / a.tau, c = it * kLog2e;
+  float den = a.den_host;
+  if (a.den_out) {
+    float s = 0.f;
+    for (int64_t i = tid; i < a.N; i += NT) s += a.weights[i];
+    s = all_sum<NT>(s, red_kl);
+    den = fmaxf(s, 1e-8f);
+    if (blockIdx.x == 0 && tid == 0) *a.den_out = den;
+  } else if (a.den) {
+    den = *a.den;
+  }
+  const unsigned my = tid * 16u;                        // bytes: with the block's own base in scalar registers, one offset for all vectors
+  auto vec_at = [](auto* base, unsigned off) {
+    typedef std::conditional_t<std::is_const_v<std::remove_pointer_t<decltype(base)>>, const Vec, Vec> V1;
+    typedef std::conditional_t<std::is_const_v<V1>, const char, char> C1;
+    return reinterpret_cast<V1*>(reinterpret_cast<C1*>(base) + off);
+  };
+  auto shape = [&](const T* z, int& nh, int& nb) {
+    nh = std::min(a.V, (int)((16 - ((uintptr_t)z & 15)) & 15) / (int)sizeof(T));
+    nb = (a.V - nh) / E;
+  };
+  auto weight = [&](int64_t t) { return t < a.N ? (a.weights ? a.weights[t] : 1.f) : 0.f; };
+  Vec r[NV];
+  T loose = {};                                         // as loaded: the conversions wait until the values are needed
+  int64_t pair_raw = -1;
+  unsigned top_raw = 0;
+  auto load_head = [&](int64_t t, int nh, int nb) {     // row t's loose element and pair of this thread
+    const T* z = (const T*)a.z + t * a.ldz;
+    if (tid < a.V - nb * E) loose = z[tid < nh ? tid : tid + nb * E];
+    if (tid < a.K) {
+      const int64_t at = t * a.K + tid;
+      if (a.idx64) pair_raw = ((const int64_t*)a.idx)[at];
+      else pair_raw = ((const int32_t*)a.idx)[at];
+      if (a.top_bf16) top_raw = ((const uint16_t*)a.top)[at];
+      else top_raw = ((const uint32_t*)a.top)[at];
+    }
+  };
+  int64_t row = blockIdx.x;
+  float w = weight(row);
+  {
+    const T* z = (const T*)a.z + row * a.ldz;
+    int nh, nb;
+    shape(z, nh, nb);
+    if (w != 0.f) {
+      load_head(row, nh, nb);
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+        if (tid < nb - k * NT) r[k] = *vec_at(z + nh + k * NT * E, my);
+    }
+  }
+  T* fix_at = nullptr;                                  // the row before: where this thread's pair stands and the gradient there
+  float fix = 0.f;
+  for (; row < a.N; row += gridDim.x) {
+    const T* z = (const T*)a.z + row * a.ldz;
+    T* dz = a.dz ? (T*)a.dz + row * a.lddz : nullptr;
+    const int64_t next = row + gridDim.x;
+    const float wn = weight(next);
+    int nh, nb;
+    shape(z, nh, nb);
+    const bool has_loose = tid < a.V - nb * E;
+    const bool paired = w != 0.f && tid < a.K && pair_raw >= 0 && pair_raw < a.V;
+    const int pi = paired ? (int)pair_raw : -1;
+    const float pt = __builtin_bit_cast(float, a.top_bf16 ? top_raw << 16 : top_raw);
+    const float zp = paired ? to_f32(z[pi]) : 0.f;
+    const float zl = to_f32(loose);
+    float m = kFloor, s = 0.f;
+    if (w != 0.f) {
+      if (has_loose) {
+        m = fmaxf(m, zl);
+        s = __builtin_amdgcn_exp2f(fmaf(zl, c, -mul_rn(m, c)));
+      }
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        if (tid < nb - k * NT) {
+          float f[E], mk = m;
+#pragma unroll
+          for (int e = 0; e < E; ++e) { f[e] = to_f32(r[k][e]); mk = fmaxf(mk, f[e]); }
+          const float mc = mul_rn(mk, c);
+          s *= __builtin_amdgcn_exp2f(mul_rn(m, c) - mc);
+#pragma unroll
+          for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f(fmaf(f[e], c, -mc));
+          m = mk;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    {
+      const float wm = wave_max(m);
+      const float ws = wave_sum(s * __builtin_amdgcn_exp2f(mul_rn(m, c) - mul_rn(wm, c)));
+      const float tm = wave_max(paired ? pt : -INFINITY);
+      const float ts = wave_sum(paired ? expf((pt - tm) * it) : 0.f);
+      const bool any = __ballot(paired) != 0;
+      if (lane == 0) { red[0][wid] = wm; red[1][wid] = ws; red[2][wid] = tm; red[3][wid] = ts; red[4][wid] = any ? 1.f : 0.f; }
+    }
+    __syncthreads();                                    // and every thread has stored its part of the row before
+    if (fix_at) *fix_at = from_f32<T>(fix);
+    fix_at = nullptr;
+    const int ww = lane & (NW - 1);                     // every wave's results, over the lanes
+    const float m1 = red[0][ww], tm1 = red[2][ww], any1 = red[4][ww];
+    float M = wave_max(m1);
+    const float TM = wave_max(tm1), any = wave_max(any1);
+    float S = lane < NW ? red[1][ww] * __builtin_amdgcn_exp2f(mul_rn(m1, c) - mul_rn(M, c)) : 0.f;
+    float TS = lane < NW && any1 != 0.f ? red[3][ww] * expf((tm1 - TM) * it) : 0.f;
+    S = wave_sum(S);
+    TS = wave_sum(TS);
+    const bool live = w != 0.f && any != 0.f;
+    const bool low = live && M <= kFloor;               // no logit above the floor: the row again, from its true maximum
+    if (low) {
+      float mk = -INFINITY;
+      for (int v = tid; v < a.V; v += NT) mk = fmaxf(mk, to_f32(z[v]));
+      M = all_max<NT>(mk, red_kl);
+      float sk = 0.f;
+      for (int v = tid; v < a.V; v += NT) sk += __builtin_amdgcn_exp2f((to_f32(z[v]) - M) * c);
+      S = all_sum<NT>(sk, red_kl);
+      __syncthreads();
+    }
+    const float gc = w * a.tau / den, gs = gc / S, mc = mul_rn(M, c);
+    if (tid < kKeptPairs) {
+      float p = 0.f, kl = 0.f;
+      if (live && paired) {
+        const float lt = (pt - TM) * it;
+        p = expf(lt) / TS;
+        const Expo x(M, c);
+        if (!(p == 0.f)) kl = p * ((lt - logf(TS)) - (x.at(zp) * kLn2 - logf(S)));
+      }
+      pair_i[tid] = pi;
+      pair_p[tid] = p;
+      kl = wave_sum(kl);
+      if (lane == 0) red_kl[wid] = kl;
+    }
+    __syncthreads();
+    if (tid == 0) {
+      float kl = 0.f;
+#pragma unroll
+      for (int i = 0; i < kKeptPairs / 64; ++i) kl += red_kl[i];
+      a.row_loss[row] = live ? kl * a.tau * a.tau * w : 0.f;
+      if (a.row_stats) keep_stats(a, row, M, S, TM, TS);
+    }
+    if (dz && live && wid * 64 < a.K) {                 // the gradient at the pairs' indices, in the order of the pairs
+      const Expo x(M, c);
+      fix = gs * __builtin_amdgcn_exp2f(x.at(zp));
+      for (int j = 0; j < a.K; ++j) fix = pair_i[j] == pi ? fmaf(-gc, pair_p[j], fix) : fix;
+      if (paired) fix_at = dz + pi;
+    }
+    const T* zn = (const T*)a.z + next * a.ldz;
+    int nhn, nbn;
+    shape(zn, nhn, nbn);
+    if (wn != 0.f) load_head(next, nhn, nbn);
+    else nbn = 0;
+    if (dz && has_loose && !low) dz[tid < nh ? tid : tid + nb * E] = from_f32<T>(live ? gs * __builtin_amdgcn_exp2f(fmaf(zl, c, -mc)) : 0.f);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (dz && !low && tid < nb - k * NT) {
+        Vec o = {};
+        if (live)
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[e] = from_f32<T>(gs * __builtin_amdgcn_exp2f(fmaf(to_f32(r[k][e]), c, -mc)));
+        *vec_at(dz + nh + k * NT * E, my) = o;
+      }
+      if (tid < nbn - k * NT) r[k] = *vec_at(zn + nhn + k * NT * E, my);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (dz && low)
+      for (int v = tid; v < a.V; v += NT) dz[v] = from_f32<T>(gs * __builtin_amdgcn_exp2f((to_f32(z[v]) - M) * c));
+    w = wn;
+  }
+  __syncthreads();
+  if (fix_at) *fix_at = from_f32<T>(fix);
+}
+
+// any row length, the logits read once for the maximum and the sum and once for the gradient; with grad_only, the gradient alone, from
+// the maxima and sums of an earlier pass.  fmaxf drops a NaN; the sum brings it back
 template <typename T, int NT>
-__global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a, int grad_only) {
+__global__ __launch_bounds__(NT) void distill_wide_kernel(DistillArgs a, int grad_only) {
+  constexpr int E = Elem<T>::EPL;
+  typedef typename Elem<T>::Vec Vec;
   __shared__ float red[NT / 64];
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x;
   const T* z = (const T*)a.z + row * a.ldz;
   T* dz = a.dz ? (T*)a.dz + row * a.lddz : nullptr;
+  const int off = row_off(z), nv = (a.V + off + E - 1) / E;
+  const bool whole = dz && row_off(dz) == off;
   const float w = a.weights ? a.weights[row] : 1.f;
   float gup = 1.f;
   if (grad_only) {
     gup = a.g[row * a.g_stride];
     if (a.ready && gup == 1.f) return;         // dz still holds the forward pass's gradient, which is this one
   }
-  // teacher
   const int64_t k0 = row * a.K;
   float tm = -INFINITY, any = 0.f;
   for (int k = tid; k < a.K; k += NT) {
@@ -90,36 +335,50 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a, int grad_onl
   }
   tm = all_max<NT>(tm, red);
   any = all_max<NT>(any, red);
+  if (grad_only) tm = a.row_stats[2 * a.N + row];
   if (w == 0.f || any == 0.f) {
     if (tid == 0) {
       if (!grad_only) a.row_loss[row] = 0.f;
-      if (a.row_max) { a.row_max[row] = 0.f; a.row_sum[row] = 0.f; }
+      if (!grad_only && a.row_stats) keep_stats(a, row, 0.f, 0.f, 0.f, 0.f);
     }
-    if (dz) for (int v = tid; v < a.V; v += NT) dz[v] = from_f32<T>(0.f);
+    const Vec zero = {};
+    if (dz) for (int v = tid; v < nv; v += NT) store_row_vec<T>(dz, off, a.V, v, whole, zero);
     return;
   }
-  const float it = 1.f / a.tau, it2 = it * kLog2e;
+  const float it = 1.f / a.tau, c = it * kLog2e;
   float ts = 0.f;
   for (int k = tid; k < a.K; k += NT) {
     const int64_t id = pair_idx(a, k0 + k);
     if (id >= 0 && id < a.V) ts += expf((pair_top(a, k0 + k) - tm) * it);
   }
-  ts = all_sum<NT>(ts, red);
-  const float lts = logf(ts), its = 1.f / ts;
-  // student
+  ts = grad_only ? a.row_stats[3 * a.N + row] : all_sum<NT>(ts, red);
+  const float lts = logf(ts);
   float m, s;
-  if (grad_only && a.row_max) {
-    m = a.row_max[row];
-    s = a.row_sum[row];
+  if (grad_only) {
+    m = a.row_stats[row];
+    s = a.row_stats[a.N + row];
   } else {
     m = -INFINITY;
-    for (int v = tid; v < a.V; v += NT) m = fmaxf(m, to_f32(z[v]));
+    for (int v = tid; v < nv; v += NT) {
+      const Vec r = load_row_vec<T>(z, off, a.V, v);
+#pragma unroll
+      for (int e = 0; e < E; ++e) m = fmaxf(m, to_f32(r[e]));
+    }
     m = all_max<NT>(m, red);
+    const Expo x(m, c);
     s = 0.f;
-    for (int v = tid; v < a.V; v += NT) s += __builtin_amdgcn_exp2f((to_f32(z[v]) - m) * it2);
+    for (int v = tid; v < nv; v += NT) {
+      const Vec r = load_row_vec<T>(z, off, a.V, v);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int i = v * E + e - off;
+        s += i >= 0 && i < a.V ? __builtin_amdgcn_exp2f(x.at(to_f32(r[e]))) : 0.f;
+      }
+    }
     s = all_sum<NT>(s, red);
-    if (tid == 0 && a.row_max) { a.row_max[row] = m; a.row_sum[row] = s; }
+    if (tid == 0 && a.row_stats) keep_stats(a, row, m, s, tm, ts);
   }
+  const Expo x(m, c);
   if (!grad_only) {
     const float ls = logf(s);
     float kl = 0.f;
@@ -127,26 +386,30 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a, int grad_onl
       const int64_t id = pair_idx(a, k0 + k);
       if (id < 0 || id >= a.V) continue;
       const float lp = (pair_top(a, k0 + k) - tm) * it;
-      const float p = expf(lp) * its;
-      if (!(p == 0.f)) kl += p * ((lp - lts) - ((to_f32(z[id]) - m) * it - ls));
+      const float p = expf(lp) / ts;
+      if (!(p == 0.f)) kl += p * ((lp - lts) - (x.at(to_f32(z[id])) * kLn2 - ls));
     }
     kl = all_sum<NT>(kl, red);
     if (tid == 0) a.row_loss[row] = kl * a.tau * a.tau * w;
   }
   if (!dz) return;
-  const float c = gup * w * a.tau / (a.den ? *a.den : a.den_host);
-  const float cs = c / s;
-  for (int v = tid; v < a.V; v += NT) dz[v] = from_f32<T>(cs * __builtin_amdgcn_exp2f((to_f32(z[v]) - m) * it2));
+  const float gc = gup * w * a.tau / (a.den ? *a.den : a.den_host), gs = gc / s;
+  for (int v = tid; v < nv; v += NT) {
+    const Vec r = load_row_vec<T>(z, off, a.V, v);
+    Vec o;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = from_f32<T>(gs * __builtin_amdgcn_exp2f(x.at(to_f32(r[e]))));
+    store_row_vec<T>(dz, off, a.V, v, whole, o);
+  }
   __syncthreads();
   // the teacher's entries over what was just stored; entries that name the same index all store the same value
   for (int k = tid; k < a.K; k += NT) {
     const int64_t id = pair_idx(a, k0 + k);
     if (id < 0 || id >= a.V) continue;
-    float p = 0.f;
+    float g = gs * __builtin_amdgcn_exp2f(x.at(to_f32(z[id])));
     for (int j = 0; j < a.K; ++j)
-      if (pair_idx(a, k0 + j) == id) p += expf((pair_top(a, k0 + j) - tm) * it) * its;
-    const float q = __builtin_amdgcn_exp2f((to_f32(z[id]) - m) * it2) / s;
-    dz[id] = from_f32<T>(c * (q - p));
+      if (pair_idx(a, k0 + j) == id) g = fmaf(-gc, expf((pair_top(a, k0 + j) - tm) * it) / ts, g);
+    dz[id] = from_f32<T>(g);
   }
 }
 
@@ -168,11 +431,41 @@ __global__ __launch_bounds__(1024) void distill_total_kernel(const float* __rest
   if (threadIdx.x == 0) *out = s / (den ? *den : den_host);
 }
 
-template <typename T>
-static int distill_launch(const DistillArgs& a, int grad_only, hipStream_t st) {
-  hipLaunchKernelGGL((distill_kernel<T, 256>), dim3((unsigned)a.N), dim3(256), 0, st, a, grad_only);
-  SX_LAUNCH_CHECK("distill");
+template <typename T, int NT, int NV>
+static int rows_launch(const DistillArgs& a, int per_cu, hipStream_t st) {
+  hipLaunchKernelGGL((distill_rows_kernel<T, NT, NV>), dim3((unsigned)std::min<int64_t>(a.N, 256 * per_cu)), dim3(NT), 0, st, a);
+  SX_LAUNCH_CHECK("distill_rows");
   return SX_OK;
+}
+
+template <typename T>
+static int wide_launch(const DistillArgs& a, int grad_only, hipStream_t st) {
+  if (a.V <= 4096) hipLaunchKernelGGL((distill_wide_kernel<T, 256>), dim3((unsigned)a.N), dim3(256), 0, st, a, grad_only);
+  else hipLaunchKernelGGL((distill_wide_kernel<T, 1024>), dim3((unsigned)a.N), dim3(1024), 0, st, a, grad_only);
+  SX_LAUNCH_CHECK("distill_wide");
+  return SX_OK;
+}
+
+// rows_kernel: the row fits the registers, its pairs the threads, exponents the fma form, and the gradient's rows lie to the 16-byte
+// boundaries as the logits' do
+static bool rows_fit(const DistillArgs& a, int dtype) {
+  const int64_t b = (int64_t)dtype_size(dtype), e = 16 / b;
+  return a.V <= 16 * 1024 * e && a.K <= kKeptPairs && a.tau >= 1e-6f &&
+         (!a.dz || (((uintptr_t)a.dz - (uintptr_t)a.z) % 16 == 0 && (a.N == 1 || (a.lddz - a.ldz) * b % 16 == 0)));
+}
+
+template <typename T>
+static int distill_launch(const DistillArgs& a, hipStream_t st) {
+  constexpr int E = Elem<T>::EPL;
+  if (!rows_fit(a, Elem<T>::kDtype)) return wide_launch<T>(a, 0, st);
+  const int nv = a.V / E;                               // whole vectors, at most
+  if (nv <= 256) return rows_launch<T, 256, 1>(a, 8, st);
+  if (nv <= 512) return rows_launch<T, 256, 2>(a, 8, st);
+  if (nv <= 1024) return rows_launch<T, 256, 4>(a, 6, st);
+  if (nv <= 2048) return rows_launch<T, 512, 4>(a, 3, st);
+  if (nv <= 4096) return rows_launch<T, 512, 8>(a, 2, st);
+  if (nv <= 8192) return rows_launch<T, 1024, 8>(a, 1, st);
+  return rows_launch<T, 1024, 16>(a, 1, st);
 }
 
 static int distill_check(const char* who, int dtype, int64_t N, int V, int K, int64_t ld, int top_dtype, float tau) {
@@ -195,15 +488,19 @@ extern "C" int sx_distill_forward(int dtype, int64_t N, int V, int K, const void
   DistillArgs a = {};
   a.z = logits; a.ldz = ld; a.top = top; a.top_bf16 = top_dtype == SX_BF16; a.idx = idx; a.idx64 = idx64; a.N = N; a.V = V; a.K = K; a.tau = tau;
   a.weights = weights; a.den_host = mean ? fmaxf((float)N, 1e-8f) : 1.f; a.row_loss = row_loss;
-  a.row_max = row_stats; a.row_sum = row_stats ? row_stats + N : nullptr; a.dz = dlogits; a.lddz = ldd;
+  a.row_stats = row_stats; a.dz = dlogits; a.lddz = ldd;
   if (mean && weights) {
-    hipLaunchKernelGGL(distill_den_kernel, dim3(1), dim3(1024), 0, st, weights, N, den);
-    SX_LAUNCH_CHECK("distill_den");
-    a.den = den;
+    if (N > 0 && N <= 16384 && rows_fit(a, dtype)) {
+      a.den_out = den;                                  // few enough weights for every block to add up itself
+    } else {
+      hipLaunchKernelGGL(distill_den_kernel, dim3(1), dim3(1024), 0, st, weights, N, den);
+      SX_LAUNCH_CHECK("distill_den");
+      a.den = den;
+    }
   }
-  if (N > 0) SX_TRY(dtype == SX_BF16 ? distill_launch<bf16>(a, 0, st) : distill_launch<float>(a, 0, st));
+  if (N > 0) SX_TRY(dtype == SX_BF16 ? distill_launch<bf16>(a, st) : distill_launch<float>(a, st));
   if (loss) {
-    hipLaunchKernelGGL(distill_total_kernel, dim3(1), dim3(1024), 0, st, row_loss, N, a.den, a.den_host, loss);
+    hipLaunchKernelGGL(distill_total_kernel, dim3(1), dim3(1024), 0, st, row_loss, N, mean && weights ? den : nullptr, a.den_host, loss);
     SX_LAUNCH_CHECK("distill_total");
   }
   return SX_OK;
@@ -218,6 +515,6 @@ extern "C" int sx_distill_backward(int dtype, int64_t N, int V, int K, const voi
   DistillArgs a = {};
   a.z = logits; a.ldz = ld; a.top = top; a.top_bf16 = top_dtype == SX_BF16; a.idx = idx; a.idx64 = idx64; a.N = N; a.V = V; a.K = K; a.tau = tau;
   a.weights = weights; a.den_host = mean ? fmaxf((float)N, 1e-8f) : 1.f; a.den = mean && weights ? den : nullptr;
-  a.row_max = (float*)row_stats; a.row_sum = (float*)row_stats + N; a.dz = dlogits; a.lddz = ldd; a.g = g; a.g_stride = g_stride; a.ready = ready;
-  return dtype == SX_BF16 ? distill_launch<bf16>(a, 1, (hipStream_t)stream) : distill_launch<float>(a, 1, (hipStream_t)stream);
+  a.row_stats = (float*)row_stats; a.dz = dlogits; a.lddz = ldd; a.g = g; a.g_stride = g_stride; a.ready = ready;
+  return dtype == SX_BF16 ? wide_launch<bf16>(a, 1, (hipStream_t)stream) : wide_launch<float>(a, 1, (hipStream_t)stream);
 }

@@ -156,15 +156,16 @@ def masked_weighted_loss(pred, target, mask, *, w=None, lam_grad=0.2, lam_w=1.0,
 
 
 def _distill(logits, top, idx, weights, tau, reduction, need):
-    """(loss, sum of the weights and row statistics, d loss / d logits), the last two only if `need`"""
+    """(loss, sum of the weights and row statistics, d loss / d logits), the last two only if `need`.  The gradient is formed here for the
+    losses whose upstream gradient is mostly 1; that of a loss per row waits for its upstream gradient."""
     who = "distillation_loss"
     V, K = logits.shape[-1], top.shape[-1]
     z, ld = L.rows_2d(logits, V)
     N, dev = z.shape[0], logits.device
     rows = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
     loss = None if reduction == "none" else torch.empty((), dtype=torch.float32, device=dev)
-    keep = torch.empty(1 + (2 * N if need else 0), dtype=torch.float32, device=dev)
-    d = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if need else None
+    keep = torch.empty(1 + (4 * N if need else 0), dtype=torch.float32, device=dev)
+    d = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if need and reduction != "none" else None
     L.launch("sx_distill_forward", dev, L.dtype_code(logits, who), N, V, K, L.addr(z), ld, L.dtype_code(top, who), L.addr(top), L.addr(idx),
              L.ids_flag(idx, who), tau, L.addr(weights), 1 if reduction == "mean" else 0, L.addr(rows), L.addr(keep) + 4 if need else None, L.addr(keep),
              L.addr(loss), L.addr(d), V)
@@ -182,8 +183,8 @@ class _DistillFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        """The forward pass left the gradient for an upstream gradient of 1; rows with another one are computed again from the
-        logits (one rounding), not scaled after theirs."""
+        """Where the forward pass left the gradient for an upstream gradient of 1, that is it; for another one the gradient is computed
+        again from the logits (one rounding), not scaled after its own."""
         who = "distillation_loss"
         logits, top, idx, weights, keep = ctx.saved_tensors
         tau, reduction = ctx.meta
