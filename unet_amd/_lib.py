@@ -9,6 +9,8 @@ from __future__ import annotations
 import ctypes as C
 import os
 
+import torch
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsolpex_hip.so")
 
@@ -149,13 +151,11 @@ def ptr(t):
 
 
 def stream_ptr():
-    import torch
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
 def dtype_code(t, who):
     """sx dtype of a floating tensor the kernels read (float32 or bfloat16), ValueError otherwise."""
-    import torch
     if t.dtype == torch.float32:
         return SX_F32
     if t.dtype == torch.bfloat16:
@@ -165,7 +165,6 @@ def dtype_code(t, who):
 
 def ids_flag(t, who):
     """1 for int64 ids, 0 for int32, ValueError otherwise."""
-    import torch
     if t.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"{who}: ids must be int64 or int32, got {t.dtype}")
     return 1 if t.dtype == torch.int64 else 0
@@ -189,7 +188,6 @@ def rows_2d(t, width, aligned=False):
 
 
 def torch_clone(t):
-    import torch
     return t.clone(memory_format=torch.contiguous_format)
 
 
@@ -200,7 +198,6 @@ def addr(t):
 
 def launch(name, device, *args):
     """Call the entry point `name` with `args` and, behind them, the current stream of `device`, with that device current."""
-    import torch
     fn = getattr(_lib or lib(), name)
     i = device.index
     if torch._C._cuda_getDevice() == i:
@@ -211,8 +208,13 @@ def launch(name, device, *args):
     return rc if rc >= 0 else check(rc, name)
 
 
+def once(who):
+    """For the top of a backward pass that has no derivative of its own (cheaper than a decorator's context manager)."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{who}: not differentiable twice (create_graph=True)")
+
+
 def wants_grad(*tensors):
-    import torch
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 

@@ -118,7 +118,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(Projec
   for (int at = 0; at < rows;) {
     const int g = __builtin_amdgcn_readfirstlane(a.key[w0 + at]);
     if (g >= a.G) break;                                      // the rows without an adapter come last
-    const int end = (int)std::min<int64_t>(rows, __builtin_amdgcn_readfirstlane(a.start[g + 1]) - w0);
+    const int end = (int)std::min<int64_t>(rows, __builtin_amdgcn_readfirstlane(a.end[g]) - w0);
     const bf16* qg = (const bf16*)a.q + g * a.q_g;
     for (int j0 = 0; j0 < a.r; j0 += 16) {
       const int jr = j0 + (gq & 1) * 8;

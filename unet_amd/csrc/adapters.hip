@@ -109,7 +109,7 @@ struct ShrinkArgs {
   const void* x; int64_t ldx;                 // rows of C elements
   const void* p; int64_t p_g; int p_ld;       // P(g, j, c) = p[g * p_g + j * p_ld + c]
   const float* scales;
-  const int* perm; const int* key; const int* start;
+  const int* perm; const int* key; const int* start; const int* end;
   int64_t T; int C, r, G, rp;
   void* h;                                    // see ProjectArgs
   bf16* ht; int64_t ldt;                      // bf16: [2][rp][ldt], hi and lo parts with the rows along memory; or null
@@ -131,7 +131,7 @@ __global__ __launch_bounds__(64 * NW) void adapter_shrink_kernel(ShrinkArgs a) {
   f32x4 tot[MT][RT] = {};
   for (int at = 0; at < rows;) {
     const int g = a.key[m0 + at];
-    const int end = (int)std::min<int64_t>(rows, a.start[g + 1] - m0);
+    const int end = (int)std::min<int64_t>(rows, a.end[g] - m0);
     if (g < a.G) {
       const T* pr[RT];                        // ranks past the last one read it again: their products are not stored
 #pragma unroll
@@ -267,7 +267,7 @@ __global__ __launch_bounds__(256) void adapter_project_kernel(ProjectArgs a) {
   for (int at = 0; at < rows;) {
     const int g = a.key[m0 + at];
     if (g >= a.G) break;                                  // the rows without an adapter come last
-    const int end = (int)std::min<int64_t>(rows, a.start[g + 1] - m0);
+    const int end = (int)std::min<int64_t>(rows, a.end[g] - m0);
     const T* qg = (const T*)a.q + g * a.q_g;
     for (int j0 = 0; j0 < a.r; j0 += 16) {
       const int jr = j0 + (sizeof(T) == 2 ? (gq & 1) * 8 : gq * 4);
@@ -319,7 +319,7 @@ struct OuterJob {
 };
 struct OuterArgs {
   OuterJob job[2]; int n;
-  const int* perm; const int* start;
+  const int* perm; const int* start; const int* end;
   int r, rp, G; int64_t ldt;
 };
 
@@ -338,7 +338,7 @@ __global__ __launch_bounds__(256) void adapter_outer_f32_kernel(OuterArgs a) {
   outer_block(a, j, c0, g);
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int c = c0 + lane, j0 = blockIdx.y * 16;
-  const int t0 = a.start[g], t1 = a.start[g + 1];
+  const int t0 = a.start[g], t1 = a.end[g];
   float acc[16] = {};
   for (int t = t0 + wid; t < t1; t += 4) {
     const float xv = c < j.C ? ((const float*)j.x)[(int64_t)a.perm[t] * j.ldx + c] : 0.f;
@@ -368,7 +368,7 @@ __global__ __launch_bounds__(256) void adapter_outer_kernel(OuterArgs a) {
   outer_block(a, j, c0, g);
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, n = lane & 15, gq = lane >> 4;
   const int j0 = blockIdx.y * (RT * 16), c = c0 + 4 * n;
-  const int t0 = a.start[g], t1 = a.start[g + 1];
+  const int t0 = a.start[g], t1 = a.end[g];
   const bf16* x = (const bf16*)j.x;
   const bf16* ht = (const bf16*)j.h;
   f32x4 acc[RT][4] = {};
@@ -439,7 +439,7 @@ __global__ __launch_bounds__(256) void adapter_outer_kernel(OuterArgs a) {
 
 // ------------------------------------------------------------------ host
 // kept: what a backward call needs of the forward one
-struct AdapterKept { size_t perm, key, start, h, ht, total; int rp; int64_t ldt; };
+struct AdapterKept { size_t perm, key, start, end, h, ht, total; int rp; int64_t ldt; };
 static AdapterKept adapter_kept(int dtype, int64_t T, int r, int G) {
   AdapterKept w;
   size_t o = 0;
@@ -447,7 +447,8 @@ static AdapterKept adapter_kept(int dtype, int64_t T, int r, int G) {
   w.ldt = (int64_t)align_up((size_t)T, 64);
   w.perm = o; o = align_up(o + (size_t)T * 4, 256);
   w.key = o; o = align_up(o + (size_t)T * 4, 256);
-  w.start = o; o = align_up(o + (size_t)(G + 2) * 4, 256);
+  w.start = o; o = align_up(o + (size_t)(G + 1) * 4, 256);
+  w.end = o; o = align_up(o + (size_t)(G + 1) * 4, 256);
   w.h = o; o = align_up(o + (size_t)T * w.rp * 4, 256);
   w.ht = o; o = align_up(o + (dtype == SX_BF16 ? (size_t)w.rp * w.ldt * 4 : 0), 256);
   w.total = o;
@@ -540,7 +541,7 @@ static int adapter_forward(const AdapterCall& c, const void* ids, int ids64, voi
   const AdapterKept k = adapter_kept(c.dtype, c.T, c.r, c.G);
   const AdapterWs o = adapter_ws(c.dtype, c.T, c.K, c.N, c.r, c.G, false);
   const int Kp = padded(c.dtype, c.K), r8 = padded(c.dtype, c.r);
-  int *perm = (int*)(kept + k.perm), *key = (int*)(kept + k.key), *start = (int*)(kept + k.start);
+  int *perm = (int*)(kept + k.perm), *key = (int*)(kept + k.key), *start = (int*)(kept + k.start), *end = (int*)(kept + k.end);
   const void *x = c.x, *w = c.w, *A = c.A, *B = c.B;
   int64_t ldx = c.ldx, ldw = c.ldw;
   Packer pk;
@@ -555,14 +556,14 @@ static int adapter_forward(const AdapterCall& c, const void* ids, int ids64, voi
     B = ws + o.B;
   }
   SX_TRY(pk.launch<T>(st));
-  SX_TRY(launch_sort_ids(ids, ids64, c.T, c.G, perm, key, start, st));
+  SX_TRY(launch_sort_ids(ids, ids64, c.T, c.G, false, perm, key, start, end, st));
   ShrinkArgs s = {};
-  s.x = x; s.ldx = ldx; s.p = A; s.p_g = (int64_t)c.r * Kp; s.p_ld = Kp; s.scales = c.scales; s.perm = perm; s.key = key; s.start = start;
+  s.x = x; s.ldx = ldx; s.p = A; s.p_g = (int64_t)c.r * Kp; s.p_ld = Kp; s.scales = c.scales; s.perm = perm; s.key = key; s.start = start; s.end = end;
   s.T = c.T; s.C = Kp; s.r = c.r; s.G = c.G; s.rp = k.rp; s.h = kept + k.h; s.ht = sizeof(T) == 2 ? (bf16*)(kept + k.ht) : nullptr; s.ldt = k.ldt;
   SX_TRY(shrink_launch<T>(s, st));
   ProjectArgs p = {};
   p.x = x; p.ldx = ldx; p.w = w; p.ldw = ldw; p.bias = c.bias; p.q = B; p.q_g = (int64_t)c.N * r8; p.q_ld = r8; p.h = kept + k.h; p.rp = k.rp;
-  p.perm = perm; p.key = key; p.start = start; p.T = c.T; p.K = Kp; p.N = c.N; p.r = c.r; p.G = c.G; p.y = y; p.ldy = ldy;
+  p.perm = perm; p.key = key; p.start = start; p.end = end; p.T = c.T; p.K = Kp; p.N = c.N; p.r = c.r; p.G = c.G; p.y = y; p.ldy = ldy;
   return project_launch<T>(p, st);
 }
 
@@ -571,7 +572,7 @@ static int adapter_backward(const AdapterCall& c, const void* dy, int64_t lddy, 
   const AdapterKept k = adapter_kept(c.dtype, c.T, c.r, c.G);
   const AdapterWs o = adapter_ws(c.dtype, c.T, c.K, c.N, c.r, c.G, true);
   const int Np = padded(c.dtype, c.N), r8 = padded(c.dtype, c.r);
-  const int *perm = (const int*)(kept + k.perm), *key = (const int*)(kept + k.key), *start = (const int*)(kept + k.start);
+  const int *perm = (const int*)(kept + k.perm), *key = (const int*)(kept + k.key), *start = (const int*)(kept + k.start), *end = (const int*)(kept + k.end);
   Packer pk;
   const void* d = dy;
   int64_t ldd = lddy;
@@ -589,18 +590,18 @@ static int adapter_backward(const AdapterCall& c, const void* dy, int64_t lddy, 
   bf16* dht = sizeof(T) == 2 ? (bf16*)(ws + o.dht) : nullptr;
   if (dx || dA) {
     ShrinkArgs s = {};
-    s.x = d; s.ldx = ldd; s.p = ws + o.bt; s.p_g = (int64_t)c.r * Np; s.p_ld = Np; s.scales = c.scales; s.perm = perm; s.key = key; s.start = start;
+    s.x = d; s.ldx = ldd; s.p = ws + o.bt; s.p_g = (int64_t)c.r * Np; s.p_ld = Np; s.scales = c.scales; s.perm = perm; s.key = key; s.start = start; s.end = end;
     s.T = c.T; s.C = Np; s.r = c.r; s.G = c.G; s.rp = k.rp; s.h = ws + o.dh; s.ht = dht; s.ldt = k.ldt;
     SX_TRY(shrink_launch<T>(s, st));
   }
   if (dx) {
     ProjectArgs p = {};
     p.x = d; p.ldx = ldd; p.w = ws + o.wt; p.ldw = Np; p.q = ws + o.at; p.q_g = (int64_t)c.K * r8; p.q_ld = r8; p.h = ws + o.dh; p.rp = k.rp;
-    p.perm = perm; p.key = key; p.start = start; p.T = c.T; p.K = Np; p.N = c.K; p.r = c.r; p.G = c.G; p.y = dx; p.ldy = c.K;
+    p.perm = perm; p.key = key; p.start = start; p.end = end; p.T = c.T; p.K = Np; p.N = c.K; p.r = c.r; p.G = c.G; p.y = dx; p.ldy = c.K;
     SX_TRY(project_launch<T>(p, st));
   }
   OuterArgs q = {};
-  q.perm = perm; q.start = start; q.r = c.r; q.rp = k.rp; q.G = c.G; q.ldt = k.ldt;
+  q.perm = perm; q.start = start; q.end = end; q.r = c.r; q.rp = k.rp; q.G = c.G; q.ldt = k.ldt;
   if (dA) {
     OuterJob& j = q.job[q.n++];
     j.x = c.x; j.ldx = c.ldx; j.C = c.K; j.h = sizeof(T) == 2 ? (const void*)dht : ws + o.dh; j.out = dA; j.o_g = (int64_t)c.r * c.K; j.o_j = c.K; j.o_c = 1;

@@ -3,14 +3,21 @@
 // Ids outside [0, rows) are padding: a row of zeros, no gradient.  Both directions are bound by memory: the lookup reads and
 // writes each row once; the gradient reads dout once and writes every row of the table once.  The sums run in fp32 over the
 // entries sorted by id (sort_ids.hip), each row summed by one group of threads in the order of its tokens, so the result does
-// not depend on the run.  A row with more than kRun tokens would keep its group busy long after the others: its entries are cut
-// into runs of kRun, summed by groups of their own into partial rows, and joined in order by a second launch.
+// not depend on the run.  A row with more than `run` tokens would keep its group busy long after the others: its entries are cut
+// into runs, summed by groups of their own into partial rows, and joined in order by a second launch.
 #include "sort_ids.h"
 #include <algorithm>
+#include <type_traits>
 
 namespace sx {
 
-constexpr int kRun = 64;
+// Entries a group sums in a row: about 1024 runs, 16 entries at least.  A group's time is a chain of memory latencies, eight rows at a
+// time: 16384 tokens took 48 us in runs of 64.
+static inline int embed_run(int64_t n) {
+  int run = 16;
+  while ((int64_t)run * 1024 < n) run *= 2;
+  return run;
+}
 constexpr int64_t kMaxRows = 1 << 24;      // the gradient's grid gives every row of the table up to 128 threads of a 2^32 limit
 
 template <typename T, typename I, bool VEC>
@@ -40,130 +47,212 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* __restrict__ ta
 
 struct EmbedBwdArgs {
   const void* dout; int64_t ld;
-  const int* perm; const int* key; const int* start;
+  const int* perm; const int* key; const int* start; const int* end;
   int64_t rows; int dim; int64_t n;
   float scale;
   void* dtable;
   float* part;              // [runs][2][dim]: the first and the last long row that a run of entries holds part of
+  int run;                  // entries per run
   int64_t run_blocks;       // blocks behind those of the rows
-  int64_t row_groups;
 };
 
-template <typename T, int E>
-__device__ __forceinline__ void add_row(const T* __restrict__ p, float (&acc)[E]) {
-  if constexpr (E == 1) acc[0] += to_f32(*p);
-  else {
-    typename Elem<T>::Vec v = *reinterpret_cast<const typename Elem<T>::Vec*>(p);
+// Columns of a thread: NC pieces of E elements, GROUP * E apart, from column c on.  Group = GROUP threads that share a row.
+template <typename T, bool VEC, int GROUP, int NC>
+struct RowSum {
+  static constexpr int E = VEC ? 16 / (int)sizeof(T) : 1;
+  typedef std::conditional_t<VEC, typename Elem<T>::Vec, T> Piece;
+  float acc[NC][E];
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += to_f32(v[e]);
-  }
-}
-
-// sum of dout rows perm[a .. b) at column c
-template <typename T, int E>
-__device__ __forceinline__ void sum_rows(const EmbedBwdArgs& q, int a, int b, int c, float (&acc)[E]) {
-  const T* dout = (const T*)q.dout + c;
-  for (int i = a; i < b; ++i) add_row<T, E>(dout + (int64_t)q.perm[i] * q.ld, acc);
-}
-
-template <typename T, int E>
-__device__ __forceinline__ void put_row(const EmbedBwdArgs& q, int64_t v, int c, const float (&acc)[E]) {
-  T* dst = (T*)q.dtable + v * q.dim + c;
-  if constexpr (E == 1) *dst = from_f32<T>(acc[0] * q.scale);
-  else {
-    typename Elem<T>::Vec o;
+    for (int k = 0; k < NC; ++k)
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = from_f32<T>(acc[e] * q.scale);
-    *reinterpret_cast<typename Elem<T>::Vec*>(dst) = o;
+      for (int e = 0; e < E; ++e) acc[k][e] = 0.f;
   }
-}
+  static __device__ __forceinline__ void load(Piece (&x)[NC], const T* __restrict__ row, int c, int dim) {
+#pragma unroll
+    for (int k = 0; k < NC; ++k)
+      if (c + k * GROUP * E < dim) x[k] = *reinterpret_cast<const Piece*>(row + c + k * GROUP * E);
+  }
+  __device__ __forceinline__ void add(const Piece (&x)[NC], int c, int dim) {
+#pragma unroll
+    for (int k = 0; k < NC; ++k)
+      if (c + k * GROUP * E < dim) {
+        if constexpr (VEC) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[k][e] += to_f32(x[k][e]);
+        } else {
+          acc[k][0] += to_f32(x[k]);
+        }
+      }
+  }
+  // += dout rows perm[a .. b), in that order, U of them in flight
+  __device__ __forceinline__ void rows(const EmbedBwdArgs& q, int a, int b, int c) {
+    constexpr int U = NC == 1 ? 8 : 4;
+    const T* dout = (const T*)q.dout;
+    for (int i = a; i < b; i += U) {
+      Piece x[U][NC];
+      int t[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) t[u] = q.perm[std::min(i + u, b - 1)];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + u < b) load(x[u], dout + (int64_t)t[u] * q.ld, c, q.dim);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + u < b) add(x[u], c, q.dim);
+    }
+  }
+  __device__ __forceinline__ void put(const EmbedBwdArgs& q, int64_t v, int c) const {
+    T* dst = (T*)q.dtable + v * q.dim + c;
+#pragma unroll
+    for (int k = 0; k < NC; ++k)
+      if (c + k * GROUP * E < q.dim) {
+        if constexpr (VEC) {
+          typename Elem<T>::Vec o;
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[e] = from_f32<T>(acc[k][e] * q.scale);
+          *reinterpret_cast<typename Elem<T>::Vec*>(dst + k * GROUP * E) = o;
+        } else {
+          dst[k * GROUP] = from_f32<T>(acc[k][0] * q.scale);
+        }
+      }
+  }
+};
 
-// GROUP threads share a row (or a run of a long row); blocks [0, gridDim.x - run_blocks) take the rows
-template <typename T, bool VEC, int GROUP>
+// Blocks [0, gridDim.x - run_blocks) take the rows of the table, kRows per group (most of them have no token or one: the loads of several
+// rows are what keeps memory busy); the others take the runs of long rows
+constexpr int kRows = 4;
+
+template <typename T, bool VEC, int GROUP, int NC>
 __global__ __launch_bounds__(256) void embed_bwd_kernel(EmbedBwdArgs q) {
-  constexpr int E = VEC ? 16 / (int)sizeof(T) : 1;
+  typedef RowSum<T, VEC, GROUP, NC> Sum;
+  constexpr int E = Sum::E, STEP = GROUP * E * NC;
   const int sub = threadIdx.x / GROUP, li = threadIdx.x % GROUP;
   const int64_t row_blocks = gridDim.x - q.run_blocks;
   if ((int64_t)blockIdx.x < row_blocks) {
-    const int64_t v = blockIdx.x * (int64_t)(256 / GROUP) + sub;
-    if (v >= q.rows) return;
-    const int a = q.start[v], b = q.start[v + 1];
-    if (b - a > kRun) return;
-    for (int c = li * E; c < q.dim; c += GROUP * E) {
-      float acc[E] = {};
-      sum_rows<T, E>(q, a, b, c, acc);
-      put_row<T, E>(q, v, c, acc);
+    const int64_t v0 = (blockIdx.x * (int64_t)(256 / GROUP) + sub) * kRows;
+    if (v0 >= q.rows) return;
+    int st[kRows], en[kRows], first[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      st[i] = q.start[std::min<int64_t>(v0 + i, q.rows)];
+      en[i] = q.end[std::min<int64_t>(v0 + i, q.rows)];
+    }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) first[i] = en[i] > st[i] ? q.perm[st[i]] : -1;
+    for (int c = li * E; c < q.dim; c += STEP) {
+      typename Sum::Piece x[kRows][NC];
+#pragma unroll
+      for (int i = 0; i < kRows; ++i)
+        if (first[i] >= 0) Sum::load(x[i], (const T*)q.dout + (int64_t)first[i] * q.ld, c, q.dim);
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        if (v0 + i >= q.rows || en[i] - st[i] > q.run) continue;
+        Sum s;
+        s.clear();
+        if (first[i] >= 0) {
+          s.add(x[i], c, q.dim);
+          s.rows(q, st[i] + 1, en[i], c);
+        }
+        s.put(q, v0 + i, c);
+      }
     }
   } else {
     const int64_t run = (blockIdx.x - row_blocks) * (int64_t)(256 / GROUP) + sub;
-    const int64_t e0 = run * kRun, e1 = std::min<int64_t>(q.n, e0 + kRun);
+    const int64_t e0 = run * q.run, e1 = std::min<int64_t>(q.n, e0 + q.run);
     if (e0 >= q.n) return;
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
       const int v = q.key[side ? e1 - 1 : e0];
       if (v >= q.rows) continue;
-      const int a = q.start[v], b = q.start[v + 1];
-      if (b - a <= kRun) continue;
+      const int a = q.start[v], b = q.end[v];
+      if (b - a <= q.run) continue;
       if (side && a < e0) continue;                      // one long row fills the run: it is its first
       const int f = (int)std::max<int64_t>(a, e0), t = (int)std::min<int64_t>(b, e1);
       if (!side && a >= e0 && t == e1) continue;         // it begins in this run and goes on: it is its last
-      for (int c = li * E; c < q.dim; c += GROUP * E) {
-        float acc[E] = {};
-        sum_rows<T, E>(q, f, t, c, acc);
+      for (int c = li * E; c < q.dim; c += STEP) {
+        Sum s;
+        s.clear();
+        s.rows(q, f, t, c);
         float* dst = q.part + (run * 2 + side) * q.dim + c;
 #pragma unroll
-        for (int e = 0; e < E; ++e) dst[e] = acc[e];
+        for (int k = 0; k < NC; ++k)
+          if (c + k * GROUP * E < q.dim)
+#pragma unroll
+            for (int e = 0; e < E; ++e) dst[k * GROUP * E + e] = s.acc[k][e];
       }
     }
   }
 }
 
-// the long row that begins in a run (its last one) = that run's last part + the first parts of the runs it goes on into
-template <typename T, bool VEC, int GROUP>
-__global__ __launch_bounds__(256) void embed_join_kernel(EmbedBwdArgs q) {
-  constexpr int E = VEC ? 16 / (int)sizeof(T) : 1;
+// The long row that begins in a run (its last one) = that run's last part + the first parts of the runs it goes on into.  One run per
+// block: its 512 / GROUP groups take every so many parts and add up through LDS, in the order of the groups.
+template <typename T, bool VEC, int GROUP, int NC>
+__global__ __launch_bounds__(512) void embed_join_kernel(EmbedBwdArgs q) {
+  typedef RowSum<T, VEC, GROUP, NC> Sum;
+  constexpr int E = Sum::E, STEP = GROUP * E * NC, SUBS = 512 / GROUP;
+  __shared__ float part[SUBS][GROUP][NC * E];
   const int sub = threadIdx.x / GROUP, li = threadIdx.x % GROUP;
-  const int64_t run = blockIdx.x * (int64_t)(256 / GROUP) + sub;
-  const int64_t e0 = run * kRun, e1 = std::min<int64_t>(q.n, e0 + kRun);
-  if (e0 >= q.n) return;
+  const int64_t run = blockIdx.x, e0 = run * q.run, e1 = std::min<int64_t>(q.n, e0 + q.run);
   const int v = q.key[e1 - 1];
   if (v >= q.rows) return;
-  const int a = q.start[v], b = q.start[v + 1];
-  if (b - a <= kRun || a < e0) return;
-  const int64_t last = (b - 1) / kRun;
-  for (int c = li * E; c < q.dim; c += GROUP * E) {
-    float acc[E] = {};
-    for (int64_t r = run; r <= last; ++r) {
+  const int a = q.start[v], b = q.end[v];
+  if (b - a <= q.run || a < e0) return;
+  const int64_t last = (b - 1) / q.run;
+  for (int c = li * E; c - li * E < q.dim; c += STEP) {
+    Sum s;
+    s.clear();
+#pragma unroll 4
+    for (int64_t r = run + sub; r <= last; r += SUBS) {
       const float* p = q.part + (r * 2 + (r == run ? 1 : 0)) * q.dim + c;
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] += p[e];
+      for (int k = 0; k < NC; ++k)
+        if (c + k * GROUP * E < q.dim)
+#pragma unroll
+          for (int e = 0; e < E; ++e) s.acc[k][e] += p[k * GROUP * E + e];
     }
-    put_row<T, E>(q, v, c, acc);
+#pragma unroll
+    for (int k = 0; k < NC; ++k)
+#pragma unroll
+      for (int e = 0; e < E; ++e) part[sub][li][k * E + e] = s.acc[k][e];
+    __syncthreads();
+    if (sub == 0) {
+      for (int o = 1; o < SUBS; ++o)
+#pragma unroll
+        for (int k = 0; k < NC; ++k)
+#pragma unroll
+          for (int e = 0; e < E; ++e) s.acc[k][e] += part[o][li][k * E + e];
+      s.put(q, v, c);
+    }
+    __syncthreads();
   }
 }
 
-struct EmbedWs { size_t perm, key, start, part, total; };
+struct EmbedWs { size_t perm, key, start, end, part, total; };
 static EmbedWs embed_ws(int64_t n, int64_t rows, int dim) {
   EmbedWs w;
   size_t o = 0;
   w.perm = o; o = align_up(o + (size_t)n * 4, 256);
   w.key = o; o = align_up(o + (size_t)n * 4, 256);
-  w.start = o; o = align_up(o + (size_t)(rows + 2) * 4, 256);
-  w.part = o; o = align_up(o + (n > kRun ? (size_t)cdiv64(n, kRun) * 2 * (size_t)dim * 4 : 0), 256);
+  w.start = o; o = align_up(o + (size_t)(rows + 1) * 4, 256);
+  w.end = o; o = align_up(o + (size_t)(rows + 1) * 4, 256);
+  const int run = embed_run(n);
+  w.part = o; o = align_up(o + (n > run ? (size_t)cdiv64(n, run) * 2 * (size_t)dim * 4 : 0), 256);
   w.total = o;
   return w;
 }
 
-template <typename T, bool VEC, int GROUP>
+template <typename T, bool VEC, int GROUP, int NC>
 static int embed_bwd_launch(EmbedBwdArgs q, hipStream_t st) {
   const int per = 256 / GROUP;
-  const int64_t runs = q.n > kRun ? cdiv64(q.n, kRun) : 0;
+  q.run = embed_run(q.n);
+  const int64_t runs = q.n > q.run ? cdiv64(q.n, q.run) : 0;
   q.run_blocks = cdiv64(runs, per);
-  const int64_t blocks = cdiv64(q.rows, per) + q.run_blocks;
-  hipLaunchKernelGGL((embed_bwd_kernel<T, VEC, GROUP>), dim3((unsigned)blocks), dim3(256), 0, st, q);
+  const int64_t blocks = cdiv64(q.rows, per * kRows) + q.run_blocks;
+  hipLaunchKernelGGL((embed_bwd_kernel<T, VEC, GROUP, NC>), dim3((unsigned)blocks), dim3(256), 0, st, q);
   SX_LAUNCH_CHECK("embed_bwd");
   if (runs) {
-    hipLaunchKernelGGL((embed_join_kernel<T, VEC, GROUP>), dim3((unsigned)q.run_blocks), dim3(256), 0, st, q);
+    hipLaunchKernelGGL((embed_join_kernel<T, VEC, GROUP, NC>), dim3((unsigned)runs), dim3(512), 0, st, q);
     SX_LAUNCH_CHECK("embed_join");
   }
   return SX_OK;
@@ -172,9 +261,10 @@ static int embed_bwd_launch(EmbedBwdArgs q, hipStream_t st) {
 template <typename T, bool VEC>
 static int embed_bwd_pick(const EmbedBwdArgs& q, hipStream_t st) {
   const int pieces = q.dim / (VEC ? 16 / (int)sizeof(T) : 1);
-  if (pieces <= 16) return embed_bwd_launch<T, VEC, 16>(q, st);
-  if (pieces <= 64) return embed_bwd_launch<T, VEC, 64>(q, st);
-  return embed_bwd_launch<T, VEC, 128>(q, st);
+  if (pieces <= 16) return embed_bwd_launch<T, VEC, 16, 1>(q, st);
+  if (pieces <= 64) return embed_bwd_launch<T, VEC, 64, 1>(q, st);
+  if (pieces <= 128) return embed_bwd_launch<T, VEC, 128, 1>(q, st);
+  return embed_bwd_launch<T, VEC, 128, 4>(q, st);
 }
 
 template <typename T>
@@ -233,8 +323,8 @@ extern "C" int sx_embedding_backward(int dtype, int64_t n, int64_t rows, int dim
   char* ws = (char*)workspace;
   EmbedBwdArgs q = {};
   q.dout = dout; q.ld = ld; q.rows = rows; q.dim = dim; q.n = n; q.scale = scale; q.dtable = dtable;
-  q.perm = (int*)(ws + w.perm); q.key = (int*)(ws + w.key); q.start = (int*)(ws + w.start); q.part = (float*)(ws + w.part);
+  q.perm = (int*)(ws + w.perm); q.key = (int*)(ws + w.key); q.start = (int*)(ws + w.start); q.end = (int*)(ws + w.end); q.part = (float*)(ws + w.part);
   hipStream_t st = (hipStream_t)stream;
-  SX_TRY(launch_sort_ids(ids, ids64, n, rows, (int*)q.perm, (int*)q.key, (int*)q.start, st));
+  SX_TRY(launch_sort_ids(ids, ids64, n, rows, true, (int*)q.perm, (int*)q.key, (int*)q.start, (int*)q.end, st));
   return dtype == SX_BF16 ? embed_bwd<bf16>(q, st) : embed_bwd<float>(q, st);
 }

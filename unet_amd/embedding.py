@@ -29,8 +29,8 @@ class _EmbeddingFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
+        L.once("scaled_embedding")
         (i,) = ctx.saved_tensors
         V, D, scale, dtype = ctx.meta
         n, dev = i.numel(), dout.device

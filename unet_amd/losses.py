@@ -181,11 +181,11 @@ class _DistillFn(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         """Where the forward pass left the gradient for an upstream gradient of 1, that is it; for another one the gradient is computed
         again from the logits (one rounding), not scaled after its own."""
         who = "distillation_loss"
+        L.once(who)
         logits, top, idx, weights, keep = ctx.saved_tensors
         tau, reduction = ctx.meta
         V, K = logits.shape[-1], top.shape[-1]
