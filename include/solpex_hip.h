@@ -390,15 +390,18 @@ int sx_embedding_backward(int dtype, int64_t n, int64_t rows, int dim, const voi
  * x (T, K), w (N, K), y / dy (T, N) with row strides in elements; A (G, r, K), B (G, N, r), dx (T, K), dA, dB contiguous; all of
  * `dtype`.  bias [N] and scales [G] (fp32) may be NULL.  Sums in fp32, one rounding; the same bits on every run.
  *   kept      : sx_adapter_kept_bytes, written by the forward call (rows in the order of their adapter, A x), read by the backward call.
- *   workspace : sx_adapter_workspace_bytes for the forward (backward = 0) or the backward call, contents irrelevant before and after.
- *               Both 16-byte aligned.
+ *               NULL: no backward call will follow; up to 64 rows then take a path of their own (two launches).
+ *   workspace : sx_adapter_workspace_bytes for the call's mode, contents irrelevant before and after.  Both 16-byte aligned.
  *   alignment : operands that are read along K (x, w, A forward), N (dy backward) or r (B forward) are read 16 bytes at a time: where that
  *               size is a multiple of 16 bytes, their rows must start 16-byte aligned; where it is not, they may lie anywhere.
  *   sx_adapter_backward: dx, dA, dB may each be NULL (not wanted); dA and dB are written whole (zeros where no row names the adapter).
  * 1 <= r <= 128, 1 <= G <= 65535, T <= 2^24, K and N <= 2^20, G * K and G * N <= 2^29.
  * --------------------------------------------------------------------------------------------- */
 int64_t sx_adapter_kept_bytes(int dtype, int64_t T, int r, int G);
-int64_t sx_adapter_workspace_bytes(int dtype, int64_t T, int K, int N, int r, int G, int backward);
+#define SX_ADAPTER_FORWARD 0   /* sx_adapter_forward with `kept`         */
+#define SX_ADAPTER_BACKWARD 1  /* sx_adapter_backward                    */
+#define SX_ADAPTER_ALONE 2     /* sx_adapter_forward with kept = NULL    */
+int64_t sx_adapter_workspace_bytes(int dtype, int64_t T, int K, int N, int r, int G, int mode);
 int sx_adapter_forward(int dtype, int64_t T, int K, int N, int r, int G, const void* x, int64_t ldx, const void* w, int64_t ldw,
                        const void* bias, const void* A, const void* B, const float* scales, const void* ids, int ids64,
                        void* y, int64_t ldy, void* kept, int64_t kept_bytes, void* workspace, int64_t workspace_bytes,

@@ -184,8 +184,57 @@ def test_gradients_not_wanted():
         ts = [t for t in (x, A, B) if t.requires_grad]
         for got, ref in zip(torch.autograd.grad(y, ts, i["dy"]), [w for w, f in zip(want[1:], (nx, na, nb)) if f]):
             assert torch.equal(got, ref)
+    with torch.no_grad():                       # another path: one launch less order, the same result up to the roundings of the sums
+        y = adapter_linear(i["x"], i["w"], i["b"], i["A"], i["B"], i["ids"], scales=i["sc"])
+    ref, tol = _ref(i)[0]
+    assert ((y.double().cpu() - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,K,N,r,G", [(1, 1, 1, 1, 1), (1, 2048, 2048, 8, 4), (1, 40, 17, 128, 2), (2, 96, 256, 16, 1), (15, 517, 100, 5, 3), (16, 256, 300, 24, 16),
+                                       (17, 1000, 33, 33, 9), (32, 512, 512, 16, 40), (33, 64, 2000, 128, 33), (48, 129, 130, 3, 7), (63, 4096, 272, 16, 64),
+                                       (64, 1032, 1001, 64, 64), (64, 512, 512, 8, 300), (65, 96, 80, 8, 3), (200, 100, 64, 7, 5)])
+def test_forward_alone(T, K, N, r, G, dtype):
+    """Without a gradient: single tokens of up to 64 requests in two launches, more rows as before."""
+    from unet_amd.adapters import adapter_linear
+    for n, kind in enumerate(("random", "one", "none")):
+        i = _inputs(T, K, N, r, G, dtype, kind, bias=n != 1, scales=n != 2, seed=n, idt=torch.int32 if n == 1 else torch.int64)
+        with torch.no_grad():
+            y = adapter_linear(i["x"], i["w"], i["b"], i["A"], i["B"], i["ids"], scales=i["sc"])
+            again = adapter_linear(i["x"], i["w"], i["b"], i["A"], i["B"], i["ids"], scales=i["sc"])
+        ref, tol = _ref(i)[0]
+        assert y.dtype == dtype and ((y.double().cpu() - ref).abs() <= tol).all() and torch.equal(y, again)
+
+
+def test_forward_alone_keeps_nan_in_its_rows():
+    from unet_amd.adapters import adapter_linear
+    for dtype in (torch.float32, torch.bfloat16):
+        i = _inputs(40, 96, 80, 8, 5, dtype)
+        with torch.no_grad():
+            i["A"][3] = float("nan")
+            i["B"][3] = float("inf")
+            i["x"][7] = float("nan")
+            y = adapter_linear(i["x"], i["w"], i["b"], i["A"], i["B"], i["ids"], scales=i["sc"])
+        clean = (i["ids"] != 3) & (torch.arange(40, device="cuda") != 7)
+        assert torch.isfinite(y[clean]).all() and torch.isnan(y[~clean]).all()
+
+
+def test_forward_alone_in_a_graph():
+    from unet_amd.adapters import adapter_linear
+    i = _inputs(20, 256, 320, 16, 6, torch.bfloat16)
+    f = lambda: adapter_linear(i["x"], i["w"], i["b"], i["A"], i["B"], i["ids"], scales=i["sc"])
     with torch.no_grad():
-        assert torch.equal(adapter_linear(i["x"], i["w"], i["b"], i["A"], i["B"], i["ids"], scales=i["sc"]), want[0])
+        f()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = f()
+        for seed in range(3):
+            j = _inputs(20, 256, 320, 16, 6, torch.bfloat16, seed=seed + 50)
+            for k in ("x", "A", "B", "ids"):
+                i[k].copy_(j[k])
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, f())
 
 
 @pytest.mark.parametrize("T,K,N", [(40, 96, 64), (520, 512, 512)])

@@ -77,11 +77,13 @@ def test_adapter_c_entry_refusals():
     from unet_amd import _lib as L
     lib = L.lib()
     nk, nw, nb = lib.sx_adapter_kept_bytes(0, 10, 4, 3), lib.sx_adapter_workspace_bytes(0, 10, 16, 8, 4, 3, 0), lib.sx_adapter_workspace_bytes(0, 10, 16, 8, 4, 3, 1)
+    na = lib.sx_adapter_workspace_bytes(0, 10, 16, 8, 4, 3, 2)
     assert nk > 0 and nw > 0 and nb > 0
     for T, r, G in ((-1, 4, 3), ((1 << 24) + 1, 4, 3), (1, 0, 3), (1, 129, 3), (1, 4, 0), (1, 4, 65536)):
         _bad(lib.sx_adapter_kept_bytes(0, T, r, G))
         _bad(lib.sx_adapter_workspace_bytes(0, T, 16, 8, r, G, 0))
     _bad(lib.sx_adapter_kept_bytes(4, 10, 4, 3))
+    _bad(lib.sx_adapter_workspace_bytes(0, 10, 16, 8, 4, 3, 3))
     _bad(lib.sx_adapter_workspace_bytes(1, 10, 1 << 20, 8, 4, 1000, 1))
     for dt, K, N in ((2, 16, 8), (0, 0, 8), (0, 16, 0), (0, (1 << 20) + 1, 8), (1, 16, (1 << 20) + 1)):
         _bad(lib.sx_adapter_workspace_bytes(dt, 10, K, N, 4, 3, 1))
@@ -90,7 +92,7 @@ def test_adapter_c_entry_refusals():
         return lib.sx_adapter_forward(dt, T, 16, 8, r, G, x, ldx, w, ldw, None, A, B, None, ids, 1, y, ldy, kept, nk, ws, nw, None)
     odd = ctypes.c_void_p(4100)
     for kw in (dict(dt=9), dict(T=-5), dict(r=0), dict(r=200), dict(G=0), dict(x=None), dict(w=None), dict(A=None), dict(B=None), dict(ids=None),
-               dict(y=None), dict(kept=None), dict(ws=None), dict(ldx=15), dict(ldw=15), dict(ldy=7), dict(nk=nk - 1), dict(nw=nw - 1), dict(kept=odd),
+               dict(y=None), dict(ws=None), dict(kept=None, nk=0, nw=na - 1), dict(ldx=15), dict(ldw=15), dict(ldy=7), dict(nk=nk - 1), dict(nw=nw - 1), dict(kept=odd),
                dict(ws=odd), dict(x=odd), dict(w=odd), dict(A=odd), dict(B=odd), dict(ldx=18), dict(ldw=17)):
         _bad(fwd(**kw))
     assert fwd(T=0) == 0

@@ -20,8 +20,8 @@ def _factors(A, B):
     return L.rows_2d(A.contiguous(), A.shape[2], aligned=True)[0], L.rows_2d(B.contiguous(), B.shape[2], aligned=True)[0]
 
 
-def _project(x, weight, bias, A, B, ids, scales):
-    """(y, what the backward pass needs of it)"""
+def _project(x, weight, bias, A, B, ids, scales, keep):
+    """(y, what the backward pass needs of it if `keep`)"""
     lib = L.lib()
     N, K = weight.shape
     G, r = A.shape[:2]
@@ -31,9 +31,9 @@ def _project(x, weight, bias, A, B, ids, scales):
     T = x2.shape[0]
     Ad, Bd = _factors(A, B)
     y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=dev)
-    nk = L.check(lib.sx_adapter_kept_bytes(dt, T, r, G), "sx_adapter_kept_bytes")
-    nw = L.check(lib.sx_adapter_workspace_bytes(dt, T, K, N, r, G, 0), "sx_adapter_workspace_bytes")
-    kept = torch.empty(nk, dtype=torch.uint8, device=dev)
+    nk = L.check(lib.sx_adapter_kept_bytes(dt, T, r, G), "sx_adapter_kept_bytes") if keep else 0
+    nw = L.check(lib.sx_adapter_workspace_bytes(dt, T, K, N, r, G, L.SX_ADAPTER_FORWARD if keep else L.SX_ADAPTER_ALONE), "sx_adapter_workspace_bytes")
+    kept = torch.empty(nk, dtype=torch.uint8, device=dev) if keep else None
     ws = torch.empty(nw, dtype=torch.uint8, device=dev)
     L.launch("sx_adapter_forward", dev, dt, T, K, N, r, G, L.addr(x2), ldx, L.addr(w), ldw, L.addr(bias), L.addr(Ad), L.addr(Bd), L.addr(scales),
              L.addr(ids), L.ids_flag(ids, "adapter_linear"), L.addr(y), N, L.addr(kept), nk, L.addr(ws), nw)
@@ -43,7 +43,7 @@ def _project(x, weight, bias, A, B, ids, scales):
 class _AdapterFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, A, B, ids, scales):
-        y, kept = _project(x.detach(), weight, bias, A.detach(), B.detach(), ids, scales)
+        y, kept = _project(x.detach(), weight, bias, A.detach(), B.detach(), ids, scales, True)
         ctx.save_for_backward(x, weight, A, B, scales, kept)
         return y
 
@@ -68,7 +68,7 @@ class _AdapterFn(torch.autograd.Function):
         w, ldw = L.rows_2d(weight, K)
         d2, ldd = L.rows_2d(dy, N, aligned=True)
         Ad, Bd = A.contiguous(), B.contiguous()
-        nw = L.check(L.lib().sx_adapter_workspace_bytes(dt, T, K, N, r, G, 1), "sx_adapter_workspace_bytes")
+        nw = L.check(L.lib().sx_adapter_workspace_bytes(dt, T, K, N, r, G, L.SX_ADAPTER_BACKWARD), "sx_adapter_workspace_bytes")
         ws = torch.empty(nw, dtype=torch.uint8, device=dev)
         L.launch("sx_adapter_backward", dev, dt, T, K, N, r, G, L.addr(x2), ldx, L.addr(w), ldw, L.addr(Ad), L.addr(Bd), L.addr(scales), L.addr(d2), ldd,
                  L.addr(kept), kept.numel(), L.addr(dx), L.addr(dA), L.addr(dB), L.addr(ws), nw)
@@ -114,7 +114,7 @@ def adapter_linear(x, weight, bias, A, B, ids, *, scales=None):
     if scales is not None:
         scales = scales.detach().float().contiguous()
     args = (x, weight, None if bias is None else bias.contiguous(), A, B, ids.contiguous(), scales)
-    return _AdapterFn.apply(*args) if L.wants_grad(x, A, B) else _project(*args)[0]
+    return _AdapterFn.apply(*args) if L.wants_grad(x, A, B) else _project(*args, False)[0]
 
 
 class AdapterLinear(nn.Module):

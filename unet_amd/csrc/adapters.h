@@ -46,4 +46,10 @@ struct ProjectArgs {
 bool project_tiles_ok(const ProjectArgs& a);
 int project_tiles_launch(const ProjectArgs& a, hipStream_t st);
 
+// a few rows, forward alone (adapter_tokens.hip)
+constexpr int kTokens = 64;
+size_t tokens_workspace(int dtype, int T, int K, int N, int r);
+int tokens_forward(int dtype, int T, int K, int N, int r, int G, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* A,
+                   const void* B, const float* scales, const void* ids, int ids64, void* y, int64_t ldy, char* ws, hipStream_t st);
+
 }  // namespace sx

@@ -636,9 +636,15 @@ extern "C" int64_t sx_adapter_kept_bytes(int dtype, int64_t T, int r, int G) {
   return (int64_t)adapter_kept(dtype, T, r, G).total;
 }
 
-extern "C" int64_t sx_adapter_workspace_bytes(int dtype, int64_t T, int K, int N, int r, int G, int backward) {
+// what a forward call without `kept` needs besides: nothing more for a few rows, else the kept part itself, behind the rest
+static size_t adapter_alone(int dtype, int64_t T, int K, int N, int r, int G) {
+  return T <= kTokens ? tokens_workspace(dtype, (int)T, K, N, r) : adapter_ws(dtype, T, K, N, r, G, false).total + adapter_kept(dtype, T, r, G).total;
+}
+
+extern "C" int64_t sx_adapter_workspace_bytes(int dtype, int64_t T, int K, int N, int r, int G, int mode) {
   SX_TRY(adapter_check("sx_adapter_workspace_bytes", dtype, T, K, N, r, G));
-  return (int64_t)adapter_ws(dtype, T, K, N, r, G, backward != 0).total;
+  SX_REQUIRE(mode >= 0 && mode <= 2, "sx_adapter_workspace_bytes: mode %d", mode);
+  return (int64_t)std::max<size_t>(256, mode == SX_ADAPTER_ALONE ? adapter_alone(dtype, T, K, N, r, G) : adapter_ws(dtype, T, K, N, r, G, mode == SX_ADAPTER_BACKWARD).total);
 }
 
 extern "C" int sx_adapter_forward(int dtype, int64_t T, int K, int N, int r, int G, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
@@ -646,13 +652,19 @@ extern "C" int sx_adapter_forward(int dtype, int64_t T, int K, int N, int r, int
                                   int64_t kept_bytes, void* workspace, int64_t workspace_bytes, void* stream) {
   SX_TRY(adapter_check("sx_adapter_forward", dtype, T, K, N, r, G));
   if (T == 0) return SX_OK;
-  SX_REQUIRE(x && w && A && B && ids && y && kept && workspace, "sx_adapter_forward: null pointer");
+  SX_REQUIRE(x && w && A && B && ids && y && workspace, "sx_adapter_forward: null pointer");
   SX_REQUIRE(rows_ok(dtype, x, ldx, K) && rows_ok(dtype, w, ldw, K) && rows_ok(dtype, A, K, K) && rows_ok(dtype, B, r, r) && ldy >= N,
              "sx_adapter_forward: rows of x, w, A (K=%d) or B (r=%d) shorter than that or not 16-byte aligned (ldx=%lld ldw=%lld ldy=%lld)", K, r,
              (long long)ldx, (long long)ldw, (long long)ldy);
-  SX_REQUIRE(kept_bytes >= (int64_t)adapter_kept(dtype, T, r, G).total && (uintptr_t)kept % 16 == 0 &&
-                 workspace_bytes >= (int64_t)adapter_ws(dtype, T, K, N, r, G, false).total && (uintptr_t)workspace % 16 == 0,
-             "sx_adapter_forward: kept or workspace too small or not 16-byte aligned");
+  const size_t need = adapter_ws(dtype, T, K, N, r, G, false).total;
+  SX_REQUIRE(!kept || (kept_bytes >= (int64_t)adapter_kept(dtype, T, r, G).total && (uintptr_t)kept % 16 == 0), "sx_adapter_forward: kept too small or not 16-byte aligned");
+  SX_REQUIRE(workspace_bytes >= (int64_t)(kept ? need : adapter_alone(dtype, T, K, N, r, G)) && (uintptr_t)workspace % 16 == 0,
+             "sx_adapter_forward: workspace too small or not 16-byte aligned");
+  if (!kept) {
+    if (T <= kTokens)
+      return tokens_forward(dtype, (int)T, K, N, r, G, x, ldx, w, ldw, bias, A, B, scales, ids, ids64, y, ldy, (char*)workspace, (hipStream_t)stream);
+    kept = (char*)workspace + need;
+  }
   const AdapterCall c = {dtype, T, K, N, r, G, x, ldx, w, ldw, bias, A, B, scales};
   return dtype == SX_BF16 ? adapter_forward<bf16>(c, ids, ids64, y, ldy, (char*)kept, (char*)workspace, (hipStream_t)stream)
                           : adapter_forward<float>(c, ids, ids64, y, ldy, (char*)kept, (char*)workspace, (hipStream_t)stream);
