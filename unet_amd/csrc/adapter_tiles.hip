@@ -1,11 +1,13 @@
 // The shared product of the adapter projection (adapters.hip) on bf16 tiles.
 //
-// A block of WM x WN waves computes BM sorted rows x BN columns, each wave MI x NJ 16x16x32 MFMA fragments.  K steps of 32 go through
-// a ring of four LDS buffers filled by LDS-DMA; x is gathered through perm by the DMA's addresses.  The fragments of step s + 1 are
-// read while the MFMAs of step s run, so at the top of step s buffer s is free again: the DMA of step s + 4 goes there, with steps s + 2
-// and s + 3 in flight behind it.  One barrier and one counted wait per step.  A 64-byte row of a step holds its four 16-byte pieces at
-// (piece ^ (row >> 1) & 3): eight lanes that read one piece of consecutive rows then meet eight different parts of the banks.
-// The W fragment is the MFMA's left operand: a lane ends up with four consecutive columns of one row.
+// A block of WM x WN waves computes BM sorted rows x BN columns, each wave MI x NJ 16x16x32 MFMA fragments.  A stage is 64 of K: 128 bytes
+// of each row of x (gathered through perm by the addresses) and of w, brought by LDS-DMA as whole cache lines (with 64-byte rows, two
+// requests per line, the L2s were the bound: 0.73 us per 32 of K on 256 x 256 tiles).  x and w have rings of NA and NB stages.  Fragments
+// are read half a stage ahead of their MFMAs, so that the buffers of stage s are free in the middle of its MFMAs: there stands the one
+// barrier of a stage, with a wait for stage s + 1 and the DMA of the stages NA and NB on.
+// The eight 16-byte pieces of a row lie at (piece ^ row & 7): eight lanes that read one piece of consecutive rows then meet eight different
+// parts of the banks (no conflicts counted).  The W fragment is the MFMA's left operand: a lane ends up with four consecutive columns of
+// one row.
 #include "adapters.h"
 #include <algorithm>
 #include <atomic>
@@ -14,12 +16,12 @@ namespace sx {
 
 template <int N> __device__ __forceinline__ void tiles_wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
-template <int WM, int WN, int MI, int NJ, int OCC>
+template <int WM, int WN, int MI, int NJ, int OCC, int NA, int NB>
 __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(ProjectArgs a, int gm, int gn, unsigned x_bytes, unsigned w_bytes) {
-  constexpr int NT = 64 * WM * WN, BM = WM * MI * 16, BN = WN * NJ * 16, NBUF = 4, RPR = NT / 4;      // RPR: rows per DMA round
-  constexpr int SA = BM * 64, SB = BN * 64, STAGE = SA + SB;
-  constexpr int QA = SA / (NT * 16), QB = SB / (NT * 16);
-  static_assert(SA % (NT * 16) == 0 && SB % (NT * 16) == 0, "whole DMA rounds");
+  constexpr int NT = 64 * WM * WN, BM = WM * MI * 16, BN = WN * NJ * 16, RPR = NT / 8;      // RPR: rows per DMA round
+  constexpr int SA = BM * 128, SB = BN * 128, QA = SA / (NT * 16), QB = SB / (NT * 16);
+  static_assert(SA % (NT * 16) == 0 && SB % (NT * 16) == 0 && RPR % 8 == 0, "whole DMA rounds");
+  static_assert(NB >= 2 && NA >= NB, "the order of the DMA (w first) and the counts of the waits");
   extern __shared__ __align__(16) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, n = lane & 15, gq = lane >> 4;
   // consecutive blocks go to different XCDs: give each XCD a contiguous range of tiles, walked in patches of 8 row tiles
@@ -36,33 +38,37 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(Projec
   const int wm = wid / WN, wn = wid % WN;
 
   unsigned xo[QA], wo[QB];
-  const int piece = (tid & 3) ^ ((tid >> 3) & 3);          // rows advance by RPR, a multiple of 8, from round to round: the same piece in all
+  const int piece = (tid & 7) ^ ((tid >> 3) & 7);          // rows advance by RPR, a multiple of 8, from round to round: the same piece in all
 #pragma unroll
   for (int q = 0; q < QA; ++q) {
-    const int64_t m = m0 + q * RPR + (tid >> 2);
+    const int64_t m = m0 + q * RPR + (tid >> 3);
     xo[q] = m < a.T ? (unsigned)((int64_t)a.perm[m] * a.ldx * 2) + piece * 16 : 0x80000000u;
   }
 #pragma unroll
   for (int q = 0; q < QB; ++q) {
-    const int c = n0 + q * RPR + (tid >> 2);
+    const int c = n0 + q * RPR + (tid >> 3);
     wo[q] = c < a.N ? (unsigned)(c * a.ldw * 2) + piece * 16 : 0x80000000u;
   }
-  const int nst = (a.K + 31) / 32;
-  auto issue = [&](int s) {
-    char* buf = smem + (s % NBUF) * STAGE + wid * 1024;
-    const bool live = s < nst;                             // past the end: zeros, which keep the count of loads uniform
-    const unsigned far = piece * 8 + s * 32 < a.K ? 0u : 0x80000000u;
-    __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc((void*)a.x, 0, live ? x_bytes : 0, 0x00020000);
-    __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)a.w, 0, live ? w_bytes : 0, 0x00020000);
+  const int nst = (a.K + 63) / 64;
+  char* const sx = smem;
+  char* const sw = smem + NA * SA;
+  // past the end: zeros, which keep the count of loads uniform
+  auto issue_x = [&](int s, int slot) {
+    const unsigned far = piece * 8 + s * 64 < a.K ? 0u : 0x80000000u;
+    __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)a.x, 0, s < nst ? x_bytes : 0, 0x00020000);
 #pragma unroll
     for (int q = 0; q < QA; ++q) {
-      const unsigned off = (xo[q] + s * 64u) | far;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (__attribute__((address_space(3))) void*)(buf + q * (NT * 16)), 16, off, 0, 0, 0);
+      const unsigned off = (xo[q] + s * 128u) | far;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(sx + slot * SA + wid * 1024 + q * (NT * 16)), 16, off, 0, 0, 0);
     }
+  };
+  auto issue_w = [&](int s, int slot) {
+    const unsigned far = piece * 8 + s * 64 < a.K ? 0u : 0x80000000u;
+    __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)a.w, 0, s < nst ? w_bytes : 0, 0x00020000);
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
-      const unsigned off = (wo[q] + s * 64u) | far;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (__attribute__((address_space(3))) void*)(buf + SA + q * (NT * 16)), 16, off, 0, 0, 0);
+      const unsigned off = (wo[q] + s * 128u) | far;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(sw + slot * SB + wid * 1024 + q * (NT * 16)), 16, off, 0, 0, 0);
     }
   };
 
@@ -71,22 +77,17 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(Projec
   for (int i = 0; i < MI; ++i)
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int row_off = n * 64 + ((gq ^ ((n >> 1) & 3)) << 4);
-  const int x_off = wm * MI * 1024 + row_off, w_off = SA + wn * NJ * 1024 + row_off;
+  // fragment row n of the first 32 of a stage's 64; the others' pieces differ in bit 2 of the position
+  const int row_off = n * 128 + ((gq ^ (n & 7)) << 4);
+  const int x_off = wm * MI * 2048 + row_off, w_off = wn * NJ * 2048 + row_off;
   bf16x8 xa[MI], wa[NJ], xb[MI], wb[NJ];
-  // step s: multiply the fragments in (xc, wc) while those of step s + 1 arrive in (xn, wn_)
-  auto step = [&](int s, bf16x8 (&xc)[MI], bf16x8 (&wc)[NJ], bf16x8 (&xn)[MI], bf16x8 (&wn_)[NJ]) {
-    tiles_wait_vm<2 * (QA + QB)>();                           // this wave's pieces of step s + 1 have landed
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");        // and its fragments of step s
-    __builtin_amdgcn_s_barrier();                             // ... for every wave: buffer s is free
-    issue(s + 4);
-    const char* buf = smem + ((s + 1) % NBUF) * STAGE;
+  // multiply the fragments (xc, wc) while (xn, wn_) are read from (px, pw)
+  auto half = [&](const char* px, const char* pw, bf16x8 (&xc)[MI], bf16x8 (&wc)[NJ], bf16x8 (&xn)[MI], bf16x8 (&wn_)[NJ]) {
     constexpr int READS = MI + NJ, GROUP = MI * NJ / READS;   // MFMAs between two reads
-    int done = 0;
 #pragma unroll
     for (int t = 0; t < READS; ++t) {
-      if (t < NJ) wn_[t] = *reinterpret_cast<const bf16x8*>(buf + w_off + t * 1024);
-      else xn[t - NJ] = *reinterpret_cast<const bf16x8*>(buf + x_off + (t - NJ) * 1024);
+      if (t < NJ) wn_[t] = *reinterpret_cast<const bf16x8*>(pw + t * 2048);
+      else xn[t - NJ] = *reinterpret_cast<const bf16x8*>(px + (t - NJ) * 2048);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int e = 0; e < (t == READS - 1 ? MI * NJ - GROUP * (READS - 1) : GROUP); ++e) {
@@ -97,51 +98,57 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(Projec
     }
   };
 #pragma unroll
-  for (int s = 0; s < 4; ++s) issue(s);
-  tiles_wait_vm<3 * (QA + QB)>();
+  for (int s = -NA; s < 0; ++s) {
+    if (s + NB >= 0) issue_w(s + NB, s + NB);
+    issue_x(s + NA, s + NA);
+  }
+  tiles_wait_vm<(NA - 1) * QA + (NB - 1) * QB>();
   __builtin_amdgcn_s_barrier();
 #pragma unroll
-  for (int j = 0; j < NJ; ++j) wa[j] = *reinterpret_cast<const bf16x8*>(smem + w_off + j * 1024);
+  for (int j = 0; j < NJ; ++j) wa[j] = *reinterpret_cast<const bf16x8*>(sw + w_off + j * 2048);
 #pragma unroll
-  for (int i = 0; i < MI; ++i) xa[i] = *reinterpret_cast<const bf16x8*>(smem + x_off + i * 1024);
-  int s = 0;
-  for (; s + 1 < nst; s += 2) {
-    step(s, xa, wa, xb, wb);
-    step(s + 1, xb, wb, xa, wa);
+  for (int i = 0; i < MI; ++i) xa[i] = *reinterpret_cast<const bf16x8*>(sx + x_off + i * 2048);
+  int ax = 0, aw = 0;                                         // the slots of stage s
+  for (int s = 0; s < nst; ++s) {
+    half(sx + ax * SA + (x_off ^ 64), sw + aw * SB + (w_off ^ 64), xa, wa, xb, wb);
+    tiles_wait_vm<(NA - 2) * QA + (NB - 2) * QB>();           // this wave's pieces of stage s + 1 have landed
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");        // and its reads of stage s
+    __builtin_amdgcn_s_barrier();                             // ... for every wave: the buffers of stage s are free
+    issue_w(s + NB, aw);
+    issue_x(s + NA, ax);
+    ax = ax + 1 == NA ? 0 : ax + 1;
+    aw = aw + 1 == NB ? 0 : aw + 1;
+    half(sx + ax * SA + x_off, sw + aw * SB + w_off, xb, wb, xa, wa);
   }
-  if (s < nst) step(s, xa, wa, xb, wb);
   tiles_wait_vm<0>();                                         // no DMA may land in LDS that this block has given back
 
-  // the adapters that this wave's rows meet, 16 ranks at a time
+  // The adapters that this wave's rows meet, 16 ranks at a time, as one more short K step each.  A fragment of 16 rows that one adapter
+  // owns takes it in its accumulators; one that several share gets each adapter's product apart and picks its rows, in the epilogue:
+  // masking h alone would let a NaN or an infinity of one adapter reach the others' rows as 0 * NaN.
   const int64_t w0 = m0 + wm * MI * 16;
   const int rows = (int)std::min<int64_t>(MI * 16, a.T - w0);
+  auto q_piece = [&](int g, int j, int jr) {
+    const int c = std::min(n0 + (wn * NJ + j) * 16 + n, a.N - 1);
+    return load_piece<bf16>((const bf16*)a.q + g * a.q_g + (int64_t)c * a.q_ld, jr, a.q_ld);
+  };
+  auto h_piece = [&](int i, int j0) {
+    const int64_t m = w0 + std::min(i * 16 + n, rows - 1);
+    return *reinterpret_cast<const bf16x8*>((const bf16*)a.h + m * (2 * a.rp) + j0 * 2 + gq * 8);
+  };
   for (int at = 0; at < rows;) {
     const int g = __builtin_amdgcn_readfirstlane(a.key[w0 + at]);
     if (g >= a.G) break;                                      // the rows without an adapter come last
     const int end = (int)std::min<int64_t>(rows, __builtin_amdgcn_readfirstlane(a.end[g]) - w0);
-    const bf16* qg = (const bf16*)a.q + g * a.q_g;
     for (int j0 = 0; j0 < a.r; j0 += 16) {
-      const int jr = j0 + (gq & 1) * 8;
       bf16x8 qf[NJ];
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const int c = std::min(n0 + (wn * NJ + j) * 16 + n, a.N - 1);
-        qf[j] = load_piece<bf16>(qg + (int64_t)c * a.q_ld, jr, a.q_ld);
-      }
+      for (int j = 0; j < NJ; ++j) qf[j] = q_piece(g, j, j0 + (gq & 1) * 8);
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
-        if (i * 16 >= end || i * 16 + 16 <= at) continue;
-        const int64_t m = w0 + std::min(i * 16 + n, rows - 1);
-        const bf16x8 hf = *reinterpret_cast<const bf16x8*>((const bf16*)a.h + m * (2 * a.rp) + j0 * 2 + gq * 8);
-        const bool mine = i * 16 + n >= at && i * 16 + n < end;     // only its rows: 0 * NaN must not reach the others
+        if (i * 16 < at || i * 16 >= end || std::min(i * 16 + 16, rows) > end) continue;
+        const bf16x8 hf = h_piece(i, j0);
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          const f32x4 z = {0.f, 0.f, 0.f, 0.f};
-          const f32x4 d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf[j], hf, z, 0, 0, 0);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][j][e] += mine ? d[e] : 0.f;
-        }
-        __builtin_amdgcn_sched_barrier(0);
+        for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf[j], hf, acc[i][j], 0, 0, 0);
       }
     }
     at = end;
@@ -149,16 +156,30 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(Projec
   const bool wide = a.N % 4 == 0 && a.ldy % 4 == 0 && (uintptr_t)a.y % 8 == 0;
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
-    const int64_t m = w0 + i * 16 + n;
-    if (m < a.T) {
-      bf16* y = (bf16*)a.y + (int64_t)a.perm[m] * a.ldy;
+    if (i * 16 >= rows) continue;
+    const int64_t m = w0 + std::min(i * 16 + n, rows - 1);
+    const int mine = a.key[m], last = std::min(i * 16 + 15, rows - 1);
+    const int g0 = __builtin_amdgcn_readfirstlane(a.key[w0 + i * 16]), g1 = __builtin_amdgcn_readfirstlane(a.key[w0 + last]);
+    bf16* y = (bf16*)a.y + (int64_t)a.perm[m] * a.ldy;
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const int c = n0 + (wn * NJ + j) * 16 + 4 * gq;
-        f32x4 v = acc[i][j];
+    for (int j = 0; j < NJ; ++j) {
+      const int c = n0 + (wn * NJ + j) * 16 + 4 * gq;
+      f32x4 v = acc[i][j];
+      if (g0 != g1) {
+        for (int at = i * 16; at <= last;) {
+          const int g = __builtin_amdgcn_readfirstlane(a.key[w0 + at]);
+          if (g >= a.G) break;
+          f32x4 d = {0.f, 0.f, 0.f, 0.f};
+          for (int j0 = 0; j0 < a.r; j0 += 16) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q_piece(g, j, j0 + (gq & 1) * 8), h_piece(i, j0), d, 0, 0, 0);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (a.bias && c + e < a.N) v[e] += (float)((const bf16*)a.bias)[c + e];
+          for (int e = 0; e < 4; ++e) v[e] += mine == g ? d[e] : 0.f;
+          at = (int)std::min<int64_t>(last + 1, __builtin_amdgcn_readfirstlane(a.end[g]) - w0);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (a.bias && c + e < a.N) v[e] += (float)((const bf16*)a.bias)[c + e];
+      if (i * 16 + n < rows) {
         if (wide) {
           if (c < a.N) store4(y + c, v);
         } else {
@@ -184,15 +205,15 @@ bool project_tiles_ok(const ProjectArgs& a) {
   return xb < (1ll << 31) - 4096 && wb < (1ll << 31) - 4096;
 }
 
-template <int WM, int WN, int MI, int NJ, int OCC>
+template <int WM, int WN, int MI, int NJ, int OCC, int NA, int NB>
 static int tiles_launch(const ProjectArgs& a, hipStream_t st) {
-  constexpr int BM = WM * MI * 16, BN = WN * NJ * 16, LDS = 4 * (BM + BN) * 64;
+  constexpr int BM = WM * MI * 16, BN = WN * NJ * 16, LDS = (NA * BM + NB * BN) * 128;
   static std::atomic<unsigned long long> done{0};
-  SX_TRY(ensure_max_lds((const void*)adapter_tiles_kernel<WM, WN, MI, NJ, OCC>, done, "adapter_tiles"));
+  SX_TRY(ensure_max_lds((const void*)adapter_tiles_kernel<WM, WN, MI, NJ, OCC, NA, NB>, done, "adapter_tiles"));
   int64_t xb, wb;
   tiles_bytes(a, xb, wb);
   const int gm = (int)cdiv64(a.T, BM), gn = cdiv(a.N, BN);
-  hipLaunchKernelGGL((adapter_tiles_kernel<WM, WN, MI, NJ, OCC>), dim3((unsigned)(gm * gn)), dim3(64 * WM * WN), LDS, st, a, gm, gn, (unsigned)xb, (unsigned)wb);
+  hipLaunchKernelGGL((adapter_tiles_kernel<WM, WN, MI, NJ, OCC, NA, NB>), dim3((unsigned)(gm * gn)), dim3(64 * WM * WN), LDS, st, a, gm, gn, (unsigned)xb, (unsigned)wb);
   SX_LAUNCH_CHECK("adapter_tiles");
   return SX_OK;
 }
@@ -205,10 +226,10 @@ static double tiles_cost(const ProjectArgs& a, int bm, int bn, int per_cu, doubl
 
 int project_tiles_launch(const ProjectArgs& a, hipStream_t st) {
   const double c0 = tiles_cost(a, 256, 256, 1, 1.0), c1 = tiles_cost(a, 128, 256, 1, 1.2), c2 = tiles_cost(a, 128, 128, 2, 1.4), c3 = tiles_cost(a, 64, 64, 4, 2.0);
-  if (c0 <= c1 && c0 <= c2 && c0 <= c3) return tiles_launch<2, 4, 8, 4, 2>(a, st);
-  if (c1 <= c2 && c1 <= c3) return tiles_launch<2, 4, 4, 4, 2>(a, st);
-  if (c2 <= c3) return tiles_launch<2, 2, 4, 4, 2>(a, st);
-  return tiles_launch<2, 2, 2, 2, 4>(a, st);
+  if (c0 <= c1 && c0 <= c2 && c0 <= c3) return tiles_launch<2, 4, 8, 4, 2, 3, 2>(a, st);
+  if (c1 <= c2 && c1 <= c3) return tiles_launch<2, 4, 4, 4, 2, 3, 3>(a, st);
+  if (c2 <= c3) return tiles_launch<2, 2, 4, 4, 2, 3, 2>(a, st);
+  return tiles_launch<1, 4, 4, 1, 4, 3, 3>(a, st);
 }
 
 }  // namespace sx
