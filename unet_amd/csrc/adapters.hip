@@ -118,7 +118,7 @@ struct ShrinkArgs {
 // MT * 16 sorted rows and RT * 16 ranks per block; its NW waves split the columns
 template <typename T, int MT, int RT, int NW>
 __global__ __launch_bounds__(64 * NW) void adapter_shrink_kernel(ShrinkArgs a) {
-  constexpr int EPL = Elem<T>::EPL, CK = Elem<T>::CK, RJ = RT * 16, U = 4;
+  constexpr int EPL = Elem<T>::EPL, CK = Elem<T>::CK, RJ = RT * 16, U = MT + RT <= 2 ? 8 : 4;      // U: chunks in flight per wave
   typedef typename Elem<T>::Vec Vec;
   __shared__ float red[NW][MT * 16][RJ + 1];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, n = lane & 15, gq = lane >> 4;
@@ -356,13 +356,15 @@ __global__ __launch_bounds__(256) void adapter_outer_f32_kernel(OuterArgs a) {
   }
 }
 
-// bf16: 64 columns and RT * 16 ranks per block; a wave takes every fourth block of 32 rows.  h comes with the rows along memory (16 bytes
-// = 8 rows of one rank); x comes as it lies, 4 columns of 8 rows per lane, and is turned in registers: fragment f holds columns 4 n + f.
-// 32-row blocks are aligned, so that h's 16-byte reads are: rows of other adapters in the first and last one are cleared on both
-// sides.
+// bf16: 64 columns and RT * 16 ranks per block; a wave takes every eighth block of 32 rows, the next block's x on its way under the MFMAs
+// of one.  h comes with the rows along memory (16 bytes = 8 rows of one rank); x comes as it lies, 4 columns of 8 rows per lane, and is
+// turned in registers: fragment f holds columns 4 n + f.  32-row blocks are aligned, so that h's and perm's 16-byte reads are: rows of
+// other adapters in the first and last one are cleared on both sides.
 template <int RT>
-__global__ __launch_bounds__(256) void adapter_outer_kernel(OuterArgs a) {
-  __shared__ float red[4][RT * 16][64 + 1];
+__global__ __launch_bounds__(512) void adapter_outer_kernel(OuterArgs a) {
+  constexpr int NW = 8;
+  typedef __attribute__((ext_vector_type(4))) int i32x4;
+  __shared__ float red[NW / 2][RT * 16][64 + 1];
   OuterJob j;
   int c0, g;
   outer_block(a, j, c0, g);
@@ -372,30 +374,36 @@ __global__ __launch_bounds__(256) void adapter_outer_kernel(OuterArgs a) {
   const bf16* x = (const bf16*)j.x;
   const bf16* ht = (const bf16*)j.h;
   f32x4 acc[RT][4] = {};
-  for (int tb = (t0 & ~31) + wid * 32; tb < t1; tb += 128) {
-    const int t = tb + gq * 8;
-    u32x4 lo, hi;                             // columns (0, 1) and (2, 3) of rows t + 2 e, t + 2 e + 1
-    uint32_t v[8][2];
+  auto load_perm = [&](int tb, int (&p)[8]) {               // (perm's storage reaches to a multiple of 64 rows)
+    if (tb >= t1) return;
+    const i32x4 lo = *reinterpret_cast<const i32x4*>(a.perm + tb + gq * 8), hi = *reinterpret_cast<const i32x4*>(a.perm + tb + gq * 8 + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { p[e] = lo[e]; p[4 + e] = hi[e]; }
+  };
+  auto load_x = [&](int tb, const int (&p)[8], uint32_t (&v)[8][2]) {      // columns (0, 1) and (2, 3) of 8 rows
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       v[e][0] = v[e][1] = 0;
-      if (t + e >= t0 && t + e < t1) {
-        const bf16* p = x + (int64_t)a.perm[t + e] * j.ldx + c;
+      const int t = tb + gq * 8 + e;
+      if (t >= t0 && t < t1) {
+        const bf16* q = x + (int64_t)p[e] * j.ldx + c;
         if (j.vec) {
           if (c < j.C) {
-            const uint64_t q = *reinterpret_cast<const uint64_t*>(p);
-            v[e][0] = (uint32_t)q;
-            v[e][1] = (uint32_t)(q >> 32);
+            const uint64_t w = *reinterpret_cast<const uint64_t*>(q);
+            v[e][0] = (uint32_t)w;
+            v[e][1] = (uint32_t)(w >> 32);
           }
         } else {
-          const uint16_t* p16 = reinterpret_cast<const uint16_t*>(p);
-          if (c < j.C) v[e][0] = p16[0];
-          if (c + 1 < j.C) v[e][0] |= (uint32_t)p16[1] << 16;
-          if (c + 2 < j.C) v[e][1] = p16[2];
-          if (c + 3 < j.C) v[e][1] |= (uint32_t)p16[3] << 16;
+          const uint16_t* q16 = reinterpret_cast<const uint16_t*>(q);
+          if (c < j.C) v[e][0] = q16[0];
+          if (c + 1 < j.C) v[e][0] |= (uint32_t)q16[1] << 16;
+          if (c + 2 < j.C) v[e][1] = q16[2];
+          if (c + 3 < j.C) v[e][1] |= (uint32_t)q16[3] << 16;
         }
       }
     }
+  };
+  auto multiply = [&](int tb, const uint32_t (&v)[8][2], const bf16x8 (&hv)[RT][2]) {
     bf16x8 xf[4];
 #pragma unroll
     for (int f = 0; f < 4; ++f) {
@@ -409,28 +417,64 @@ __global__ __launch_bounds__(256) void adapter_outer_kernel(OuterArgs a) {
     }
     const bool whole = tb >= t0 && tb + 32 <= t1;
 #pragma unroll
-    for (int k = 0; k < RT; ++k) {
-      const bf16* h = ht + (int64_t)std::min(j0 + k * 16 + n, a.rp - 1) * a.ldt + t;
+    for (int k = 0; k < RT; ++k)
 #pragma unroll
       for (int part = 0; part < 2; ++part) {
-        bf16x8 hv = *reinterpret_cast<const bf16x8*>(h + part * (int64_t)a.rp * a.ldt);
+        bf16x8 h = hv[k][part];
         if (!whole)
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (t + e < t0 || t + e >= t1) hv[e] = (bf16)0.f;
+            if (tb + gq * 8 + e < t0 || tb + gq * 8 + e >= t1) h[e] = (bf16)0.f;
 #pragma unroll
-        for (int f = 0; f < 4; ++f) acc[k][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hv, xf[f], acc[k][f], 0, 0, 0);
+        for (int f = 0; f < 4; ++f) acc[k][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(h, xf[f], acc[k][f], 0, 0, 0);
       }
+  };
+  auto load_h = [&](int tb, bf16x8 (&hv)[RT][2]) {
+#pragma unroll
+    for (int k = 0; k < RT; ++k) {
+      const bf16* h = ht + (int64_t)std::min(j0 + k * 16 + n, a.rp - 1) * a.ldt + tb + gq * 8;
+#pragma unroll
+      for (int part = 0; part < 2; ++part) hv[k][part] = *reinterpret_cast<const bf16x8*>(h + part * (int64_t)a.rp * a.ldt);
+    }
+  };
+  constexpr int STEP = NW * 32;
+  int tb = (t0 & ~31) + wid * 32;
+  if (t0 < t1) {
+    int p[8];
+    uint32_t va[8][2], vb[8][2];
+    bf16x8 hv[RT][2];
+    load_perm(tb, p);
+    load_x(tb, p, va);
+    load_perm(tb + STEP, p);
+    for (; tb < t1; tb += 2 * STEP) {
+      load_h(tb, hv);
+      load_x(tb + STEP, p, vb);
+      load_perm(tb + 2 * STEP, p);
+      multiply(tb, va, hv);
+      if (tb + STEP < t1) load_h(tb + STEP, hv);
+      load_x(tb + 2 * STEP, p, va);
+      load_perm(tb + 3 * STEP, p);
+      if (tb + STEP < t1) multiply(tb + STEP, vb, hv);
     }
   }
+  auto slot = [&](int k, int q, int f) -> float& { return red[wid & (NW / 2 - 1)][k * 16 + 4 * gq + q][4 * n + f]; };
+  if (wid >= NW / 2)
 #pragma unroll
-  for (int k = 0; k < RT; ++k)
+    for (int k = 0; k < RT; ++k)
 #pragma unroll
-    for (int f = 0; f < 4; ++f)
+      for (int f = 0; f < 4; ++f)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) red[wid][k * 16 + 4 * gq + q][4 * n + f] = acc[k][f][q];
+        for (int q = 0; q < 4; ++q) slot(k, q, f) = acc[k][f][q];
   __syncthreads();
-  for (int i = tid; i < RT * 16 * 64; i += 256) {
+  if (wid < NW / 2)
+#pragma unroll
+    for (int k = 0; k < RT; ++k)
+#pragma unroll
+      for (int f = 0; f < 4; ++f)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) slot(k, q, f) += acc[k][f][q];
+  __syncthreads();
+  for (int i = tid; i < RT * 16 * 64; i += 64 * NW) {
     const int k = j.o_j == 1 ? i % (RT * 16) : i >> 6, cc = j.o_j == 1 ? i / (RT * 16) : i & 63;
     if (j0 + k < a.r && c0 + cc < j.C)
       ((bf16*)j.out)[g * j.o_g + (j0 + k) * j.o_j + (int64_t)(c0 + cc) * j.o_c] = (bf16)(red[0][k][cc] + red[1][k][cc] + red[2][k][cc] + red[3][k][cc]);
@@ -445,7 +489,7 @@ static AdapterKept adapter_kept(int dtype, int64_t T, int r, int G) {
   size_t o = 0;
   w.rp = round_up(r, 16);
   w.ldt = (int64_t)align_up((size_t)T, 64);
-  w.perm = o; o = align_up(o + (size_t)T * 4, 256);
+  w.perm = o; o = align_up(o + (size_t)w.ldt * 4, 256);      // read 16 bytes at a time by adapter_outer_kernel
   w.key = o; o = align_up(o + (size_t)T * 4, 256);
   w.start = o; o = align_up(o + (size_t)(G + 1) * 4, 256);
   w.end = o; o = align_up(o + (size_t)(G + 1) * 4, 256);
@@ -522,8 +566,8 @@ static int outer_launch(OuterArgs a, hipStream_t st) {
   }
   if (!blocks) return SX_OK;
   if (sizeof(T) == 4) hipLaunchKernelGGL(adapter_outer_f32_kernel, dim3(blocks, cdiv(a.r, 16)), dim3(256), 0, st, a);
-  else if (a.rp <= 16) hipLaunchKernelGGL(adapter_outer_kernel<1>, dim3(blocks, 1), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL(adapter_outer_kernel<2>, dim3(blocks, cdiv(a.rp, 32)), dim3(256), 0, st, a);
+  else if (a.rp <= 16) hipLaunchKernelGGL(adapter_outer_kernel<1>, dim3(blocks, 1), dim3(512), 0, st, a);
+  else hipLaunchKernelGGL(adapter_outer_kernel<2>, dim3(blocks, cdiv(a.rp, 32)), dim3(512), 0, st, a);
   SX_LAUNCH_CHECK("adapter_outer");
   return SX_OK;
 }
