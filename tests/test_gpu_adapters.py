@@ -99,6 +99,28 @@ def test_largest_tiles(T, K, N, r, G, kind):
     _check(_inputs(T, K, N, r, G, torch.bfloat16, kind))
 
 
+@pytest.mark.parametrize("T,K,N,r,G,kind", [(4100, 36, 4096, 20, 3, "random"), (4100, 2048, 132, 5, 40, "segments")])
+def test_largest_tiles_fp32(T, K, N, r, G, kind):
+    _check(_inputs(T, K, N, r, G, torch.float32, kind))
+
+
+def test_operands_beyond_two_gib():
+    """x of 2.2 GB (offsets that pass 32 bits): the rows of its end against a call on them alone."""
+    from unet_amd.adapters import adapter_linear
+    T, K, N, r, G = 1 << 20, 1048, 24, 4, 3
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(T, K, generator=g, device="cuda", dtype=torch.bfloat16)
+    i = _inputs(8, K, N, r, G, torch.bfloat16)
+    ids = torch.randint(-1, G, (T,), generator=g, device="cuda")
+    with torch.no_grad():
+        y = adapter_linear(x, i["w"], i["b"], i["A"], i["B"], ids)
+        assert y.shape == (T, N)
+        for a in (0, 500000, T - 200):
+            i["x"], i["ids"], i["sc"] = x[a:a + 200], ids[a:a + 200], None
+            ref, tol = _ref({**i, "dy": torch.zeros(200, N)})[0]
+            assert ((y[a:a + 200].double().cpu() - ref).abs() <= tol).all()
+
+
 def test_rows_without_an_adapter():
     for dtype in (torch.float32, torch.bfloat16):
         y, dx, dA, dB = _check(_inputs(70, 40, 33, 6, 4, dtype, "none"))

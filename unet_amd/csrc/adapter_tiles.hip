@@ -1,7 +1,7 @@
-// The shared product of the adapter projection (adapters.hip) on bf16 tiles.
+// The shared product of the adapter projection (adapters.hip) by tiles.
 //
-// A block of WM x WN waves computes BM sorted rows x BN columns, each wave MI x NJ 16x16x32 MFMA fragments.  A stage is 64 of K: 128 bytes
-// of each row of x (gathered through perm by the addresses) and of w, brought by LDS-DMA as whole cache lines (with 64-byte rows, two
+// A block of WM x WN waves computes BM sorted rows x BN columns, each wave MI x NJ MFMA fragments of 16 x 16.  A stage is 128 bytes of K (64
+// bf16, 32 fp32) of each row of x (gathered through perm by the addresses) and of w, brought by LDS-DMA as whole cache lines (with 64-byte rows, two
 // requests per line, the L2s were the bound: 0.73 us per 32 of K on 256 x 256 tiles).  x and w have rings of NA and NB stages.  Fragments
 // are read half a stage ahead of their MFMAs, so that the buffers of stage s are free in the middle of its MFMAs: there stands the one
 // barrier of a stage, with a wait for stage s + 1 and the DMA of the stages NA and NB on.
@@ -16,11 +16,13 @@ namespace sx {
 
 template <int N> __device__ __forceinline__ void tiles_wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
-template <int WM, int WN, int MI, int NJ, int OCC, int NA, int NB>
+template <typename T, int WM, int WN, int MI, int NJ, int OCC, int NA, int NB>
 __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(ProjectArgs a, int gm, int gn, unsigned x_bytes, unsigned w_bytes) {
   constexpr int NT = 64 * WM * WN, BM = WM * MI * 16, BN = WN * NJ * 16, RPR = NT / 8;      // RPR: rows per DMA round
   constexpr int SA = BM * 128, SB = BN * 128, QA = SA / (NT * 16), QB = SB / (NT * 16);
   static_assert(SA % (NT * 16) == 0 && SB % (NT * 16) == 0 && RPR % 8 == 0, "whole DMA rounds");
+  constexpr int E = sizeof(T), EPL = Elem<T>::EPL, KS = 128 / E;      // KS: K per stage
+  typedef typename Elem<T>::Vec Vec;
   static_assert(NB >= 2 && NA >= NB, "the order of the DMA (w first) and the counts of the waits");
   extern __shared__ __align__(16) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, n = lane & 15, gq = lane >> 4;
@@ -42,19 +44,19 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(Projec
 #pragma unroll
   for (int q = 0; q < QA; ++q) {
     const int64_t m = m0 + q * RPR + (tid >> 3);
-    xo[q] = m < a.T ? (unsigned)((int64_t)a.perm[m] * a.ldx * 2) + piece * 16 : 0x80000000u;
+    xo[q] = m < a.T ? (unsigned)((int64_t)a.perm[m] * a.ldx * E) + piece * 16 : 0x80000000u;
   }
 #pragma unroll
   for (int q = 0; q < QB; ++q) {
     const int c = n0 + q * RPR + (tid >> 3);
-    wo[q] = c < a.N ? (unsigned)(c * a.ldw * 2) + piece * 16 : 0x80000000u;
+    wo[q] = c < a.N ? (unsigned)(c * a.ldw * E) + piece * 16 : 0x80000000u;
   }
-  const int nst = (a.K + 63) / 64;
+  const int nst = (a.K + KS - 1) / KS;
   char* const sx = smem;
   char* const sw = smem + NA * SA;
   // past the end: zeros, which keep the count of loads uniform
   auto issue_x = [&](int s, int slot) {
-    const unsigned far = piece * 8 + s * 64 < a.K ? 0u : 0x80000000u;
+    const unsigned far = piece * EPL + s * KS < a.K ? 0u : 0x80000000u;
     __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)a.x, 0, s < nst ? x_bytes : 0, 0x00020000);
 #pragma unroll
     for (int q = 0; q < QA; ++q) {
@@ -63,7 +65,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(Projec
     }
   };
   auto issue_w = [&](int s, int slot) {
-    const unsigned far = piece * 8 + s * 64 < a.K ? 0u : 0x80000000u;
+    const unsigned far = piece * EPL + s * KS < a.K ? 0u : 0x80000000u;
     __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)a.w, 0, s < nst ? w_bytes : 0, 0x00020000);
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
@@ -77,22 +79,22 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(Projec
   for (int i = 0; i < MI; ++i)
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  // fragment row n of the first 32 of a stage's 64; the others' pieces differ in bit 2 of the position
+  // fragment row n of the first half of a stage; the other half's pieces differ in bit 2 of the position
   const int row_off = n * 128 + ((gq ^ (n & 7)) << 4);
   const int x_off = wm * MI * 2048 + row_off, w_off = wn * NJ * 2048 + row_off;
-  bf16x8 xa[MI], wa[NJ], xb[MI], wb[NJ];
+  Vec xa[MI], wa[NJ], xb[MI], wb[NJ];
   // multiply the fragments (xc, wc) while (xn, wn_) are read from (px, pw)
-  auto half = [&](const char* px, const char* pw, bf16x8 (&xc)[MI], bf16x8 (&wc)[NJ], bf16x8 (&xn)[MI], bf16x8 (&wn_)[NJ]) {
+  auto half = [&](const char* px, const char* pw, Vec (&xc)[MI], Vec (&wc)[NJ], Vec (&xn)[MI], Vec (&wn_)[NJ]) {
     constexpr int READS = MI + NJ, GROUP = MI * NJ / READS;   // MFMAs between two reads
 #pragma unroll
     for (int t = 0; t < READS; ++t) {
-      if (t < NJ) wn_[t] = *reinterpret_cast<const bf16x8*>(pw + t * 2048);
-      else xn[t - NJ] = *reinterpret_cast<const bf16x8*>(px + (t - NJ) * 2048);
+      if (t < NJ) wn_[t] = *reinterpret_cast<const Vec*>(pw + t * 2048);
+      else xn[t - NJ] = *reinterpret_cast<const Vec*>(px + (t - NJ) * 2048);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int e = 0; e < (t == READS - 1 ? MI * NJ - GROUP * (READS - 1) : GROUP); ++e) {
         const int f = t * GROUP + e, i = f / NJ, j = f % NJ;
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wc[j], xc[i], acc[i][j], 0, 0, 0);
+        acc[i][j] = Mma<T>::run(wc[j], xc[i], acc[i][j]);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -105,9 +107,9 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(Projec
   tiles_wait_vm<(NA - 1) * QA + (NB - 1) * QB>();
   __builtin_amdgcn_s_barrier();
 #pragma unroll
-  for (int j = 0; j < NJ; ++j) wa[j] = *reinterpret_cast<const bf16x8*>(sw + w_off + j * 2048);
+  for (int j = 0; j < NJ; ++j) wa[j] = *reinterpret_cast<const Vec*>(sw + w_off + j * 2048);
 #pragma unroll
-  for (int i = 0; i < MI; ++i) xa[i] = *reinterpret_cast<const bf16x8*>(sx + x_off + i * 2048);
+  for (int i = 0; i < MI; ++i) xa[i] = *reinterpret_cast<const Vec*>(sx + x_off + i * 2048);
   int ax = 0, aw = 0;                                         // the slots of stage s
   for (int s = 0; s < nst; ++s) {
     half(sx + ax * SA + (x_off ^ 64), sw + aw * SB + (w_off ^ 64), xa, wa, xb, wb);
@@ -127,40 +129,37 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(Projec
   // masking h alone would let a NaN or an infinity of one adapter reach the others' rows as 0 * NaN.
   const int64_t w0 = m0 + wm * MI * 16;
   const int rows = (int)std::min<int64_t>(MI * 16, a.T - w0);
-  auto q_piece = [&](int g, int j, int jr) {
+  auto q_piece = [&](int g, int j, int j0) {
     const int c = std::min(n0 + (wn * NJ + j) * 16 + n, a.N - 1);
-    return load_piece<bf16>((const bf16*)a.q + g * a.q_g + (int64_t)c * a.q_ld, jr, a.q_ld);
+    return load_piece<T>((const T*)a.q + g * a.q_g + (int64_t)c * a.q_ld, j0 + h_rank<T>(gq), a.q_ld);
   };
-  auto h_piece = [&](int i, int j0) {
-    const int64_t m = w0 + std::min(i * 16 + n, rows - 1);
-    return *reinterpret_cast<const bf16x8*>((const bf16*)a.h + m * (2 * a.rp) + j0 * 2 + gq * 8);
-  };
+  auto h_piece = [&](int i, int j0) { return load_h<T>(a, w0 + std::min(i * 16 + n, rows - 1), j0, gq); };
   for (int at = 0; at < rows;) {
     const int g = __builtin_amdgcn_readfirstlane(a.key[w0 + at]);
     if (g >= a.G) break;                                      // the rows without an adapter come last
     const int end = (int)std::min<int64_t>(rows, __builtin_amdgcn_readfirstlane(a.end[g]) - w0);
     for (int j0 = 0; j0 < a.r; j0 += 16) {
-      bf16x8 qf[NJ];
+      Vec qf[NJ];
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) qf[j] = q_piece(g, j, j0 + (gq & 1) * 8);
+      for (int j = 0; j < NJ; ++j) qf[j] = q_piece(g, j, j0);
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
         if (i * 16 < at || i * 16 >= end || std::min(i * 16 + 16, rows) > end) continue;
-        const bf16x8 hf = h_piece(i, j0);
+        const Vec hf = h_piece(i, j0);
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf[j], hf, acc[i][j], 0, 0, 0);
+        for (int j = 0; j < NJ; ++j) acc[i][j] = Mma<T>::run(qf[j], hf, acc[i][j]);
       }
     }
     at = end;
   }
-  const bool wide = a.N % 4 == 0 && a.ldy % 4 == 0 && (uintptr_t)a.y % 8 == 0;
+  const bool wide = a.N % 4 == 0 && a.ldy % 4 == 0 && (uintptr_t)a.y % (4 * E) == 0;
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     if (i * 16 >= rows) continue;
     const int64_t m = w0 + std::min(i * 16 + n, rows - 1);
     const int mine = a.key[m], last = std::min(i * 16 + 15, rows - 1);
     const int g0 = __builtin_amdgcn_readfirstlane(a.key[w0 + i * 16]), g1 = __builtin_amdgcn_readfirstlane(a.key[w0 + last]);
-    bf16* y = (bf16*)a.y + (int64_t)a.perm[m] * a.ldy;
+    T* y = (T*)a.y + (int64_t)a.perm[m] * a.ldy;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const int c = n0 + (wn * NJ + j) * 16 + 4 * gq;
@@ -170,7 +169,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(Projec
           const int g = __builtin_amdgcn_readfirstlane(a.key[w0 + at]);
           if (g >= a.G) break;
           f32x4 d = {0.f, 0.f, 0.f, 0.f};
-          for (int j0 = 0; j0 < a.r; j0 += 16) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q_piece(g, j, j0 + (gq & 1) * 8), h_piece(i, j0), d, 0, 0, 0);
+          for (int j0 = 0; j0 < a.r; j0 += 16) d = Mma<T>::run(q_piece(g, j, j0), h_piece(i, j0), d);
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[e] += mine == g ? d[e] : 0.f;
           at = (int)std::min<int64_t>(last + 1, __builtin_amdgcn_readfirstlane(a.end[g]) - w0);
@@ -178,14 +177,14 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(Projec
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (a.bias && c + e < a.N) v[e] += (float)((const bf16*)a.bias)[c + e];
+        if (a.bias && c + e < a.N) v[e] += to_f32(((const T*)a.bias)[c + e]);
       if (i * 16 + n < rows) {
         if (wide) {
           if (c < a.N) store4(y + c, v);
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (c + e < a.N) y[c + e] = (bf16)v[e];
+            if (c + e < a.N) y[c + e] = from_f32<T>(v[e]);
         }
       }
     }
@@ -193,27 +192,27 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(Projec
   }
 }
 
-static void tiles_bytes(const ProjectArgs& a, int64_t& xb, int64_t& wb) {
-  xb = ((a.T - 1) * a.ldx + a.K) * 2;
-  wb = ((int64_t)(a.N - 1) * a.ldw + a.K) * 2;
+static void tiles_bytes(const ProjectArgs& a, int64_t size, int64_t& xb, int64_t& wb) {
+  xb = ((a.T - 1) * a.ldx + a.K) * size;
+  wb = ((int64_t)(a.N - 1) * a.ldw + a.K) * size;
 }
 
 // The DMA's offsets are 32-bit with bit 31 for "out of range"; operands of 2 GiB and more take the other kernel.
-bool project_tiles_ok(const ProjectArgs& a) {
+bool project_tiles_ok(const ProjectArgs& a, int dtype) {
   int64_t xb, wb;
-  tiles_bytes(a, xb, wb);
+  tiles_bytes(a, (int64_t)dtype_size(dtype), xb, wb);
   return xb < (1ll << 31) - 4096 && wb < (1ll << 31) - 4096;
 }
 
-template <int WM, int WN, int MI, int NJ, int OCC, int NA, int NB>
+template <typename T, int WM, int WN, int MI, int NJ, int OCC, int NA, int NB>
 static int tiles_launch(const ProjectArgs& a, hipStream_t st) {
   constexpr int BM = WM * MI * 16, BN = WN * NJ * 16, LDS = (NA * BM + NB * BN) * 128;
   static std::atomic<unsigned long long> done{0};
-  SX_TRY(ensure_max_lds((const void*)adapter_tiles_kernel<WM, WN, MI, NJ, OCC, NA, NB>, done, "adapter_tiles"));
+  SX_TRY(ensure_max_lds((const void*)adapter_tiles_kernel<T, WM, WN, MI, NJ, OCC, NA, NB>, done, "adapter_tiles"));
   int64_t xb, wb;
-  tiles_bytes(a, xb, wb);
+  tiles_bytes(a, sizeof(T), xb, wb);
   const int gm = (int)cdiv64(a.T, BM), gn = cdiv(a.N, BN);
-  hipLaunchKernelGGL((adapter_tiles_kernel<WM, WN, MI, NJ, OCC, NA, NB>), dim3((unsigned)(gm * gn)), dim3(64 * WM * WN), LDS, st, a, gm, gn, (unsigned)xb, (unsigned)wb);
+  hipLaunchKernelGGL((adapter_tiles_kernel<T, WM, WN, MI, NJ, OCC, NA, NB>), dim3((unsigned)(gm * gn)), dim3(64 * WM * WN), LDS, st, a, gm, gn, (unsigned)xb, (unsigned)wb);
   SX_LAUNCH_CHECK("adapter_tiles");
   return SX_OK;
 }
@@ -224,12 +223,15 @@ static double tiles_cost(const ProjectArgs& a, int bm, int bn, int per_cu, doubl
   return (double)cdiv64(tiles, 256 * per_cu) * per_cu * bm * bn * per_area;
 }
 
-int project_tiles_launch(const ProjectArgs& a, hipStream_t st) {
+template <typename T>
+static int tiles_pick(const ProjectArgs& a, hipStream_t st) {
   const double c0 = tiles_cost(a, 256, 256, 1, 1.0), c1 = tiles_cost(a, 128, 256, 1, 1.2), c2 = tiles_cost(a, 128, 128, 2, 1.4), c3 = tiles_cost(a, 64, 64, 4, 2.0);
-  if (c0 <= c1 && c0 <= c2 && c0 <= c3) return tiles_launch<2, 4, 8, 4, 2, 3, 2>(a, st);
-  if (c1 <= c2 && c1 <= c3) return tiles_launch<2, 4, 4, 4, 2, 3, 3>(a, st);
-  if (c2 <= c3) return tiles_launch<2, 2, 4, 4, 2, 3, 2>(a, st);
-  return tiles_launch<1, 4, 4, 1, 4, 3, 3>(a, st);
+  if (c0 <= c1 && c0 <= c2 && c0 <= c3) return tiles_launch<T, 2, 4, 8, 4, 2, 3, 2>(a, st);
+  if (c1 <= c2 && c1 <= c3) return tiles_launch<T, 2, 4, 4, 4, 2, 3, 3>(a, st);
+  if (c2 <= c3) return tiles_launch<T, 2, 2, 4, 4, 2, 3, 2>(a, st);
+  return tiles_launch<T, 1, 4, 4, 1, 4, 3, 3>(a, st);
 }
+
+int project_tiles_launch(const ProjectArgs& a, int dtype, hipStream_t st) { return dtype == SX_BF16 ? tiles_pick<bf16>(a, st) : tiles_pick<float>(a, st); }
 
 }  // namespace sx

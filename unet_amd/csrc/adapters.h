@@ -42,9 +42,18 @@ struct ProjectArgs {
   void* y; int64_t ldy;
 };
 
-// the shared product on large bf16 tiles (adapter_tiles.hip); false: not for this kernel
-bool project_tiles_ok(const ProjectArgs& a);
-int project_tiles_launch(const ProjectArgs& a, hipStream_t st);
+// a lane's 16 bytes of h (row m, ranks from j0 on), and the first of the ranks whose factors they meet
+template <typename T>
+__device__ __forceinline__ int h_rank(int gq) { return sizeof(T) == 2 ? (gq & 1) * 8 : gq * 4; }
+template <typename T>
+__device__ __forceinline__ typename Elem<T>::Vec load_h(const ProjectArgs& a, int64_t m, int j0, int gq) {
+  const T* h = (const T*)a.h + (sizeof(T) == 2 ? m * (2 * a.rp) + j0 * 2 + gq * 8 : m * a.rp + j0 + gq * 4);
+  return *reinterpret_cast<const typename Elem<T>::Vec*>(h);
+}
+
+// the shared product by tiles (adapter_tiles.hip); false: not for this kernel
+bool project_tiles_ok(const ProjectArgs& a, int dtype);
+int project_tiles_launch(const ProjectArgs& a, int dtype, hipStream_t st);
 
 // a few rows, forward alone (adapter_tokens.hip)
 constexpr int kTokens = 64;

@@ -215,7 +215,7 @@ __global__ __launch_bounds__(64 * NW) void adapter_shrink_kernel(ShrinkArgs a) {
   }
 }
 
-// ------------------------------------------------------------------ project (fp32, and bf16 operands of 2 GiB and more)
+// ------------------------------------------------------------------ project (operands of 2 GiB and more; adapter_tiles.hip has the others)
 // A block's tile is BM sorted rows x BN columns: four waves of (BM / 2) x (BN / 2), K steps of 128 bytes through LDS
 template <typename T, int BM, int BN>
 __global__ __launch_bounds__(256) void adapter_project_kernel(ProjectArgs a) {
@@ -270,17 +270,14 @@ __global__ __launch_bounds__(256) void adapter_project_kernel(ProjectArgs a) {
     const int end = (int)std::min<int64_t>(rows, a.end[g] - m0);
     const T* qg = (const T*)a.q + g * a.q_g;
     for (int j0 = 0; j0 < a.r; j0 += 16) {
-      const int jr = j0 + (sizeof(T) == 2 ? (gq & 1) * 8 : gq * 4);
       Vec bv[NI];
 #pragma unroll
-      for (int j = 0; j < NI; ++j) bv[j] = load_piece<T>(qg + (int64_t)std::min(n0 + wn + j * 16 + n, a.N - 1) * a.q_ld, jr, a.q_ld);
+      for (int j = 0; j < NI; ++j) bv[j] = load_piece<T>(qg + (int64_t)std::min(n0 + wn + j * 16 + n, a.N - 1) * a.q_ld, j0 + h_rank<T>(gq), a.q_ld);
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
         const int f = wm + i * 16;
         if (f >= end || f + 16 <= at) continue;
-        const int64_t m = m0 + std::min(f + n, rows - 1);
-        const T* h = (const T*)a.h + (sizeof(T) == 2 ? m * (2 * a.rp) + j0 * 2 + gq * 8 : m * a.rp + j0 + gq * 4);
-        const Vec av = *reinterpret_cast<const Vec*>(h);
+        const Vec av = load_h<T>(a, m0 + std::min(f + n, rows - 1), j0, gq);
 #pragma unroll
         for (int j = 0; j < NI; ++j) {
           const f32x4 z = {0.f, 0.f, 0.f, 0.f};
@@ -545,12 +542,8 @@ static int shrink_launch(const ShrinkArgs& a, hipStream_t st) {
 
 template <typename T>
 static int project_launch(const ProjectArgs& a, hipStream_t st) {
-  if (sizeof(T) == 2 && project_tiles_ok(a)) return project_tiles_launch(a, st);
-  if (cdiv64(a.T, 128) * cdiv(a.N, 128) >= 256) {
-    hipLaunchKernelGGL((adapter_project_kernel<T, 128, 128>), dim3((unsigned)cdiv64(a.T, 128), cdiv(a.N, 128)), dim3(256), 0, st, a);
-  } else {
-    hipLaunchKernelGGL((adapter_project_kernel<T, 64, 64>), dim3((unsigned)cdiv64(a.T, 64), cdiv(a.N, 64)), dim3(256), 0, st, a);
-  }
+  if (project_tiles_ok(a, Elem<T>::kDtype)) return project_tiles_launch(a, Elem<T>::kDtype, st);
+  hipLaunchKernelGGL((adapter_project_kernel<T, 128, 128>), dim3((unsigned)cdiv64(a.T, 128), cdiv(a.N, 128)), dim3(256), 0, st, a);
   SX_LAUNCH_CHECK("adapter_project");
   return SX_OK;
 }
