@@ -14,7 +14,7 @@ from .train import train_unet, TrainEngine
 from .predict import load_checkpoint, predict_fields, predict_te, predict_fields_batch, scale_params
 from .utils import (pick_device, sample_from_loader, eval_param2z_one, nearest_neighbor_in_Z, scale_params_for_inference,
                     save_geometry_h5, fp32_exact)
-from .latent import (extract_z_dataset, ParamToZ, ZToParam, train_param2z, train_z2param,   # noqa: F811  (as the reference,
+from .latent import (extract_z_dataset, ParamToZ, ZToParam, AdaptedMLP, train_param2z, train_z2param,   # noqa: F811  (as the reference,
                      train_cycle_consistent)                                              # latent.ParamToZ wins)
 from .data import ResidentLoader
 
@@ -26,5 +26,5 @@ __all__ = [
     "predict_fields", "predict_te", "predict_fields_batch", "scale_params", "pick_device", "sample_from_loader", "eval_param2z_one",
     "nearest_neighbor_in_Z", "scale_params_for_inference", "save_geometry_h5", "extract_z_dataset", "ZToParam", "train_param2z", "train_z2param",
     "train_cycle_consistent", "ResidentLoader", "fp32_exact", "distillation_loss", "scaled_embedding", "ScaledEmbedding", "adapter_linear",
-    "AdapterLinear",
+    "AdapterLinear", "AdaptedMLP",
 ]

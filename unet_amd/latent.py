@@ -182,6 +182,26 @@ class ZToParam(_MLP):
         self.net = _build(z_dim, P, hidden, dropout, use_layernorm)
 
 
+class AdaptedMLP(nn.Module):
+    """A trained `ParamToZ` / `ZToParam` kept frozen, with `num` low-rank adapters beside every Linear: one set of weights for many
+    machines or scenarios.  `forward(x, ids)` takes rows of any of them at once (ids as in `adapters.adapter_linear`; -1: the shared
+    MLP alone); activations, LayerNorm and Dropout are the shared MLP's own modules.  Trains through autograd: only the adapters
+    have gradients."""
+
+    def __init__(self, mlp, num, rank, alpha=None):
+        super().__init__()
+        from .adapters import AdapterLinear
+        for p in mlp.parameters():
+            p.requires_grad_(False)
+        self.net = nn.ModuleList([AdapterLinear(m, num, rank, alpha) if isinstance(m, nn.Linear) else m for m in mlp.net])
+
+    def forward(self, x, ids):
+        from .adapters import AdapterLinear
+        for m in self.net:
+            x = m(x, ids) if isinstance(m, AdapterLinear) else m(x)
+        return x
+
+
 # ---------------------------------------------------------------------------------------------- training engine
 class _Trainer:
     """Flat fp32 arenas (parameters, gradients, Adam moments) over one or two MLPs; clip 1.0 + AdamW in two launches
