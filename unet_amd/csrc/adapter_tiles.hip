@@ -129,55 +129,66 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(Projec
   // masking h alone would let a NaN or an infinity of one adapter reach the others' rows as 0 * NaN.
   const int64_t w0 = m0 + wm * MI * 16;
   const int rows = (int)std::min<int64_t>(MI * 16, a.T - w0);
+  if (rows <= 0) return;
+  int at_y[MI], own[MI];                                      // all rows' places and adapters at once: one latency
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int64_t m = w0 + std::min(i * 16 + n, rows - 1);
+    at_y[i] = a.perm[m];
+    own[i] = a.key[m];
+  }
+  f32x4 bias[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bias[j][e] = a.bias ? to_f32(((const T*)a.bias)[std::min(n0 + (wn * NJ + j) * 16 + 4 * gq + e, a.N - 1)]) : 0.f;
   auto q_piece = [&](int g, int j, int j0) {
     const int c = std::min(n0 + (wn * NJ + j) * 16 + n, a.N - 1);
     return load_piece<T>((const T*)a.q + g * a.q_g + (int64_t)c * a.q_ld, j0 + h_rank<T>(gq), a.q_ld);
   };
   auto h_piece = [&](int i, int j0) { return load_h<T>(a, w0 + std::min(i * 16 + n, rows - 1), j0, gq); };
-  for (int at = 0; at < rows;) {
-    const int g = __builtin_amdgcn_readfirstlane(a.key[w0 + at]);
-    if (g >= a.G) break;                                      // the rows without an adapter come last
-    const int end = (int)std::min<int64_t>(rows, __builtin_amdgcn_readfirstlane(a.end[g]) - w0);
-    for (int j0 = 0; j0 < a.r; j0 += 16) {
-      Vec qf[NJ];
+  auto front = [&](int i) { return __builtin_amdgcn_readlane(own[i], 0); };
+  auto back = [&](int i) { return __builtin_amdgcn_readlane(own[i], 15); };
+  for (int j0 = 0; j0 < a.r && front(0) < a.G; j0 += 16) {    // (the rows without an adapter come last)
+    Vec hf[MI], qf[NJ];
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) qf[j] = q_piece(g, j, j0);
+    for (int i = 0; i < MI; ++i) hf[i] = h_piece(i, j0);
+    int g = -1;
 #pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        if (i * 16 < at || i * 16 >= end || std::min(i * 16 + 16, rows) > end) continue;
-        const Vec hf = h_piece(i, j0);
+    for (int i = 0; i < MI; ++i) {
+      const int gi = front(i);
+      if (gi != back(i) || gi >= a.G) continue;
+      if (gi != g) {
+        g = gi;
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[i][j] = Mma<T>::run(qf[j], hf, acc[i][j]);
+        for (int j = 0; j < NJ; ++j) qf[j] = q_piece(g, j, j0);
       }
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[i][j] = Mma<T>::run(qf[j], hf[i], acc[i][j]);
     }
-    at = end;
   }
   const bool wide = a.N % 4 == 0 && a.ldy % 4 == 0 && (uintptr_t)a.y % (4 * E) == 0;
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     if (i * 16 >= rows) continue;
-    const int64_t m = w0 + std::min(i * 16 + n, rows - 1);
-    const int mine = a.key[m], last = std::min(i * 16 + 15, rows - 1);
-    const int g0 = __builtin_amdgcn_readfirstlane(a.key[w0 + i * 16]), g1 = __builtin_amdgcn_readfirstlane(a.key[w0 + last]);
-    T* y = (T*)a.y + (int64_t)a.perm[m] * a.ldy;
+    const int end = std::min(i * 16 + 16, rows);
+    T* y = (T*)a.y + (int64_t)at_y[i] * a.ldy;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const int c = n0 + (wn * NJ + j) * 16 + 4 * gq;
       f32x4 v = acc[i][j];
-      if (g0 != g1) {
-        for (int at = i * 16; at <= last;) {
+      if (front(i) != back(i)) {
+        for (int at = i * 16; at < end;) {
           const int g = __builtin_amdgcn_readfirstlane(a.key[w0 + at]);
           if (g >= a.G) break;
           f32x4 d = {0.f, 0.f, 0.f, 0.f};
           for (int j0 = 0; j0 < a.r; j0 += 16) d = Mma<T>::run(q_piece(g, j, j0), h_piece(i, j0), d);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] += mine == g ? d[e] : 0.f;
-          at = (int)std::min<int64_t>(last + 1, __builtin_amdgcn_readfirstlane(a.end[g]) - w0);
+          for (int e = 0; e < 4; ++e) v[e] += own[i] == g ? d[e] : 0.f;
+          at = (int)std::min<int64_t>(end, __builtin_amdgcn_readfirstlane(a.end[g]) - w0);
         }
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (a.bias && c + e < a.N) v[e] += to_f32(((const T*)a.bias)[c + e]);
+      v += bias[j];
       if (i * 16 + n < rows) {
         if (wide) {
           if (c < a.N) store4(y + c, v);
