@@ -173,29 +173,37 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(Projec
     if (i * 16 >= rows) continue;
     const int end = std::min(i * 16 + 16, rows);
     T* y = (T*)a.y + (int64_t)at_y[i] * a.ldy;
+    f32x4 v[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) v[j] = acc[i][j];
+    if (front(i) != back(i)) {
+      for (int at = i * 16; at < end;) {
+        const int g = __builtin_amdgcn_readfirstlane(a.key[w0 + at]);
+        if (g >= a.G) break;
+        f32x4 d[NJ] = {};
+        for (int j0 = 0; j0 < a.r; j0 += 16) {
+          const Vec hf = h_piece(i, j0);
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) d[j] = Mma<T>::run(q_piece(g, j, j0), hf, d[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[j][e] += own[i] == g ? d[j][e] : 0.f;
+        at = (int)std::min<int64_t>(end, __builtin_amdgcn_readfirstlane(a.end[g]) - w0);
+      }
+    }
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const int c = n0 + (wn * NJ + j) * 16 + 4 * gq;
-      f32x4 v = acc[i][j];
-      if (front(i) != back(i)) {
-        for (int at = i * 16; at < end;) {
-          const int g = __builtin_amdgcn_readfirstlane(a.key[w0 + at]);
-          if (g >= a.G) break;
-          f32x4 d = {0.f, 0.f, 0.f, 0.f};
-          for (int j0 = 0; j0 < a.r; j0 += 16) d = Mma<T>::run(q_piece(g, j, j0), h_piece(i, j0), d);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] += own[i] == g ? d[e] : 0.f;
-          at = (int)std::min<int64_t>(end, __builtin_amdgcn_readfirstlane(a.end[g]) - w0);
-        }
-      }
-      v += bias[j];
+      v[j] += bias[j];
       if (i * 16 + n < rows) {
         if (wide) {
-          if (c < a.N) store4(y + c, v);
+          if (c < a.N) store4(y + c, v[j]);
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (c + e < a.N) y[c + e] = from_f32<T>(v[e]);
+            if (c + e < a.N) y[c + e] = from_f32<T>(v[j][e]);
         }
       }
     }

@@ -118,7 +118,7 @@ struct ShrinkArgs {
 // MT * 16 sorted rows and RT * 16 ranks per block; its NW waves split the columns
 template <typename T, int MT, int RT, int NW>
 __global__ __launch_bounds__(64 * NW) void adapter_shrink_kernel(ShrinkArgs a) {
-  constexpr int EPL = Elem<T>::EPL, CK = Elem<T>::CK, RJ = RT * 16, U = MT + RT <= 2 ? 8 : 4;      // U: chunks in flight per wave
+  constexpr int EPL = Elem<T>::EPL, CK = Elem<T>::CK, RJ = RT * 16, U = MT == 1 && RT <= 2 ? 8 : 4;      // U: chunks in flight per wave
   typedef typename Elem<T>::Vec Vec;
   __shared__ float red[NW][MT * 16][RJ + 1];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, n = lane & 15, gq = lane >> 4;
@@ -523,16 +523,20 @@ static AdapterWs adapter_ws(int dtype, int64_t T, int K, int N, int r, int G, bo
 
 template <typename T>
 static int shrink_launch(const ShrinkArgs& a, hipStream_t st) {
-  // 32 rows share an adapter's factor once there are rows enough for two such blocks a CU; below, 16 rows and twice the waves
-  const bool big = a.T >= 32 * 512;
+  // 32 rows share an adapter's factor once there are rows enough for two such blocks a CU; below, 16 rows and, up to one block a CU, sixteen
+  // waves.  (32 rows from 8192 rows on: 32 us against 27 at 8192 x 4096, rank 16.)
   const int rt = a.rp <= 16 ? 1 : a.rp <= 32 ? 2 : 4;
-  const dim3 grid((unsigned)cdiv64(a.T, big ? 32 : 16), cdiv(a.rp, rt * 16));
-  if (big) {
+  if (a.T >= 32 * 512) {
+    const dim3 grid((unsigned)cdiv64(a.T, 32), cdiv(a.rp, rt * 16));
     if (rt == 1) hipLaunchKernelGGL((adapter_shrink_kernel<T, 2, 1, 4>), grid, dim3(256), 0, st, a);
     else if (rt == 2) hipLaunchKernelGGL((adapter_shrink_kernel<T, 2, 2, 4>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((adapter_shrink_kernel<T, 2, 4, 4>), grid, dim3(256), 0, st, a);
   } else {
-    if (rt == 1) hipLaunchKernelGGL((adapter_shrink_kernel<T, 1, 1, 8>), grid, dim3(512), 0, st, a);
+    const dim3 grid((unsigned)cdiv64(a.T, 16), cdiv(a.rp, rt * 16));
+    const bool wide = a.T <= 16 * 256 && a.C >= 16 * Elem<T>::CK;
+    if (rt == 1 && wide) hipLaunchKernelGGL((adapter_shrink_kernel<T, 1, 1, 16>), grid, dim3(1024), 0, st, a);
+    else if (rt == 1) hipLaunchKernelGGL((adapter_shrink_kernel<T, 1, 1, 8>), grid, dim3(512), 0, st, a);
+    else if (rt == 2 && wide) hipLaunchKernelGGL((adapter_shrink_kernel<T, 1, 2, 16>), grid, dim3(1024), 0, st, a);
     else if (rt == 2) hipLaunchKernelGGL((adapter_shrink_kernel<T, 1, 2, 8>), grid, dim3(512), 0, st, a);
     else hipLaunchKernelGGL((adapter_shrink_kernel<T, 1, 4, 8>), grid, dim3(512), 0, st, a);
   }

@@ -65,11 +65,16 @@ __global__ __launch_bounds__(1024) void sort_ids_kernel(const I* __restrict__ id
   };
   if constexpr (KEEP)
     if (n > 0) load(s0, true);
-  for (int w = 0; w < kSortWaves; ++w)
-    cnt[w][tid] = 0;
+  for (int w = 0; w < kSortWaves; ++w) cnt[w][tid] = 0;
   __syncthreads();
   each([&](int64_t t0) {
     if constexpr (!KEEP) load(t0, true);
+    if (q.bits == 0) {                                     // one bucket per block: counted without atomics
+      int c = 0;
+      unrolled<U>([&](auto u) { c += __popcll(__ballot(r[u] >= 0)); });
+      if (lane == 0) cnt[wid][0] += c;
+      return;
+    }
     unrolled<U>([&](auto u) {
       if (r[u] >= 0) atomicAdd(&cnt[wid][r[u]], 1);
     });
@@ -106,8 +111,21 @@ __global__ __launch_bounds__(1024) void sort_ids_kernel(const I* __restrict__ id
     }
   }
   __syncthreads();
+  int next = cnt[wid][0];                                  // one bucket per block: where this wave's next entry goes
   each([&](int64_t t0) {
     if constexpr (!KEEP) load(t0, false);
+    if (q.bits == 0) {
+      unrolled<U>([&](auto u) {
+        const unsigned long long same = __ballot(r[u] >= 0);
+        if (r[u] >= 0) {
+          const int p = next + __popcll(same & ((1ull << lane) - 1));
+          perm[p] = (int)(t0 + u * 64 + lane);
+          key[p] = me;
+        }
+        next += __popcll(same);
+      });
+      return;
+    }
     unrolled<U>([&](auto u) {
       const int ru = r[u];
       unsigned long long same = __ballot(ru >= 0);
