@@ -413,7 +413,8 @@ int sx_adapter_backward(int dtype, int64_t T, int K, int N, int r, int G, const 
 
 /* ---------------------------------------------------------------------------------------------
  * Distillation from a teacher's top logits.  Row t: student logits z (V, `dtype`, row stride ld), K pairs (idx, top) of the
- * teacher (contiguous; top in top_dtype, idx int64 or int32); a pair whose index is outside [0, V) is ignored.
+ * teacher (contiguous; top in top_dtype, idx int64 or int32); a pair whose index is outside [0, V) or whose logit is
+ * -inf is ignored.
  *   p = softmax(top / tau) over the row's valid pairs, q = softmax(z / tau)
  *   loss_t = tau^2 * weights[t] * sum_k p_k (log p_k - log q_{idx_k});   d loss_t / d z_v = tau * weights[t] * (q_v - sum_{idx_k = v} p_k)
  * A row of weight 0 or without a valid pair has loss 0 and gradient 0, whatever its logits hold.  weights: [N] fp32, NULL = 1.

@@ -169,6 +169,31 @@ def test_lowest_values_and_infinities_in_the_vocabulary(dtype):
     _check(z, top, idx % 300, 1.0)
 
 
+@pytest.mark.parametrize("K", [5, 300])
+def test_teacher_rows_without_mass(K):
+    """A row whose teacher logits are all -inf has no entry left, also next to padding; one finite entry among them takes all the mass."""
+    z, top, idx = _inputs((5,), 700, K)
+    with torch.no_grad():
+        top[0] = float("-inf")
+        top[1] = float("-inf")
+        idx[1, ::2] = -1
+        top[2, 1:] = float("-inf")
+        z[0, 3] = float("nan")
+    from unet_amd.losses import distillation_loss
+    for red in ("mean", "none"):
+        loss = distillation_loss(z, top, idx, reduction=red)
+        (grad,) = torch.autograd.grad(loss, (z,), torch.full_like(loss, 2.0))
+        assert torch.isfinite(loss).all() and torch.isfinite(grad).all() and not grad[:2].any()
+    assert not loss.detach()[:2].any()
+    z2 = z.detach().clone()
+    z2[0] = 0.0
+    idx[:2] = -1
+    top[:2] = 0.0
+    rl, rg, lt, gt = _ref(z2, top, idx, 1.0, None, "none", torch.full((5,), 2.0))
+    assert ((loss.detach().double().cpu() - rl).abs() <= lt + U * rl.abs()).all()
+    assert ((grad.double().cpu() - rg).abs() <= gt + 1.01 * 2 * U * rg.abs() + 1e-38).all()
+
+
 def test_strided_and_misaligned_logits():
     g = torch.Generator().manual_seed(1)
     for dtype in (torch.float32, torch.bfloat16):

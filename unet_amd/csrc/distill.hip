@@ -1,6 +1,6 @@
 // Distillation from a teacher's top logits: the loss of a row of student logits z against K (index, logit) pairs and its gradient.
 //
-//   p      = softmax over the row's valid pairs of top / tau          (valid: 0 <= index < V)
+//   p      = softmax over the row's valid pairs of top / tau          (valid: 0 <= index < V, top not -inf)
 //   log q  = z / tau - lse(z / tau)
 //   loss   = tau^2 * sum_k p_k (log p_k - log q_{idx_k})              (tau^2 keeps the gradient's size as tau changes)
 //   dz_v   = c * (q_v - sum_{k: idx_k = v} p_k),   c = tau * weight / den
@@ -198,9 +198,9 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
     int nh, nb;
     shape(z, nh, nb);
     const bool has_loose = tid < a.V - nb * E;
-    const bool paired = w != 0.f && tid < a.K && pair_raw >= 0 && pair_raw < a.V;
-    const int pi = paired ? (int)pair_raw : -1;
     const float pt = __builtin_bit_cast(float, a.top_bf16 ? top_raw << 16 : top_raw);
+    const bool paired = w != 0.f && tid < a.K && pair_raw >= 0 && pair_raw < a.V && pt != -INFINITY;
+    const int pi = paired ? (int)pair_raw : -1;
     const float zp = paired ? to_f32(z[pi]) : 0.f;
     const float zl = to_f32(loose);
     float m = kFloor, s = 0.f;
@@ -331,7 +331,7 @@ __global__ __launch_bounds__(NT) void distill_wide_kernel(DistillArgs a, int gra
   float tm = -INFINITY, any = 0.f;
   for (int k = tid; k < a.K; k += NT) {
     const int64_t id = pair_idx(a, k0 + k);
-    if (id >= 0 && id < a.V) { tm = fmaxf(tm, pair_top(a, k0 + k)); any = 1.f; }
+    if (id >= 0 && id < a.V && pair_top(a, k0 + k) != -INFINITY) { tm = fmaxf(tm, pair_top(a, k0 + k)); any = 1.f; }
   }
   tm = all_max<NT>(tm, red);
   any = all_max<NT>(any, red);

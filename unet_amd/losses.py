@@ -205,8 +205,8 @@ def distillation_loss(logits, top_logits, top_idx, *, temperature=1.0, weights=N
     """Distillation of `logits` (..., V) from a teacher's top logits: `top_logits` (..., K) at the indices `top_idx` (..., K).
 
     loss = tau^2 * sum_k p_k (log p_k - log q_k) with p = softmax(top_logits / tau) over the row's K entries and q = softmax(logits /
-    tau) over all V.  An entry whose index is outside [0, V) (-1 by convention) is ignored; a row without any entry left or of
-    weight 0 has loss 0 and gradient 0, whatever its logits hold.  `weights` (...): per row, or a mask.  reduction: "mean" =
+    tau) over all V.  An entry whose index is outside [0, V) (-1 by convention) or whose logit is -inf is ignored; a row without any
+    entry left or of weight 0 has loss 0 and gradient 0, whatever its logits hold.  `weights` (...): per row, or a mask.  reduction: "mean" =
     sum / max(sum weights, 1e-8), "sum", or "none" (a loss per row, weights included).  fp32 / bf16 logits, fp32 arithmetic, an fp32
     loss; the gradient has the logits' dtype and only goes to the logits.  Not differentiable twice."""
     who = "distillation_loss"
