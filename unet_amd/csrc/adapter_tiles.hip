@@ -51,6 +51,9 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(Projec
     const int c = n0 + q * RPR + (tid >> 3);
     wo[q] = c < a.N ? (unsigned)(c * a.ldw * E) + piece * 16 : 0x80000000u;
   }
+  const int64_t w0 = m0 + wm * MI * 16;
+  const int rows = (int)std::min<int64_t>(MI * 16, a.T - w0);      // of this wave; <= 0: none, but it takes part in the DMA and the barriers
+  const int g_first = __builtin_amdgcn_readfirstlane(a.key[std::min(w0, a.T - 1)]);
   const int nst = (a.K + KS - 1) / KS;
   char* const sx = smem;
   char* const sw = smem + NA * SA;
@@ -127,8 +130,6 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(Projec
   // The adapters that this wave's rows meet, 16 ranks at a time, as one more short K step each.  A fragment of 16 rows that one adapter
   // owns takes it in its accumulators; one that several share gets each adapter's product apart and picks its rows, in the epilogue:
   // masking h alone would let a NaN or an infinity of one adapter reach the others' rows as 0 * NaN.
-  const int64_t w0 = m0 + wm * MI * 16;
-  const int rows = (int)std::min<int64_t>(MI * 16, a.T - w0);
   if (rows <= 0) return;
   int at_y[MI], own[MI];                                      // all rows' places and adapters at once: one latency
 #pragma unroll
@@ -137,11 +138,6 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(Projec
     at_y[i] = a.perm[m];
     own[i] = a.key[m];
   }
-  f32x4 bias[NJ];
-#pragma unroll
-  for (int j = 0; j < NJ; ++j)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) bias[j][e] = a.bias ? to_f32(((const T*)a.bias)[std::min(n0 + (wn * NJ + j) * 16 + 4 * gq + e, a.N - 1)]) : 0.f;
   auto q_piece = [&](int g, int j, int j0) {
     const int c = std::min(n0 + (wn * NJ + j) * 16 + n, a.N - 1);
     return load_piece<T>((const T*)a.q + g * a.q_g + (int64_t)c * a.q_ld, j0 + h_rank<T>(gq), a.q_ld);
@@ -149,11 +145,13 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(Projec
   auto h_piece = [&](int i, int j0) { return load_h<T>(a, w0 + std::min(i * 16 + n, rows - 1), j0, gq); };
   auto front = [&](int i) { return __builtin_amdgcn_readlane(own[i], 0); };
   auto back = [&](int i) { return __builtin_amdgcn_readlane(own[i], 15); };
-  for (int j0 = 0; j0 < a.r && front(0) < a.G; j0 += 16) {    // (the rows without an adapter come last)
+  for (int j0 = 0; j0 < a.r && g_first < a.G; j0 += 16) {     // (the rows without an adapter come last)
     Vec hf[MI], qf[NJ];
+    int g = g_first;                                          // known since the start: nothing to wait for in the usual case
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) qf[j] = q_piece(g, j, j0);
 #pragma unroll
     for (int i = 0; i < MI; ++i) hf[i] = h_piece(i, j0);
-    int g = -1;
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
       const int gi = front(i);
@@ -167,6 +165,11 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(Projec
       for (int j = 0; j < NJ; ++j) acc[i][j] = Mma<T>::run(qf[j], hf[i], acc[i][j]);
     }
   }
+  f32x4 bias[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bias[j][e] = a.bias ? to_f32(((const T*)a.bias)[std::min(n0 + (wn * NJ + j) * 16 + 4 * gq + e, a.N - 1)]) : 0.f;
   const bool wide = a.N % 4 == 0 && a.ldy % 4 == 0 && (uintptr_t)a.y % (4 * E) == 0;
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
