@@ -597,7 +597,7 @@ static int adapter_forward(const AdapterCall& c, const void* ids, int ids64, voi
     B = ws + o.B;
   }
   SX_TRY(pk.launch<T>(st));
-  SX_TRY(launch_sort_ids(ids, ids64, c.T, c.G, false, perm, key, start, end, st));
+  SX_TRY(launch_sort_ids(ids, ids64, c.T, c.G, perm, key, start, end, st));
   ShrinkArgs s = {};
   s.x = x; s.ldx = ldx; s.p = A; s.p_g = (int64_t)c.r * Kp; s.p_ld = Kp; s.scales = c.scales; s.perm = perm; s.key = key; s.start = start; s.end = end;
   s.T = c.T; s.C = Kp; s.r = c.r; s.G = c.G; s.rp = k.rp; s.h = kept + k.h; s.ht = sizeof(T) == 2 ? (bf16*)(kept + k.ht) : nullptr; s.ldt = k.ldt;

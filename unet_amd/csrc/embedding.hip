@@ -325,6 +325,6 @@ extern "C" int sx_embedding_backward(int dtype, int64_t n, int64_t rows, int dim
   q.dout = dout; q.ld = ld; q.rows = rows; q.dim = dim; q.n = n; q.scale = scale; q.dtable = dtable;
   q.perm = (int*)(ws + w.perm); q.key = (int*)(ws + w.key); q.start = (int*)(ws + w.start); q.end = (int*)(ws + w.end); q.part = (float*)(ws + w.part);
   hipStream_t st = (hipStream_t)stream;
-  SX_TRY(launch_sort_ids(ids, ids64, n, rows, true, (int*)q.perm, (int*)q.key, (int*)q.start, (int*)q.end, st));
+  SX_TRY(launch_sort_ids(ids, ids64, n, rows, (int*)q.perm, (int*)q.key, (int*)q.start, (int*)q.end, st));
   return dtype == SX_BF16 ? embed_bwd<bf16>(q, st) : embed_bwd<float>(q, st);
 }

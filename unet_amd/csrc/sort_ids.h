@@ -8,9 +8,8 @@ namespace sx {
 //   perm [n]          position of the i-th entry in bucket order (equal ids keep their order)
 //   key  [n]          its bucket
 //   start[rows + 1], end[rows + 1]   first entry of each bucket and the one behind its last
-// spread = false: the buckets follow one another, `rows` last.  spread = true: in no particular order (cheaper where a few neighbouring
-// ids take most of the entries).  One launch, no scratch memory, the same result on every run.
-int launch_sort_ids(const void* ids, int ids64, int64_t n, int64_t rows, bool spread, int* perm, int* key, int* start, int* end,
+// The buckets follow one another, `rows` last.  One launch, no scratch memory, the same result on every run.
+int launch_sort_ids(const void* ids, int ids64, int64_t n, int64_t rows, int* perm, int* key, int* start, int* end,
                     hipStream_t st);
 
 }  // namespace sx
