@@ -259,3 +259,39 @@ def test_no_gradient_wanted():
         b = distillation_loss(z, top, idx)
     assert not a.requires_grad and not b.requires_grad and torch.equal(a, b)
     assert torch.equal(a, distillation_loss(z, top, idx).detach())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_highest_values(dtype):
+    """Rows whose logits lie near the type's largest value: their product with log2 e has no room in 32 bits, their differences do."""
+    top_value = torch.finfo(dtype).max
+    z, top, idx = _inputs((3,), 600, 8, dtype)
+    with torch.no_grad():
+        z[0] = top_value
+        z[1] = top_value
+        z[1, 300:] = top_value / 2
+        z[2] = torch.finfo(dtype).min
+        z[2, :300] = top_value
+    _check(z, top, idx % 300, 1.0)
+    _check(z, top, idx % 300, 2.0, None, "none")
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("wanted", [False, True])
+def test_more_rows_than_blocks(reduction, wanted):
+    """Several rows per block, rows of weight 0 (with NaN logits) among them, so that a row's loads pass over them; with and without
+    a gradient."""
+    from unet_amd.losses import distillation_loss
+    N = 2048 * 2 + 77
+    z, top, idx = _inputs((N,), 301, 4, torch.bfloat16)
+    w = torch.rand(N, generator=torch.Generator().manual_seed(5)).cuda() + 0.5
+    w[::3] = 0.0
+    w[2048:2060] = 0.0
+    with torch.no_grad():
+        z[::3] = float("nan")
+    if wanted:
+        _check(z, top, idx, 1.5, w, reduction)
+        return
+    want, _, ltol, _ = _ref(z, top, idx, 1.5, w, reduction)
+    got = distillation_loss(z.detach(), top, idx, temperature=1.5, weights=w, reduction=reduction)
+    assert bool(((got.double().cpu() - want).abs() <= ltol).all())

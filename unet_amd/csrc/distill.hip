@@ -82,11 +82,12 @@ __device__ __forceinline__ float mul_rn(float a, float b) {
 
 // exponent of 2 of a logit relative to the row's maximum.  z * c - m * c in one fma: m * c is rounded, but alike for all of the row (and
 // sums move from one maximum to another by the difference of the rounded products).
-// Beyond 1e30 (a row whose every logit is the type's lowest value) m * c could overflow: the difference is taken first.
+// Beyond kFar (a row whose every logit is the type's lowest value) m * c could overflow: the difference is taken first.
+constexpr float kFar = 1e30f;
 struct Expo {
   float c, m, mc;
   bool far;
-  __device__ __forceinline__ Expo(float m_, float c_) : c(c_), m(m_), mc(mul_rn(m_, c_)), far(fabsf(m_) > 1e30f) {}
+  __device__ __forceinline__ Expo(float m_, float c_) : c(c_), m(m_), mc(mul_rn(m_, c_)), far(!(fabsf(m_) < kFar)) {}
   __device__ __forceinline__ float at(float z) const { return far ? (z - m) * c : fmaf(z, c, -mc); }
 };
 
@@ -124,12 +125,12 @@ template <typename T>
 __device__ __forceinline__ int row_off(const T* z) { return (int)(((uintptr_t)z & 15) / sizeof(T)); }
 
 // a thread's maximum never goes below this, so that a set without a live logit joins the others as a sum of 0
-constexpr float kFloor = -1e30f;
+constexpr float kFloor = -kFar;
 
 // Row = nh elements up to the first 16-byte boundary, nb whole vectors, the rest.  Vector v belongs to thread v % NT, register v / NT; the
 // elements before and behind the vectors to threads 0, 1, ... one each.  Pair k belongs to thread k; the gradient at its index is
 // stored once more, over the plain q of the row's other elements, behind the next barrier that the block meets anyway.
-template <typename T, int NT, int NV>
+template <typename T, int NT, int NV, bool GRAD>
 __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
   constexpr int E = Elem<T>::EPL, NW = NT / 64;
   typedef typename Elem<T>::Vec Vec;
@@ -155,11 +156,17 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
     typedef std::conditional_t<std::is_const_v<V1>, const char, char> C1;
     return reinterpret_cast<V1*>(reinterpret_cast<C1*>(base) + off);
   };
+  // vector k of a row, from its descriptor: behind the last one the load is not made, with no branch around it (a branch would leave the
+  // number of loads in flight open, and a wait for one would be a wait for all)
+  auto row_desc = [](const T* z, int nh, int nb) { return __builtin_amdgcn_make_buffer_rsrc((void*)(z + nh), 0, nb * 16, 0x00020000); };
+  auto load_vec = [&](__amdgpu_buffer_rsrc_t d, int k) { return __builtin_bit_cast(Vec, __builtin_amdgcn_raw_buffer_load_b128(d, my, k * NT * 16, 0)); };
   auto shape = [&](const T* z, int& nh, int& nb) {
     nh = std::min(a.V, (int)((16 - ((uintptr_t)z & 15)) & 15) / (int)sizeof(T));
     nb = (a.V - nh) / E;
   };
   auto weight = [&](int64_t t) { return t < a.N ? (a.weights ? a.weights[t] : 1.f) : 0.f; };
+  // a weight is the same in all lanes: its test in scalar registers, so that what it selects (the descriptors) stays there
+  auto is_zero = [](float v) { return (__builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)) & 0x7fffffff) == 0; };
   Vec r[NV];
   T loose = {};                                         // as loaded: the conversions wait until the values are needed
   int64_t pair_raw = -1;
@@ -176,53 +183,56 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
     }
   };
   int64_t row = blockIdx.x;
-  float w = weight(row);
+  float w = weight(row), wn = weight(row + gridDim.x);    // of this row and the next: loaded a row ahead, for nothing to wait on them
   {
     const T* z = (const T*)a.z + row * a.ldz;
     int nh, nb;
     shape(z, nh, nb);
-    if (w != 0.f) {
-      load_head(row, nh, nb);
+    if (is_zero(w)) nb = 0;
+    else load_head(row, nh, nb);
+    const auto d = row_desc(z, nh, nb);
 #pragma unroll
-      for (int k = 0; k < NV; ++k)
-        if (tid < nb - k * NT) r[k] = *vec_at(z + nh + k * NT * E, my);
-    }
+    for (int k = 0; k < NV; ++k) r[k] = load_vec(d, k);
   }
   T* fix_at = nullptr;                                  // the row before: where this thread's pair stands and the gradient there
   float fix = 0.f;
   for (; row < a.N; row += gridDim.x) {
     const T* z = (const T*)a.z + row * a.ldz;
-    T* dz = a.dz ? (T*)a.dz + row * a.lddz : nullptr;
+    T* dz = GRAD ? (T*)a.dz + row * a.lddz : nullptr;
     const int64_t next = row + gridDim.x;
-    const float wn = weight(next);
+    const float wnn = weight(next + gridDim.x);
     int nh, nb;
     shape(z, nh, nb);
-    const bool has_loose = tid < a.V - nb * E;
+    const bool has_loose = tid < a.V - nb * E, on = !is_zero(w), onn = !is_zero(wn);
     const float pt = __builtin_bit_cast(float, a.top_bf16 ? top_raw << 16 : top_raw);
-    const bool paired = w != 0.f && tid < a.K && pair_raw >= 0 && pair_raw < a.V && pt != -INFINITY;
+    const bool paired = on && tid < a.K && pair_raw >= 0 && pair_raw < a.V && pt != -INFINITY;
     const int pi = paired ? (int)pair_raw : -1;
     const float zp = paired ? to_f32(z[pi]) : 0.f;
     const float zl = to_f32(loose);
+    const T* zn = (const T*)a.z + next * a.ldz;
+    int nhn, nbn;
+    shape(zn, nhn, nbn);
+    if (!onn) nbn = 0;
+    const auto dn = row_desc(zn, nhn, nbn);
     float m = kFloor, s = 0.f;
-    if (w != 0.f) {
-      if (has_loose) {
-        m = fmaxf(m, zl);
-        s = __builtin_amdgcn_exp2f(fmaf(zl, c, -mul_rn(m, c)));
+    if (on && has_loose) {
+      m = fmaxf(m, zl);
+      s = __builtin_amdgcn_exp2f(fmaf(zl, c, -mul_rn(m, c)));
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (on && tid < nb - k * NT) {
+        float f[E], mk = m;
+#pragma unroll
+        for (int e = 0; e < E; ++e) { f[e] = to_f32(r[k][e]); mk = fmaxf(mk, f[e]); }
+        const float mc = mul_rn(mk, c);
+        s *= __builtin_amdgcn_exp2f(mul_rn(m, c) - mc);
+#pragma unroll
+        for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f(fmaf(f[e], c, -mc));
+        m = mk;
       }
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        if (tid < nb - k * NT) {
-          float f[E], mk = m;
-#pragma unroll
-          for (int e = 0; e < E; ++e) { f[e] = to_f32(r[k][e]); mk = fmaxf(mk, f[e]); }
-          const float mc = mul_rn(mk, c);
-          s *= __builtin_amdgcn_exp2f(mul_rn(m, c) - mc);
-#pragma unroll
-          for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f(fmaf(f[e], c, -mc));
-          m = mk;
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      if (!GRAD) r[k] = load_vec(dn, k);                // without a gradient the row has done its work
+      __builtin_amdgcn_sched_barrier(0);
     }
     {
       const float wm = wave_max(m);
@@ -243,9 +253,9 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
     float TS = lane < NW && any1 != 0.f ? red[3][ww] * expf((tm1 - TM) * it) : 0.f;
     S = wave_sum(S);
     TS = wave_sum(TS);
-    const bool live = w != 0.f && any != 0.f;
-    const bool low = live && M <= kFloor;               // no logit above the floor: the row again, from its true maximum
-    if (low) {
+    const bool live = on && any != 0.f;
+    const bool far = live && !(fabsf(M) < kFar);        // no logit above the floor, or products that overflow: the row again, by differences
+    if (far) {
       float mk = -INFINITY;
       for (int v = tid; v < a.V; v += NT) mk = fmaxf(mk, to_f32(z[v]));
       M = all_max<NT>(mk, red_kl);
@@ -276,33 +286,30 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
       a.row_loss[row] = live ? kl * a.tau * a.tau * w : 0.f;
       if (a.row_stats) keep_stats(a, row, M, S, TM, TS);
     }
-    if (dz && live && wid * 64 < a.K) {                 // the gradient at the pairs' indices, in the order of the pairs
+    if (GRAD && live && wid * 64 < a.K) {                 // the gradient at the pairs' indices, in the order of the pairs
       const Expo x(M, c);
       fix = gs * __builtin_amdgcn_exp2f(x.at(zp));
       for (int j = 0; j < a.K; ++j) fix = pair_i[j] == pi ? fmaf(-gc, pair_p[j], fix) : fix;
       if (paired) fix_at = dz + pi;
     }
-    const T* zn = (const T*)a.z + next * a.ldz;
-    int nhn, nbn;
-    shape(zn, nhn, nbn);
-    if (wn != 0.f) load_head(next, nhn, nbn);
-    else nbn = 0;
-    if (dz && has_loose && !low) dz[tid < nh ? tid : tid + nb * E] = from_f32<T>(live ? gs * __builtin_amdgcn_exp2f(fmaf(zl, c, -mc)) : 0.f);
+    if (onn) load_head(next, nhn, nbn);
+    if (GRAD && has_loose && !far) dz[tid < nh ? tid : tid + nb * E] = from_f32<T>(live ? gs * __builtin_amdgcn_exp2f(fmaf(zl, c, -mc)) : 0.f);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      if (dz && !low && tid < nb - k * NT) {
+      if (GRAD && !far && tid < nb - k * NT) {
         Vec o = {};
         if (live)
 #pragma unroll
           for (int e = 0; e < E; ++e) o[e] = from_f32<T>(gs * __builtin_amdgcn_exp2f(fmaf(to_f32(r[k][e]), c, -mc)));
         *vec_at(dz + nh + k * NT * E, my) = o;
       }
-      if (tid < nbn - k * NT) r[k] = *vec_at(zn + nhn + k * NT * E, my);
+      if (GRAD) r[k] = load_vec(dn, k);
       __builtin_amdgcn_sched_barrier(0);
     }
-    if (dz && low)
+    if (GRAD && far)
       for (int v = tid; v < a.V; v += NT) dz[v] = from_f32<T>(gs * __builtin_amdgcn_exp2f((to_f32(z[v]) - M) * c));
     w = wn;
+    wn = wnn;
   }
   __syncthreads();
   if (fix_at) *fix_at = from_f32<T>(fix);
@@ -433,7 +440,9 @@ __global__ __launch_bounds__(1024) void distill_total_kernel(const float* __rest
 
 template <typename T, int NT, int NV>
 static int rows_launch(const DistillArgs& a, int per_cu, hipStream_t st) {
-  hipLaunchKernelGGL((distill_rows_kernel<T, NT, NV>), dim3((unsigned)std::min<int64_t>(a.N, 256 * per_cu)), dim3(NT), 0, st, a);
+  const dim3 grid((unsigned)std::min<int64_t>(a.N, 256 * per_cu));
+  if (a.dz) hipLaunchKernelGGL((distill_rows_kernel<T, NT, NV, true>), grid, dim3(NT), 0, st, a);
+  else hipLaunchKernelGGL((distill_rows_kernel<T, NT, NV, false>), grid, dim3(NT), 0, st, a);
   SX_LAUNCH_CHECK("distill_rows");
   return SX_OK;
 }
