@@ -7,11 +7,16 @@
 //
 // A row of weight 0 or without a valid pair has loss 0 and gradient 0, whatever its logits hold.
 //
-// Both directions are bound by memory: what a pass cannot do without is one read of the logits and one write of the gradient.  A
-// block therefore keeps its row in registers between the two (rows_kernel): 16 threads-waves hold up to 128 Ki bf16 or 64 Ki fp32
-// logits.  Maximum and sum run in one pass (a thread rescales its sum when its maximum grows).  Blocks are persistent, and as soon as
-// a register's gradient is stored the register takes the next row's logits: the loads of a row run under the stores of the one
-// before.  Longer rows, and gradients for another upstream factor than 1, read the logits twice (wide_kernel).
+// Both directions are bound by memory: what a pass cannot do without is one read of the logits and one write of the gradient.  A block
+// therefore keeps its row in registers between the two (rows_kernel): up to 16 vectors of 16 bytes a thread, 1024 threads, 128 Ki bf16 or
+// 64 Ki fp32 logits.  Maximum and sum run in one pass (a thread rescales its sum when its maximum grows).  Blocks are persistent, and as
+// soon as a register's logits have done their work -- stored as gradients, or summed where no gradient is wanted -- the register takes
+// the next row's: the loads of a row run under the work on the one before.  Longer rows, and gradients for another upstream factor
+// than 1, read the logits twice (wide_kernel).
+//
+// Measured, bf16, 256 MB of logits: with the gradient (512 MB) rows of 32000 111 us, 4.8 TB/s, rows of 50000 118 us, of 131072 (512 MB of logits)
+// 220 us, 4.9 TB/s; loss alone 50 us, 5.4 TB/s, for rows of 8000 to 50000.  A copy of that size moves 4.9 TB/s.  Shorter rows are bound
+// by what a row costs besides (five sums over the lanes, the pairs): rows of 4000 128 us, of 1000 190 us.
 #include "sx_common.h"
 #include <algorithm>
 #include <type_traits>
@@ -74,7 +79,8 @@ __device__ __forceinline__ float pair_top(const DistillArgs& a, int64_t at) {
   return a.top_bf16 ? to_f32(((const bf16*)a.top)[at]) : ((const float*)a.top)[at];
 }
 
-// a * b rounded, never fused into a neighbouring addition
+// a * b rounded, never fused into a neighbouring addition (in a sum over lanes that would round each lane's own term, and not the others',
+// away: the sum would differ from lane to lane)
 __device__ __forceinline__ float mul_rn(float a, float b) {
 #pragma clang fp contract(off)
   return a * b;
@@ -98,7 +104,7 @@ __device__ __forceinline__ void keep_stats(const DistillArgs& a, int64_t row, fl
   a.row_stats[3 * a.N + row] = ts;
 }
 
-constexpr int kKeptPairs = 256;        // pairs per row that rows_kernel takes: one per thread of its smallest block
+constexpr int kKeptPairs = 256;        // pairs per row that rows_kernel takes at most: one per thread
 
 // E logits of a row as they lie in memory, 16 bytes from 16-byte boundaries: element e of vector v is the row's element v * E + e - off,
 // off being the row's start behind a boundary.  Elements before and behind the row read as -inf and are not stored.
@@ -132,12 +138,12 @@ constexpr float kFloor = -kFar;
 // stored once more, over the plain q of the row's other elements, behind the next barrier that the block meets anyway.
 template <typename T, int NT, int NV, bool GRAD>
 __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
-  constexpr int E = Elem<T>::EPL, NW = NT / 64;
+  constexpr int E = Elem<T>::EPL, NW = NT / 64, PAIRS = NT < kKeptPairs ? NT : kKeptPairs;
   typedef typename Elem<T>::Vec Vec;
   __shared__ float red[5][NW];                          // per wave: maximum and sum of the logits and of the teacher's, any pair
   __shared__ float red_kl[NW];
-  __shared__ float pair_p[kKeptPairs];
-  __shared__ int pair_i[kKeptPairs];
+  __shared__ float pair_p[PAIRS];
+  __shared__ int pair_i[PAIRS];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   const float it = 1.f / a.tau, c = it * kLog2e;
   float den = a.den_host;
@@ -234,25 +240,22 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
       if (!GRAD) r[k] = load_vec(dn, k);                // without a gradient the row has done its work
       __builtin_amdgcn_sched_barrier(0);
     }
-    {
-      const float wm = wave_max(m);
-      const float ws = wave_sum(s * __builtin_amdgcn_exp2f(mul_rn(m, c) - mul_rn(wm, c)));
-      const float tm = wave_max(paired ? pt : -INFINITY);
-      const float ts = wave_sum(paired ? expf((pt - tm) * it) : 0.f);
-      const bool any = __ballot(paired) != 0;
-      if (lane == 0) { red[0][wid] = wm; red[1][wid] = ws; red[2][wid] = tm; red[3][wid] = ts; red[4][wid] = any ? 1.f : 0.f; }
-    }
+    float M = wave_max(m), S = wave_sum(mul_rn(s, __builtin_amdgcn_exp2f(mul_rn(m, c) - mul_rn(M, c))));
+    float TM = wave_max(paired ? pt : -INFINITY), TS = wave_sum(paired ? expf((pt - TM) * it) : 0.f);
+    float any = __ballot(paired) ? 1.f : 0.f;
+    if (NW > 1 && lane == 0) { red[0][wid] = M; red[1][wid] = S; red[2][wid] = TM; red[3][wid] = TS; red[4][wid] = any; }
     __syncthreads();                                    // and every thread has stored its part of the row before
     if (fix_at) *fix_at = from_f32<T>(fix);
     fix_at = nullptr;
-    const int ww = lane & (NW - 1);                     // every wave's results, over the lanes
-    const float m1 = red[0][ww], tm1 = red[2][ww], any1 = red[4][ww];
-    float M = wave_max(m1);
-    const float TM = wave_max(tm1), any = wave_max(any1);
-    float S = lane < NW ? red[1][ww] * __builtin_amdgcn_exp2f(mul_rn(m1, c) - mul_rn(M, c)) : 0.f;
-    float TS = lane < NW && any1 != 0.f ? red[3][ww] * expf((tm1 - TM) * it) : 0.f;
-    S = wave_sum(S);
-    TS = wave_sum(TS);
+    if constexpr (NW > 1) {                             // every wave's results, over the lanes
+      const int ww = lane & (NW - 1);
+      const float m1 = red[0][ww], tm1 = red[2][ww], any1 = red[4][ww];
+      M = wave_max(m1);
+      TM = wave_max(tm1);
+      any = wave_max(any1);
+      S = wave_sum(lane < NW ? mul_rn(red[1][ww], __builtin_amdgcn_exp2f(mul_rn(m1, c) - mul_rn(M, c))) : 0.f);
+      TS = wave_sum(lane < NW && any1 != 0.f ? mul_rn(red[3][ww], expf((tm1 - TM) * it)) : 0.f);
+    }
     const bool live = on && any != 0.f;
     const bool far = live && !(fabsf(M) < kFar);        // no logit above the floor, or products that overflow: the row again, by differences
     if (far) {
@@ -265,7 +268,7 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
       __syncthreads();
     }
     const float gc = w * a.tau / den, gs = gc / S, mc = mul_rn(M, c);
-    if (tid < kKeptPairs) {
+    if (tid < PAIRS) {
       float p = 0.f, kl = 0.f;
       if (live && paired) {
         const float lt = (pt - TM) * it;
@@ -282,7 +285,7 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
     if (tid == 0) {
       float kl = 0.f;
 #pragma unroll
-      for (int i = 0; i < kKeptPairs / 64; ++i) kl += red_kl[i];
+      for (int i = 0; i < PAIRS / 64; ++i) kl += red_kl[i];
       a.row_loss[row] = live ? kl * a.tau * a.tau * w : 0.f;
       if (a.row_stats) keep_stats(a, row, M, S, TM, TS);
     }
@@ -468,12 +471,23 @@ static int distill_launch(const DistillArgs& a, hipStream_t st) {
   constexpr int E = Elem<T>::EPL;
   if (!rows_fit(a, Elem<T>::kDtype)) return wide_launch<T>(a, 0, st);
   const int nv = a.V / E;                               // whole vectors, at most
+  // Few vectors a thread cost little to sum over the threads, many keep more of a row's loads in flight with fewer waves to wait for one
+  // another: the latter wins nearly everywhere.  256 MB of bf16 logits with / without a gradient: rows of 1000 by one wave 190 / 91 us, by four
+  // 643 / 450; of 2000 by one 151 / 64, by two 212 / 122; of 16000 by 256 threads 117 / 50, by 512 119 / 63; of 32000 by 256 115 / 51, by 512
+  // 111 / 52; of 24000 without a gradient 50 and 58; of 50000 by 512 118 / 50, by 1024 131 / 62.
+  if (a.K <= 64) {                                      // (a pair per thread)
+    if (nv <= 64) return rows_launch<T, 64, 1>(a, 32, st);
+    if (nv <= 128) return rows_launch<T, 64, 2>(a, 32, st);
+    if (nv <= 256) return rows_launch<T, 64, 4>(a, 28, st);
+    if (nv <= 512) return rows_launch<T, 64, 8>(a, 20, st);
+    if (nv <= 1024) return rows_launch<T, 64, 16>(a, 16, st);
+  }
   if (nv <= 256) return rows_launch<T, 256, 1>(a, 8, st);
   if (nv <= 512) return rows_launch<T, 256, 2>(a, 8, st);
   if (nv <= 1024) return rows_launch<T, 256, 4>(a, 6, st);
-  if (nv <= 2048) return rows_launch<T, 512, 4>(a, 3, st);
-  if (nv <= 4096) return rows_launch<T, 512, 8>(a, 2, st);
-  if (nv <= 8192) return rows_launch<T, 1024, 8>(a, 1, st);
+  if (nv <= 2048) return rows_launch<T, 256, 8>(a, 5, st);
+  if (nv <= 4096) return a.dz ? rows_launch<T, 512, 8>(a, 2, st) : rows_launch<T, 256, 16>(a, 4, st);
+  if (nv <= 8192) return rows_launch<T, 512, 16>(a, 2, st);
   return rows_launch<T, 1024, 16>(a, 1, st);
 }
 
