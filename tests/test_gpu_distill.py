@@ -295,3 +295,35 @@ def test_more_rows_than_blocks(reduction, wanted):
     want, _, ltol, _ = _ref(z, top, idx, 1.5, w, reduction)
     got = distillation_loss(z.detach(), top, idx, temperature=1.5, weights=w, reduction=reduction)
     assert bool(((got.double().cpu() - want).abs() <= ltol).all())
+
+
+@pytest.mark.parametrize("V,K", [(301, 4), (9000, 70), (9000, 300)])
+def test_upstream_gradients_of_many_rows(V, K):
+    """Several rows per block in the gradient for other upstream factors than 1; pairs that fill more than one round of the threads."""
+    N = 8192 + 3 if V < 1000 else 1100
+    z, top, idx = _inputs((N,), V, K)
+    with torch.no_grad():
+        top[1], idx[2] = float("-inf"), -1
+    w = torch.rand(N, generator=torch.Generator().manual_seed(6)).cuda()
+    w[5::7] = 0.0
+    g = torch.randn(N, generator=torch.Generator().manual_seed(7)).cuda()
+    _check_rows(z, top, idx, w, g)
+
+
+def _check_rows(z, top, idx, w, g):
+    """As _check with reduction "none", in 64 bits on the GPU."""
+    from unet_amd.losses import distillation_loss
+    loss = distillation_loss(z, top, idx, weights=w, reduction="none")
+    (grad,) = torch.autograd.grad(loss, (z,), g)
+    zd, td = z.detach().double(), top.double()
+    ok = (idx >= 0) & (idx < z.shape[1]) & ~torch.isneginf(td)
+    p = torch.softmax(td.masked_fill(~ok, float("-inf")), 1).masked_fill(~ok.any(1, keepdim=True), 0.0)
+    q = torch.softmax(zd, 1)
+    sp = torch.zeros_like(zd).scatter_add_(1, idx.clamp_min(0).long(), p)
+    c = (g * w).double().unsqueeze(1) * ok.any(1, keepdim=True)
+    d = (torch.log(p) - torch.log(q).gather(1, idx.clamp_min(0).long())).masked_fill(~ok, 0.0)
+    want = (w.double() * (p * d).sum(1)) * ok.any(1)
+    A = 60.0                                              # logits within +-3 * 6 of one another and the teacher's within +-2 * 6
+    E = (6 * A + z.shape[1] / 64 + 64) * U
+    assert bool(((grad.double() - c * (q - sp)).abs() <= c.abs() * E * (q + sp) + 1.01 * 2 * U * (c * (q - sp)).abs() + 1e-38).all())
+    assert bool(((loss.detach().double() - want).abs() <= w.double() * (2 * E + E * d.abs().amax(1) + 8 * U * (A + math.log(z.shape[1]))) + U * want.abs()).all())

@@ -318,108 +318,122 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
   if (fix_at) *fix_at = from_f32<T>(fix);
 }
 
-// any row length, the logits read once for the maximum and the sum and once for the gradient; with grad_only, the gradient alone, from
+// any row length, the logits read once for the maximum, once for the sum and once for the gradient; with GRAD_ONLY, the gradient alone, from
 // the maxima and sums of an earlier pass.  fmaxf drops a NaN; the sum brings it back
-template <typename T, int NT>
-__global__ __launch_bounds__(NT) void distill_wide_kernel(DistillArgs a, int grad_only) {
+template <typename T, int NT, bool GRAD_ONLY>
+__global__ __launch_bounds__(NT) void distill_wide_kernel(DistillArgs a) {
   constexpr int E = Elem<T>::EPL;
   typedef typename Elem<T>::Vec Vec;
   __shared__ float red[NT / 64];
-  const int64_t row = blockIdx.x;
+  __shared__ int64_t pair_i[NT];
+  __shared__ float pair_p[NT];
   const int tid = threadIdx.x;
-  const T* z = (const T*)a.z + row * a.ldz;
-  T* dz = a.dz ? (T*)a.dz + row * a.lddz : nullptr;
-  const int off = row_off(z), nv = (a.V + off + E - 1) / E;
-  const bool whole = dz && row_off(dz) == off;
-  const float w = a.weights ? a.weights[row] : 1.f;
-  float gup = 1.f;
-  if (grad_only) {
-    gup = a.g[row * a.g_stride];
-    if (a.ready && gup == 1.f) return;         // dz still holds the forward pass's gradient, which is this one
-  }
-  const int64_t k0 = row * a.K;
-  float tm = -INFINITY, any = 0.f;
-  for (int k = tid; k < a.K; k += NT) {
-    const int64_t id = pair_idx(a, k0 + k);
-    if (id >= 0 && id < a.V && pair_top(a, k0 + k) != -INFINITY) { tm = fmaxf(tm, pair_top(a, k0 + k)); any = 1.f; }
-  }
-  tm = all_max<NT>(tm, red);
-  any = all_max<NT>(any, red);
-  if (grad_only) tm = a.row_stats[2 * a.N + row];
-  if (w == 0.f || any == 0.f) {
-    if (tid == 0) {
-      if (!grad_only) a.row_loss[row] = 0.f;
-      if (!grad_only && a.row_stats) keep_stats(a, row, 0.f, 0.f, 0.f, 0.f);
-    }
-    const Vec zero = {};
-    if (dz) for (int v = tid; v < nv; v += NT) store_row_vec<T>(dz, off, a.V, v, whole, zero);
-    return;
-  }
   const float it = 1.f / a.tau, c = it * kLog2e;
-  float ts = 0.f;
-  for (int k = tid; k < a.K; k += NT) {
-    const int64_t id = pair_idx(a, k0 + k);
-    if (id >= 0 && id < a.V) ts += expf((pair_top(a, k0 + k) - tm) * it);
-  }
-  ts = grad_only ? a.row_stats[3 * a.N + row] : all_sum<NT>(ts, red);
-  const float lts = logf(ts);
-  float m, s;
-  if (grad_only) {
-    m = a.row_stats[row];
-    s = a.row_stats[a.N + row];
-  } else {
-    m = -INFINITY;
-    for (int v = tid; v < nv; v += NT) {
-      const Vec r = load_row_vec<T>(z, off, a.V, v);
-#pragma unroll
-      for (int e = 0; e < E; ++e) m = fmaxf(m, to_f32(r[e]));
+  if (GRAD_ONLY && a.ready && a.g_stride == 0 && *a.g == 1.f) return;      // dz still holds the forward pass's gradient, which is this one
+  for (int64_t row = blockIdx.x; row < a.N; row += gridDim.x) {
+    const T* z = (const T*)a.z + row * a.ldz;
+    T* dz = a.dz ? (T*)a.dz + row * a.lddz : nullptr;
+    const int off = row_off(z), nv = (a.V + off + E - 1) / E;
+    const bool whole = dz && row_off(dz) == off;
+    const float w = a.weights ? a.weights[row] : 1.f;
+    const float gup = GRAD_ONLY ? a.g[row * a.g_stride] : 1.f;
+    if (GRAD_ONLY && a.ready && gup == 1.f) continue;
+    const int64_t k0 = row * a.K;
+    float m, s, tm, ts;                                   // ts = 0: no valid pair, otherwise >= 1 or NaN
+    if constexpr (GRAD_ONLY) {
+      m = a.row_stats[row];
+      s = a.row_stats[a.N + row];
+      tm = a.row_stats[2 * a.N + row];
+      ts = a.row_stats[3 * a.N + row];
+    } else {
+      tm = -INFINITY;
+      float any = 0.f;
+      for (int k = tid; k < a.K; k += NT) {
+        const int64_t id = pair_idx(a, k0 + k);
+        const float t = pair_top(a, k0 + k);
+        if (id >= 0 && id < a.V && t != -INFINITY) { tm = fmaxf(tm, t); any = 1.f; }
+      }
+      tm = all_max<NT>(tm, red);
+      any = all_max<NT>(any, red);
+      ts = 0.f;
+      for (int k = tid; k < a.K; k += NT) {
+        const int64_t id = pair_idx(a, k0 + k);
+        const float t = pair_top(a, k0 + k);
+        if (id >= 0 && id < a.V && t != -INFINITY) ts += expf((t - tm) * it);
+      }
+      ts = all_sum<NT>(ts, red);
+      if (any == 0.f) ts = 0.f;
+      m = s = 0.f;
     }
-    m = all_max<NT>(m, red);
-    const Expo x(m, c);
-    s = 0.f;
-    for (int v = tid; v < nv; v += NT) {
-      const Vec r = load_row_vec<T>(z, off, a.V, v);
+    const bool live = w != 0.f && !(ts == 0.f);
+    if (!GRAD_ONLY && live) {
+      m = -INFINITY;
+      for (int v = tid; v < nv; v += NT) {
+        const Vec r = load_row_vec<T>(z, off, a.V, v);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int i = v * E + e - off;
-        s += i >= 0 && i < a.V ? __builtin_amdgcn_exp2f(x.at(to_f32(r[e]))) : 0.f;
+        for (int e = 0; e < E; ++e) m = fmaxf(m, to_f32(r[e]));
+      }
+      m = all_max<NT>(m, red);
+      const Expo x(m, c);
+      for (int v = tid; v < nv; v += NT) {
+        const Vec r = load_row_vec<T>(z, off, a.V, v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const int i = v * E + e - off;
+          s += i >= 0 && i < a.V ? __builtin_amdgcn_exp2f(x.at(to_f32(r[e]))) : 0.f;
+        }
+      }
+      s = all_sum<NT>(s, red);
+    }
+    const Expo x(m, c);
+    if constexpr (!GRAD_ONLY) {
+      const float ls = logf(s), lts = logf(ts);
+      float kl = 0.f;
+      if (live)
+        for (int k = tid; k < a.K; k += NT) {
+          const int64_t id = pair_idx(a, k0 + k);
+          if (id < 0 || id >= a.V) continue;
+          const float lp = (pair_top(a, k0 + k) - tm) * it;
+          const float p = expf(lp) / ts;
+          if (!(p == 0.f)) kl += p * ((lp - lts) - (x.at(to_f32(z[id])) * kLn2 - ls));
+        }
+      kl = all_sum<NT>(kl, red);
+      if (tid == 0) {
+        a.row_loss[row] = live ? kl * a.tau * a.tau * w : 0.f;
+        if (a.row_stats) keep_stats(a, row, m, s, tm, ts);
       }
     }
-    s = all_sum<NT>(s, red);
-    if (tid == 0 && a.row_stats) keep_stats(a, row, m, s, tm, ts);
-  }
-  const Expo x(m, c);
-  if (!grad_only) {
-    const float ls = logf(s);
-    float kl = 0.f;
-    for (int k = tid; k < a.K; k += NT) {
-      const int64_t id = pair_idx(a, k0 + k);
-      if (id < 0 || id >= a.V) continue;
-      const float lp = (pair_top(a, k0 + k) - tm) * it;
-      const float p = expf(lp) / ts;
-      if (!(p == 0.f)) kl += p * ((lp - lts) - (x.at(to_f32(z[id])) * kLn2 - ls));
-    }
-    kl = all_sum<NT>(kl, red);
-    if (tid == 0) a.row_loss[row] = kl * a.tau * a.tau * w;
-  }
-  if (!dz) return;
-  const float gc = gup * w * a.tau / (a.den ? *a.den : a.den_host), gs = gc / s;
-  for (int v = tid; v < nv; v += NT) {
-    const Vec r = load_row_vec<T>(z, off, a.V, v);
-    Vec o;
+    if (!dz) continue;
+    const float gc = gup * w * a.tau / (a.den ? *a.den : a.den_host), gs = gc / s;
+    for (int v = tid; v < nv; v += NT) {
+      Vec o = {};
+      if (live) {
+        const Vec r = load_row_vec<T>(z, off, a.V, v);
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = from_f32<T>(gs * __builtin_amdgcn_exp2f(x.at(to_f32(r[e]))));
-    store_row_vec<T>(dz, off, a.V, v, whole, o);
-  }
-  __syncthreads();
-  // the teacher's entries over what was just stored; entries that name the same index all store the same value
-  for (int k = tid; k < a.K; k += NT) {
-    const int64_t id = pair_idx(a, k0 + k);
-    if (id < 0 || id >= a.V) continue;
-    float g = gs * __builtin_amdgcn_exp2f(x.at(to_f32(z[id])));
-    for (int j = 0; j < a.K; ++j)
-      if (pair_idx(a, k0 + j) == id) g = fmaf(-gc, expf((pair_top(a, k0 + j) - tm) * it) / ts, g);
-    dz[id] = from_f32<T>(g);
+        for (int e = 0; e < E; ++e) o[e] = from_f32<T>(gs * __builtin_amdgcn_exp2f(x.at(to_f32(r[e]))));
+      }
+      store_row_vec<T>(dz, off, a.V, v, whole, o);
+    }
+    if (!live) continue;
+    // the teacher's entries over what was just stored (behind the barriers below), NT pairs at a time against NT; entries that name the same
+    // index all store the same value
+    for (int kb = 0; kb < a.K; kb += NT) {
+      int64_t id = -1;
+      if (kb + tid < a.K) id = pair_idx(a, k0 + kb + tid);
+      if (id >= a.V) id = -1;
+      float g = id >= 0 ? gs * __builtin_amdgcn_exp2f(x.at(to_f32(z[id]))) : 0.f;
+      for (int jb = 0; jb < a.K; jb += NT) {
+        __syncthreads();
+        if (jb + tid < a.K) {
+          pair_i[tid] = pair_idx(a, k0 + jb + tid);
+          pair_p[tid] = expf((pair_top(a, k0 + jb + tid) - tm) * it) / ts;
+        }
+        __syncthreads();
+        for (int j = 0; j < std::min(NT, a.K - jb); ++j) g = pair_i[j] == id ? fmaf(-gc, pair_p[j], g) : g;
+      }
+      if (id >= 0) dz[id] = from_f32<T>(g);
+    }
+    __syncthreads();                                      // the pairs have been read
   }
 }
 
@@ -450,12 +464,22 @@ static int rows_launch(const DistillArgs& a, int per_cu, hipStream_t st) {
   return SX_OK;
 }
 
-template <typename T>
-static int wide_launch(const DistillArgs& a, int grad_only, hipStream_t st) {
-  if (a.V <= 4096) hipLaunchKernelGGL((distill_wide_kernel<T, 256>), dim3((unsigned)a.N), dim3(256), 0, st, a, grad_only);
-  else hipLaunchKernelGGL((distill_wide_kernel<T, 1024>), dim3((unsigned)a.N), dim3(1024), 0, st, a, grad_only);
+template <typename T, int NT>
+static int wide_start(const DistillArgs& a, int grad_only, hipStream_t st) {
+  const dim3 grid((unsigned)std::min<int64_t>(a.N, 256 * (2048 / NT)));
+  if (grad_only) hipLaunchKernelGGL((distill_wide_kernel<T, NT, true>), grid, dim3(NT), 0, st, a);
+  else hipLaunchKernelGGL((distill_wide_kernel<T, NT, false>), grid, dim3(NT), 0, st, a);
   SX_LAUNCH_CHECK("distill_wide");
   return SX_OK;
+}
+
+template <typename T>
+static int wide_launch(const DistillArgs& a, int grad_only, hipStream_t st) {
+  // a wave for a short row, more for a long one, most of them where there are few rows.  Gradient of 256 MB of bf16 logits with K = 16: rows of
+  // 4000 by one wave 160 us, by four 222; of 50000 by four 122, by sixteen 137; of 131072 113 and 114
+  if (a.V <= 8192) return wide_start<T, 64>(a, grad_only, st);
+  if (a.N >= 512) return wide_start<T, 256>(a, grad_only, st);
+  return wide_start<T, 1024>(a, grad_only, st);
 }
 
 // rows_kernel: the row fits the registers, its pairs the threads, exponents the fma form, and the gradient's rows lie to the 16-byte
