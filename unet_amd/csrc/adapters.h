@@ -1,8 +1,19 @@
 // Shared by the kernels of the adapter projection (adapters.hip, adapter_tiles.hip, adapter_tokens.hip).
 #pragma once
 #include "sx_common.h"
+#include <type_traits>
 
 namespace sx {
+
+// f(0), f(1) ... f(N - 1) with constant arguments: an array indexed by them stays in registers (#pragma unroll leaves loops around
+// cross-lane operations rolled, and the array in memory)
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void unrolled(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>());
+    unrolled<N, I + 1>(static_cast<F&&>(f));
+  }
+}
 
 template <typename T> struct Mma;
 template <> struct Mma<bf16> {

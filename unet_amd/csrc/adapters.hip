@@ -327,39 +327,58 @@ __device__ __forceinline__ void outer_block(const OuterArgs& a, OuterJob& j, int
   g = t / j.cols;
 }
 
-// fp32: 64 columns and 16 ranks per block, its waves split the rows
-__global__ __launch_bounds__(256) void adapter_outer_f32_kernel(OuterArgs a) {
-  __shared__ float red[4][16][64];
+// fp32: 64 columns and 16 ranks per block, its waves split the rows, four at a time; the places of the next four are on their way meanwhile
+template <int NW>
+__global__ __launch_bounds__(64 * NW) void adapter_outer_f32_kernel(OuterArgs a) {
+  __shared__ float red[NW][16][64];
+  constexpr int U = 4;
   OuterJob j;
   int c0, g;
   outer_block(a, j, c0, g);
-  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = c0 + lane, j0 = blockIdx.y * 16;
   const int t0 = a.start[g], t1 = a.end[g];
   float acc[16] = {};
-  for (int t = t0 + wid; t < t1; t += 4) {
-    const float xv = c < j.C ? ((const float*)j.x)[(int64_t)a.perm[t] * j.ldx + c] : 0.f;
-    const float* h = (const float*)j.h + (int64_t)t * a.rp + j0;
+  int p[U];
+  auto load_perm = [&](int t) {
+    if (t >= t1) return;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) acc[k] = fmaf(h[k], xv, acc[k]);
+    for (int u = 0; u < U; ++u) p[u] = a.perm[std::min(t + u, t1 - 1)];
+  };
+  load_perm(t0 + wid * U);
+  for (int t = t0 + wid * U; t < t1; t += NW * U) {
+    float xv[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) xv[u] = c < j.C ? ((const float*)j.x)[(int64_t)p[u] * j.ldx + c] : 0.f;
+    load_perm(t + NW * U);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (t + u >= t1) continue;
+      const float* h = (const float*)j.h + (int64_t)(t + u) * a.rp + j0;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) acc[k] = fmaf(h[k], xv[u], acc[k]);
+    }
   }
 #pragma unroll
   for (int k = 0; k < 16; ++k) red[wid][k][lane] = acc[k];
   __syncthreads();
-  for (int i = threadIdx.x; i < 16 * 64; i += 256) {
+  for (int i = threadIdx.x; i < 16 * 64; i += 64 * NW) {
     const int k = j.o_j == 1 ? i & 15 : i >> 6, cc = j.o_j == 1 ? i >> 4 : i & 63;
-    if (j0 + k < a.r && c0 + cc < j.C)
-      ((float*)j.out)[g * j.o_g + (j0 + k) * j.o_j + (int64_t)(c0 + cc) * j.o_c] = red[0][k][cc] + red[1][k][cc] + red[2][k][cc] + red[3][k][cc];
+    if (j0 + k < a.r && c0 + cc < j.C) {
+      float v = red[0][k][cc];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) v += red[w][k][cc];
+      ((float*)j.out)[g * j.o_g + (j0 + k) * j.o_j + (int64_t)(c0 + cc) * j.o_c] = v;
+    }
   }
 }
 
-// bf16: 64 columns and RT * 16 ranks per block; a wave takes every eighth block of 32 rows, the next block's x on its way under the MFMAs
+// bf16: 64 columns and RT * 16 ranks per block; a wave takes every NW-th block of 32 rows, the next block's x on its way under the MFMAs
 // of one.  h comes with the rows along memory (16 bytes = 8 rows of one rank); x comes as it lies, 4 columns of 8 rows per lane, and is
 // turned in registers: fragment f holds columns 4 n + f.  32-row blocks are aligned, so that h's and perm's 16-byte reads are: rows of
 // other adapters in the first and last one are cleared on both sides.
-template <int RT>
-__global__ __launch_bounds__(512) void adapter_outer_kernel(OuterArgs a) {
-  constexpr int NW = 8;
+template <int RT, int NW>
+__global__ __launch_bounds__(64 * NW) void adapter_outer_kernel(OuterArgs a) {
   typedef __attribute__((ext_vector_type(4))) int i32x4;
   __shared__ float red[NW / 2][RT * 16][64 + 1];
   OuterJob j;
@@ -473,8 +492,12 @@ __global__ __launch_bounds__(512) void adapter_outer_kernel(OuterArgs a) {
   __syncthreads();
   for (int i = tid; i < RT * 16 * 64; i += 64 * NW) {
     const int k = j.o_j == 1 ? i % (RT * 16) : i >> 6, cc = j.o_j == 1 ? i / (RT * 16) : i & 63;
-    if (j0 + k < a.r && c0 + cc < j.C)
-      ((bf16*)j.out)[g * j.o_g + (j0 + k) * j.o_j + (int64_t)(c0 + cc) * j.o_c] = (bf16)(red[0][k][cc] + red[1][k][cc] + red[2][k][cc] + red[3][k][cc]);
+    if (j0 + k < a.r && c0 + cc < j.C) {
+      float v = red[0][k][cc];
+#pragma unroll
+      for (int w = 1; w < NW / 2; ++w) v += red[w][k][cc];
+      ((bf16*)j.out)[g * j.o_g + (j0 + k) * j.o_j + (int64_t)(c0 + cc) * j.o_c] = (bf16)v;
+    }
   }
 }
 
@@ -553,7 +576,7 @@ static int project_launch(const ProjectArgs& a, hipStream_t st) {
 }
 
 template <typename T>
-static int outer_launch(OuterArgs a, hipStream_t st) {
+static int outer_launch(OuterArgs a, int64_t T_rows, hipStream_t st) {
   int blocks = 0;
   for (int i = 0; i < a.n; ++i) {
     a.job[i].cols = cdiv(a.job[i].C, 64);
@@ -562,9 +585,18 @@ static int outer_launch(OuterArgs a, hipStream_t st) {
     blocks += a.job[i].cols * a.G;
   }
   if (!blocks) return SX_OK;
-  if (sizeof(T) == 4) hipLaunchKernelGGL(adapter_outer_f32_kernel, dim3(blocks, cdiv(a.r, 16)), dim3(256), 0, st, a);
-  else if (a.rp <= 16) hipLaunchKernelGGL(adapter_outer_kernel<1>, dim3(blocks, 1), dim3(512), 0, st, a);
-  else hipLaunchKernelGGL(adapter_outer_kernel<2>, dim3(blocks, cdiv(a.rp, 32)), dim3(512), 0, st, a);
+  // many rows per adapter: many waves for them
+  const bool tall = T_rows >= 64 * (int64_t)a.G;
+  if (sizeof(T) == 4) {
+    if (tall) hipLaunchKernelGGL(adapter_outer_f32_kernel<16>, dim3(blocks, cdiv(a.r, 16)), dim3(1024), 0, st, a);
+    else hipLaunchKernelGGL(adapter_outer_f32_kernel<4>, dim3(blocks, cdiv(a.r, 16)), dim3(256), 0, st, a);
+  } else if (a.rp <= 16) {
+    if (tall) hipLaunchKernelGGL((adapter_outer_kernel<1, 8>), dim3(blocks, 1), dim3(512), 0, st, a);
+    else hipLaunchKernelGGL((adapter_outer_kernel<1, 2>), dim3(blocks, 1), dim3(128), 0, st, a);
+  } else {
+    if (tall) hipLaunchKernelGGL((adapter_outer_kernel<2, 8>), dim3(blocks, cdiv(a.rp, 32)), dim3(512), 0, st, a);
+    else hipLaunchKernelGGL((adapter_outer_kernel<2, 2>), dim3(blocks, cdiv(a.rp, 32)), dim3(128), 0, st, a);
+  }
   SX_LAUNCH_CHECK("adapter_outer");
   return SX_OK;
 }
@@ -651,7 +683,7 @@ static int adapter_backward(const AdapterCall& c, const void* dy, int64_t lddy, 
     OuterJob& j = q.job[q.n++];
     j.x = d; j.ldx = ldd; j.C = c.N; j.h = kept + (sizeof(T) == 2 ? k.ht : k.h); j.out = dB; j.o_g = (int64_t)c.N * c.r; j.o_j = 1; j.o_c = c.r;
   }
-  return outer_launch<T>(q, st);
+  return outer_launch<T>(q, c.T, st);
 }
 
 static int adapter_check(const char* who, int dtype, int64_t T, int K, int N, int r, int G) {
