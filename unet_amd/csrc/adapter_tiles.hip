@@ -16,7 +16,7 @@ namespace sx {
 
 template <int N> __device__ __forceinline__ void tiles_wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
-template <typename T, int WM, int WN, int MI, int NJ, int OCC, int NA, int NB>
+template <typename T, int WM, int WN, int MI, int NJ, int OCC, int NA, int NB, bool SPLIT>
 __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(ProjectArgs a, int gm, int gn, unsigned x_bytes, unsigned w_bytes) {
   constexpr int NT = 64 * WM * WN, BM = WM * MI * 16, BN = WN * NJ * 16, RPR = NT / 8;      // RPR: rows per DMA round
   constexpr int SA = BM * 128, SB = BN * 128, QA = SA / (NT * 16), QB = SB / (NT * 16);
@@ -54,25 +54,26 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(Projec
   const int64_t w0 = m0 + wm * MI * 16;
   const int rows = (int)std::min<int64_t>(MI * 16, a.T - w0);      // of this wave; <= 0: none, but it takes part in the DMA and the barriers
   const int g_first = __builtin_amdgcn_readfirstlane(a.key[std::min(w0, a.T - 1)]);
-  const int nst = (a.K + KS - 1) / KS;
+  // the stages of this block: all of K, or its part of them
+  const int all = (a.K + KS - 1) / KS, sb = SPLIT ? blockIdx.y * a.part_stages : 0, nst = SPLIT ? std::min(all - sb, a.part_stages) : all;
   char* const sx = smem;
   char* const sw = smem + NA * SA;
   // past the end: zeros, which keep the count of loads uniform
   auto issue_x = [&](int s, int slot) {
-    const unsigned far = piece * EPL + s * KS < a.K ? 0u : 0x80000000u;
+    const unsigned far = piece * EPL + (sb + s) * KS < a.K ? 0u : 0x80000000u;
     __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)a.x, 0, s < nst ? x_bytes : 0, 0x00020000);
 #pragma unroll
     for (int q = 0; q < QA; ++q) {
-      const unsigned off = (xo[q] + s * 128u) | far;
+      const unsigned off = (xo[q] + (sb + s) * 128u) | far;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(sx + slot * SA + wid * 1024 + q * (NT * 16)), 16, off, 0, 0, 0);
     }
   };
   auto issue_w = [&](int s, int slot) {
-    const unsigned far = piece * EPL + s * KS < a.K ? 0u : 0x80000000u;
+    const unsigned far = piece * EPL + (sb + s) * KS < a.K ? 0u : 0x80000000u;
     __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)a.w, 0, s < nst ? w_bytes : 0, 0x00020000);
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
-      const unsigned off = (wo[q] + s * 128u) | far;
+      const unsigned off = (wo[q] + (sb + s) * 128u) | far;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(sw + slot * SB + wid * 1024 + q * (NT * 16)), 16, off, 0, 0, 0);
     }
   };
@@ -131,6 +132,17 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(Projec
   // owns takes it in its accumulators; one that several share gets each adapter's product apart and picks its rows, in the epilogue:
   // masking h alone would let a NaN or an infinity of one adapter reach the others' rows as 0 * NaN.
   if (rows <= 0) return;
+  if constexpr (SPLIT) {                                      // sums of a part of K, for adapter_join_kernel
+    float* part = a.part + ((int64_t)blockIdx.y * a.T + w0) * a.part_ld;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int c = n0 + (wn * NJ + j) * 16 + 4 * gq;
+        if (i * 16 + n < rows && c < a.part_ld) *reinterpret_cast<f32x4*>(part + (int64_t)(i * 16 + n) * a.part_ld + c) = acc[i][j];
+      }
+    return;
+  }
   int at_y[MI], own[MI];                                      // all rows' places and adapters at once: one latency
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
@@ -174,26 +186,37 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void adapter_tiles_kernel(Projec
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     if (i * 16 >= rows) continue;
-    const int end = std::min(i * 16 + 16, rows);
     T* y = (T*)a.y + (int64_t)at_y[i] * a.ldy;
     f32x4 v[NJ];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) v[j] = acc[i][j];
     if (front(i) != back(i)) {
-      for (int at = i * 16; at < end;) {
-        const int g = __builtin_amdgcn_readfirstlane(a.key[w0 + at]);
-        if (g >= a.G) break;
-        f32x4 d[NJ] = {};
-        for (int j0 = 0; j0 < a.r; j0 += 16) {
-          const Vec hf = h_piece(i, j0);
+      constexpr int B = NJ == 1 ? 8 : 2;                      // adapters whose factors are in flight together
+      for (int j0 = 0; j0 < a.r; j0 += 16) {
+        const Vec hf = h_piece(i, j0);
+        int at = 0;                                           // row of the fragment; its adapters in their order
+        while (at < 16) {
+          int g[B];
+          Vec qb[B][NJ];
+          unrolled<B>([&](auto b) {
+            g[b] = at < 16 ? __builtin_amdgcn_readlane(own[i], at) : a.G;
+            at = g[b] < a.G ? at + __popcll(__ballot(own[i] == g[b]) & 0xffffull) : 16;      // (the rows without an adapter come last)
+          });
+          unrolled<B>([&](auto b) {
+            if (g[b] < a.G)
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) d[j] = Mma<T>::run(q_piece(g, j, j0), hf, d[j]);
+              for (int j = 0; j < NJ; ++j) qb[b][j] = q_piece(g[b], j, j0);
+          });
+          unrolled<B>([&](auto b) {
+            if (g[b] < a.G)
+#pragma unroll
+              for (int j = 0; j < NJ; ++j) {
+                const f32x4 d = Mma<T>::run(qb[b][j], hf, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[j][e] += own[i] == g[b] ? d[e] : 0.f;
+              }
+          });
         }
-#pragma unroll
-        for (int j = 0; j < NJ; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[j][e] += own[i] == g ? d[j][e] : 0.f;
-        at = (int)std::min<int64_t>(end, __builtin_amdgcn_readfirstlane(a.end[g]) - w0);
       }
     }
 #pragma unroll
@@ -230,12 +253,75 @@ template <typename T, int WM, int WN, int MI, int NJ, int OCC, int NA, int NB>
 static int tiles_launch(const ProjectArgs& a, hipStream_t st) {
   constexpr int BM = WM * MI * 16, BN = WN * NJ * 16, LDS = (NA * BM + NB * BN) * 128;
   static std::atomic<unsigned long long> done{0};
-  SX_TRY(ensure_max_lds((const void*)adapter_tiles_kernel<T, WM, WN, MI, NJ, OCC, NA, NB>, done, "adapter_tiles"));
+  SX_TRY(ensure_max_lds((const void*)adapter_tiles_kernel<T, WM, WN, MI, NJ, OCC, NA, NB, false>, done, "adapter_tiles"));
   int64_t xb, wb;
   tiles_bytes(a, sizeof(T), xb, wb);
   const int gm = (int)cdiv64(a.T, BM), gn = cdiv(a.N, BN);
-  hipLaunchKernelGGL((adapter_tiles_kernel<T, WM, WN, MI, NJ, OCC, NA, NB>), dim3((unsigned)(gm * gn)), dim3(64 * WM * WN), LDS, st, a, gm, gn, (unsigned)xb, (unsigned)wb);
+  hipLaunchKernelGGL((adapter_tiles_kernel<T, WM, WN, MI, NJ, OCC, NA, NB, false>), dim3((unsigned)(gm * gn)), dim3(64 * WM * WN), LDS, st, a, gm, gn, (unsigned)xb, (unsigned)wb);
   SX_LAUNCH_CHECK("adapter_tiles");
+  return SX_OK;
+}
+
+// y of what the parts of K hold: one column of a row per thread, the parts in their order, then the row's adapter, one rounding
+template <typename T>
+__global__ __launch_bounds__(256) void adapter_join_kernel(ProjectArgs a) {
+  typedef typename Elem<T>::Vec Vec;
+  constexpr int EPL = Elem<T>::EPL;
+  const int64_t at = blockIdx.x * 256ll + threadIdx.x;
+  const int64_t m = at / a.N;
+  const int c = (int)(at - m * a.N);
+  if (m >= a.T) return;
+  const int g = a.key[m];
+  float v = a.bias ? to_f32(((const T*)a.bias)[c]) : 0.f;
+#pragma unroll 4
+  for (int s = 0; s < a.parts; ++s) v += a.part[((int64_t)s * a.T + m) * a.part_ld + c];
+  if (g < a.G) {
+    const T* q = (const T*)a.q + g * a.q_g + (int64_t)c * a.q_ld;
+    float d = 0.f;
+#pragma unroll 2
+    for (int j = 0; j < a.r; j += EPL) {
+      const Vec f = *reinterpret_cast<const Vec*>(q + j);
+      Vec h, lo = {};
+      if constexpr (sizeof(T) == 2) {
+        const T* p = (const T*)a.h + m * (2 * a.rp) + j / 16 * 32 + (j & 15);
+        h = *reinterpret_cast<const Vec*>(p);
+        lo = *reinterpret_cast<const Vec*>(p + 16);
+      } else {
+        h = *reinterpret_cast<const Vec*>((const T*)a.h + m * a.rp + j);
+      }
+#pragma unroll
+      for (int e = 0; e < EPL; ++e)
+        if (j + e < a.r) d = fmaf(to_f32(h[e]) + to_f32(lo[e]), to_f32(f[e]), d);
+    }
+    v += d;
+  }
+  ((T*)a.y)[(int64_t)a.perm[m] * a.ldy + c] = from_f32<T>(v);
+}
+
+// Parts of K for a product of few tiles of 64 x 64; 0: none, the tiles kernel finishes by itself.  A stage of such a tile takes 0.5 to 0.7 us
+// however deep its rings are (MFMA in fp32, the barriers in bf16), so few tiles with many stages leave most CUs idle; and where most
+// fragments hold rows of several adapters, their products one after the other take longer than a launch.  MEASURED
+int project_parts(int dtype, int64_t T, int K, int N, int G, int& stages) {
+  const int64_t tiles = cdiv64(T, 64) * cdiv(N, 64);
+  const int all = cdiv(K, dtype == SX_BF16 ? 64 : 32);
+  if (tiles == 0 || tiles > 512 || (all < 16 && (T > 16 * (int64_t)G || tiles > 128))) return 0;
+  int parts = (int)std::max<int64_t>(1, std::min<int64_t>(cdiv64(1024, tiles), all / 4));
+  stages = cdiv(all, parts);
+  return cdiv(all, stages);
+}
+
+template <typename T>
+static int split_launch(const ProjectArgs& a, hipStream_t st) {
+  constexpr int LDS = 3 * 128 * 128;
+  static std::atomic<unsigned long long> done{0};
+  SX_TRY(ensure_max_lds((const void*)adapter_tiles_kernel<T, 1, 4, 4, 1, 4, 3, 3, true>, done, "adapter_tiles"));
+  int64_t xb, wb;
+  tiles_bytes(a, sizeof(T), xb, wb);
+  const int gm = (int)cdiv64(a.T, 64), gn = cdiv(a.N, 64);
+  hipLaunchKernelGGL((adapter_tiles_kernel<T, 1, 4, 4, 1, 4, 3, 3, true>), dim3(gm * gn, a.parts), dim3(256), LDS, st, a, gm, gn, (unsigned)xb, (unsigned)wb);
+  SX_LAUNCH_CHECK("adapter_tiles");
+  hipLaunchKernelGGL(adapter_join_kernel<T>, dim3((unsigned)cdiv64(a.T * a.N, 256)), dim3(256), 0, st, a);
+  SX_LAUNCH_CHECK("adapter_join");
   return SX_OK;
 }
 
@@ -247,6 +333,7 @@ static double tiles_cost(const ProjectArgs& a, int bm, int bn, int per_cu, doubl
 
 template <typename T>
 static int tiles_pick(const ProjectArgs& a, hipStream_t st) {
+  if (a.parts) return split_launch<T>(a, st);
   const double c0 = tiles_cost(a, 256, 256, 1, 1.0), c1 = tiles_cost(a, 128, 256, 1, 1.2), c2 = tiles_cost(a, 128, 128, 2, 1.4), c3 = tiles_cost(a, 64, 64, 4, 2.0);
   if (c0 <= c1 && c0 <= c2 && c0 <= c3) return tiles_launch<T, 2, 4, 8, 4, 2, 3, 2>(a, st);
   if (c1 <= c2 && c1 <= c3) return tiles_launch<T, 2, 4, 4, 4, 2, 3, 3>(a, st);

@@ -51,6 +51,8 @@ struct ProjectArgs {
   const int* perm; const int* key; const int* start; const int* end;
   int64_t T; int K, N, r, G;
   void* y; int64_t ldy;
+  int parts, part_stages;                     // K in parts of that many stages, summed by a second launch; 0: in one
+  float* part; int part_ld;                   // [parts][T][part_ld], sorted rows
 };
 
 // a lane's 16 bytes of h (row m, ranks from j0 on), and the first of the ranks whose factors they meet
@@ -64,6 +66,7 @@ __device__ __forceinline__ typename Elem<T>::Vec load_h(const ProjectArgs& a, in
 
 // the shared product by tiles (adapter_tiles.hip); false: not for this kernel
 bool project_tiles_ok(const ProjectArgs& a, int dtype);
+int project_parts(int dtype, int64_t T, int K, int N, int G, int& stages);
 int project_tiles_launch(const ProjectArgs& a, int dtype, hipStream_t st);
 
 // a few rows, forward alone (adapter_tokens.hip)

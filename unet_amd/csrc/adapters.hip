@@ -118,10 +118,10 @@ struct ShrinkArgs {
 // MT * 16 sorted rows and RT * 16 ranks per block; its NW waves split the columns
 template <typename T, int MT, int RT, int NW>
 __global__ __launch_bounds__(64 * NW) void adapter_shrink_kernel(ShrinkArgs a) {
-  constexpr int EPL = Elem<T>::EPL, CK = Elem<T>::CK, RJ = RT * 16, U = MT == 1 && RT <= 2 ? 8 : 4;      // U: chunks in flight per wave
+  constexpr int EPL = Elem<T>::EPL, CK = Elem<T>::CK, RJ = RT * 16, U = MT == 1 && RT <= 2 ? 8 : 4, R = RT == 1 ? 4 : 3;      // U: chunks in flight per wave
   typedef typename Elem<T>::Vec Vec;
   __shared__ float red[NW][MT * 16][RJ + 1];
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, n = lane & 15, gq = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, gq = lane >> 4;
   const int64_t m0 = blockIdx.x * (int64_t)(MT * 16);
   const int j0 = blockIdx.y * RJ;
   const int rows = (int)std::min<int64_t>(MT * 16, a.T - m0);
@@ -129,9 +129,10 @@ __global__ __launch_bounds__(64 * NW) void adapter_shrink_kernel(ShrinkArgs a) {
 #pragma unroll
   for (int i = 0; i < MT; ++i) xr[i] = (const T*)a.x + (int64_t)a.perm[m0 + std::min(i * 16 + n, rows - 1)] * a.ldx + gq * EPL;
   f32x4 tot[MT][RT] = {};
+  const int own = a.key[m0 + std::min(lane, rows - 1)];      // the adapters of the block's rows, over the lanes
   for (int at = 0; at < rows;) {
-    const int g = a.key[m0 + at];
-    const int end = (int)std::min<int64_t>(rows, a.end[g] - m0);
+    const int g = __builtin_amdgcn_readlane(own, at);
+    const int end = at + __popcll(__ballot(lane < rows && own == g));
     if (g < a.G) {
       const T* pr[RT];                        // ranks past the last one read it again: their products are not stored
 #pragma unroll
@@ -154,16 +155,25 @@ __global__ __launch_bounds__(64 * NW) void adapter_shrink_kernel(ShrinkArgs a) {
 #pragma unroll
             for (int t = 0; t < RT; ++t) acc[i][t] = Mma<T>::run(xv[u][i], pv[u][t], acc[i][t]);
       }
-      for (; c0 < a.C; c0 += NW * CK) {
-        Vec xv[MT], pv[RT];
+      for (; c0 < a.C; c0 += R * NW * CK) {   // the rest, R chunks in flight
+        Vec xv[R][MT], pv[R][RT];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) xv[i] = load_piece<T>(xr[i] - gq * EPL, c0 + gq * EPL, a.C);
+        for (int u = 0; u < R; ++u) {
+          const int c = c0 + u * NW * CK;
+          if (c >= a.C) continue;
 #pragma unroll
-        for (int t = 0; t < RT; ++t) pv[t] = load_piece<T>(pr[t] - gq * EPL, c0 + gq * EPL, a.C);
+          for (int i = 0; i < MT; ++i) xv[u][i] = load_piece<T>(xr[i] - gq * EPL, c + gq * EPL, a.C);
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+          for (int t = 0; t < RT; ++t) pv[u][t] = load_piece<T>(pr[t] - gq * EPL, c + gq * EPL, a.C);
+        }
 #pragma unroll
-          for (int t = 0; t < RT; ++t) acc[i][t] = Mma<T>::run(xv[i], pv[t], acc[i][t]);
+        for (int u = 0; u < R; ++u) {
+          if (c0 + u * NW * CK >= a.C) continue;
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int t = 0; t < RT; ++t) acc[i][t] = Mma<T>::run(xv[u][i], pv[u][t], acc[i][t]);
+        }
       }
 #pragma unroll
       for (int i = 0; i < MT; ++i)
@@ -211,6 +221,50 @@ __global__ __launch_bounds__(64 * NW) void adapter_shrink_kernel(ShrinkArgs a) {
       bf16* h = a.ht + (int64_t)(j0 + j) * a.ldt + m0 + m;
       h[0] = (bf16)v;
       h[a.rp * a.ldt] = h_lo(v);
+    }
+  }
+}
+
+// Where rows seldom share an adapter: a block per sorted row, a wave per four ranks at a time, its lanes over the columns
+template <typename T>
+__global__ __launch_bounds__(256) void adapter_shrink_row_kernel(ShrinkArgs a) {
+  constexpr int EPL = Elem<T>::EPL, J = 4;
+  typedef typename Elem<T>::Vec Vec;
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t m = blockIdx.x;
+  const int g = a.key[m];
+  const T* x = (const T*)a.x + (int64_t)a.perm[m] * a.ldx;
+  const float scale = g < a.G && a.scales ? a.scales[g] : 1.f;
+  for (int j0 = wid * J; j0 < a.rp; j0 += 4 * J) {
+    float acc[J] = {};
+    if (g < a.G && j0 < a.r)
+#pragma unroll 2
+      for (int c = lane * EPL; c < a.C; c += 64 * EPL) {
+        const Vec xv = *reinterpret_cast<const Vec*>(x + c);
+        Vec pv[J];
+#pragma unroll
+        for (int j = 0; j < J; ++j) pv[j] = *reinterpret_cast<const Vec*>((const T*)a.p + g * a.p_g + (int64_t)std::min(j0 + j, a.r - 1) * a.p_ld + c);
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+          for (int e = 0; e < EPL; ++e) acc[j] = fmaf(to_f32(xv[e]), to_f32(pv[j][e]), acc[j]);
+      }
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const float sum = wave_sum(acc[j]), v = g < a.G && j0 + j < a.r ? scale * sum : 0.f;
+      if (lane) continue;
+      if constexpr (sizeof(T) == 2) {
+        bf16* h = (bf16*)a.h + m * (2 * a.rp) + (j0 + j) / 16 * 32 + ((j0 + j) & 15);
+        h[0] = (bf16)v;
+        h[16] = h_lo(v);
+        if (a.ht) {
+          bf16* t = a.ht + (int64_t)(j0 + j) * a.ldt + m;
+          t[0] = (bf16)v;
+          t[a.rp * a.ldt] = h_lo(v);
+        }
+      } else {
+        ((float*)a.h)[m * a.rp + j0 + j] = v;
+      }
     }
   }
 }
@@ -521,7 +575,7 @@ static AdapterKept adapter_kept(int dtype, int64_t T, int r, int G) {
 // sizes that rows of K elements lie in whole 16-byte pieces for; other ones are packed into rows that do
 static int padded(int dtype, int n) { return round_up(n, dtype == SX_BF16 ? 8 : 4); }
 
-struct AdapterWs { size_t x, w, A, B, dy, wt, at, bt, dh, dht, total; };
+struct AdapterWs { size_t x, w, A, B, dy, wt, at, bt, dh, dht, part, total; };
 static AdapterWs adapter_ws(int dtype, int64_t T, int K, int N, int r, int G, bool backward) {
   const size_t e = dtype_size(dtype);
   const int Kp = padded(dtype, K), Np = padded(dtype, N), r8 = padded(dtype, r);
@@ -540,6 +594,9 @@ static AdapterWs adapter_ws(int dtype, int64_t T, int K, int N, int r, int G, bo
     take(w.dh, (size_t)T * k.rp, 4);
     if (dtype == SX_BF16) take(w.dht, (size_t)k.rp * k.ldt, 4);
   }
+  int stages;
+  const int out = backward ? K : N, parts = project_parts(dtype, T, backward ? Np : Kp, out, G, stages);
+  take(w.part, (size_t)parts * T * round_up(out, 16), 4);
   w.total = std::max<size_t>(o, 256);
   return w;
 }
@@ -549,7 +606,9 @@ static int shrink_launch(const ShrinkArgs& a, hipStream_t st) {
   // 32 rows share an adapter's factor once there are rows enough for two such blocks a CU; below, 16 rows and, up to one block a CU, sixteen
   // waves.  (32 rows from 8192 rows on: 32 us against 27 at 8192 x 4096, rank 16.)
   const int rt = a.rp <= 16 ? 1 : a.rp <= 32 ? 2 : 4;
-  if (a.T >= 32 * 512) {
+  if (a.T <= 8 * (int64_t)a.G) {
+    hipLaunchKernelGGL(adapter_shrink_row_kernel<T>, dim3((unsigned)a.T), dim3(256), 0, st, a);
+  } else if (a.T >= 32 * 512) {
     const dim3 grid((unsigned)cdiv64(a.T, 32), cdiv(a.rp, rt * 16));
     if (rt == 1) hipLaunchKernelGGL((adapter_shrink_kernel<T, 2, 1, 4>), grid, dim3(256), 0, st, a);
     else if (rt == 2) hipLaunchKernelGGL((adapter_shrink_kernel<T, 2, 2, 4>), grid, dim3(256), 0, st, a);
@@ -568,7 +627,10 @@ static int shrink_launch(const ShrinkArgs& a, hipStream_t st) {
 }
 
 template <typename T>
-static int project_launch(const ProjectArgs& a, hipStream_t st) {
+static int project_launch(ProjectArgs a, char* part, hipStream_t st) {
+  a.parts = project_parts(Elem<T>::kDtype, a.T, a.K, a.N, a.G, a.part_stages);
+  a.part = (float*)part;
+  a.part_ld = round_up(a.N, 16);
   if (project_tiles_ok(a, Elem<T>::kDtype)) return project_tiles_launch(a, Elem<T>::kDtype, st);
   hipLaunchKernelGGL((adapter_project_kernel<T, 128, 128>), dim3((unsigned)cdiv64(a.T, 128), cdiv(a.N, 128)), dim3(256), 0, st, a);
   SX_LAUNCH_CHECK("adapter_project");
@@ -637,7 +699,7 @@ static int adapter_forward(const AdapterCall& c, const void* ids, int ids64, voi
   ProjectArgs p = {};
   p.x = x; p.ldx = ldx; p.w = w; p.ldw = ldw; p.bias = c.bias; p.q = B; p.q_g = (int64_t)c.N * r8; p.q_ld = r8; p.h = kept + k.h; p.rp = k.rp;
   p.perm = perm; p.key = key; p.start = start; p.end = end; p.T = c.T; p.K = Kp; p.N = c.N; p.r = c.r; p.G = c.G; p.y = y; p.ldy = ldy;
-  return project_launch<T>(p, st);
+  return project_launch<T>(p, ws + o.part, st);
 }
 
 template <typename T>
@@ -671,7 +733,7 @@ static int adapter_backward(const AdapterCall& c, const void* dy, int64_t lddy, 
     ProjectArgs p = {};
     p.x = d; p.ldx = ldd; p.w = ws + o.wt; p.ldw = Np; p.q = ws + o.at; p.q_g = (int64_t)c.K * r8; p.q_ld = r8; p.h = ws + o.dh; p.rp = k.rp;
     p.perm = perm; p.key = key; p.start = start; p.end = end; p.T = c.T; p.K = Np; p.N = c.K; p.r = c.r; p.G = c.G; p.y = dx; p.ldy = c.K;
-    SX_TRY(project_launch<T>(p, st));
+    SX_TRY(project_launch<T>(p, ws + o.part, st));
   }
   OuterArgs q = {};
   q.perm = perm; q.start = start; q.end = end; q.r = c.r; q.rp = k.rp; q.G = c.G; q.ldt = k.ldt;
