@@ -299,15 +299,21 @@ __global__ __launch_bounds__(256) void adapter_join_kernel(ProjectArgs a) {
 }
 
 // Parts of K for a product of few tiles of 64 x 64; 0: none, the tiles kernel finishes by itself.  A stage of such a tile takes 0.5 to 0.7 us
-// however deep its rings are (MFMA in fp32, the barriers in bf16), so few tiles with many stages leave most CUs idle; and where most
-// fragments hold rows of several adapters, their products one after the other take longer than a launch.  MEASURED
+// however deep its rings are (MFMA in fp32, the barriers in bf16), so few tiles with many stages leave most CUs idle: 84 x 2880 -> 128 in fp32
+// 11 us in parts against 61, 2481 x 3180 -> 456 101 against 121.  The join costs a launch and its reads, six such stages and one more per
+// 1.8 MB: 6198 x 896 -> 256 in fp32 54 us in parts, 44 without.  And where most fragments hold rows of several adapters, the join
+// multiplies by them faster: 256 rows of 16 adapters, 256 -> 256, 9 us against 14; 82 rows of 118 adapters 7 against 26.
 int project_parts(int dtype, int64_t T, int K, int N, int G, int& stages) {
   const int64_t tiles = cdiv64(T, 64) * cdiv(N, 64);
   const int all = cdiv(K, dtype == SX_BF16 ? 64 : 32);
-  if (tiles == 0 || tiles > 512 || (all < 16 && (T > 16 * (int64_t)G || tiles > 128))) return 0;
-  int parts = (int)std::max<int64_t>(1, std::min<int64_t>(cdiv64(1024, tiles), all / 4));
+  stages = all;
+  if (tiles == 0 || tiles > 512) return 0;
+  const bool mixed = tiles <= 128 && T <= 16 * (int64_t)G;
+  const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(cdiv64(1024, tiles), all / 3));
   stages = cdiv(all, parts);
-  return cdiv(all, stages);
+  const int used = cdiv(all, stages);
+  const int64_t one = cdiv64(tiles, 256) * all, split = cdiv64(tiles * used, 256) * stages + 6 + used * T * N * 8 / 1800000;
+  return mixed || split < one ? used : 0;
 }
 
 template <typename T>

@@ -604,9 +604,12 @@ static AdapterWs adapter_ws(int dtype, int64_t T, int K, int N, int r, int G, bo
 template <typename T>
 static int shrink_launch(const ShrinkArgs& a, hipStream_t st) {
   // 32 rows share an adapter's factor once there are rows enough for two such blocks a CU; below, 16 rows and, up to one block a CU, sixteen
-  // waves.  (32 rows from 8192 rows on: 32 us against 27 at 8192 x 4096, rank 16.)
-  const int rt = a.rp <= 16 ? 1 : a.rp <= 32 ? 2 : 4;
-  if (a.T <= 8 * (int64_t)a.G) {
+  // waves and at most 32 ranks a block.  (32 rows from 8192 rows on: 32 us against 27 at 8192 x 4096, rank 16.  2481 x 3180, rank 40, fp32: 31 us
+  // with sixteen waves, 41 with eight and 64 ranks.)  Rows that seldom share an adapter come one by one: 107 rows of 68 adapters 4 us against
+  // 12, 256 of 16 adapters 3.5 against 4.6, 399 of 36 adapters, 2112 columns, rank 24: 10 against 22.
+  const bool wide = a.T <= 16 * 256 && a.C >= 16 * Elem<T>::CK;
+  const int rt = a.rp <= 16 ? 1 : a.rp <= 32 || wide ? 2 : 4;
+  if (a.T <= 16 * (int64_t)a.G) {
     hipLaunchKernelGGL(adapter_shrink_row_kernel<T>, dim3((unsigned)a.T), dim3(256), 0, st, a);
   } else if (a.T >= 32 * 512) {
     const dim3 grid((unsigned)cdiv64(a.T, 32), cdiv(a.rp, rt * 16));
@@ -615,7 +618,6 @@ static int shrink_launch(const ShrinkArgs& a, hipStream_t st) {
     else hipLaunchKernelGGL((adapter_shrink_kernel<T, 2, 4, 4>), grid, dim3(256), 0, st, a);
   } else {
     const dim3 grid((unsigned)cdiv64(a.T, 16), cdiv(a.rp, rt * 16));
-    const bool wide = a.T <= 16 * 256 && a.C >= 16 * Elem<T>::CK;
     if (rt == 1 && wide) hipLaunchKernelGGL((adapter_shrink_kernel<T, 1, 1, 16>), grid, dim3(1024), 0, st, a);
     else if (rt == 1) hipLaunchKernelGGL((adapter_shrink_kernel<T, 1, 1, 8>), grid, dim3(512), 0, st, a);
     else if (rt == 2 && wide) hipLaunchKernelGGL((adapter_shrink_kernel<T, 1, 2, 16>), grid, dim3(1024), 0, st, a);
