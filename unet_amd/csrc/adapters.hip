@@ -649,8 +649,10 @@ static int outer_launch(OuterArgs a, int64_t T_rows, hipStream_t st) {
     blocks += a.job[i].cols * a.G;
   }
   if (!blocks) return SX_OK;
-  // many rows per adapter: many waves for them
-  const bool tall = T_rows >= 64 * (int64_t)a.G;
+  // Many rows per adapter: many waves for them, in fp32 only where there are very many or few blocks (the sum of sixteen waves through LDS costs
+  // more than it gives).  fp32 with sixteen waves and with four: 6198 rows of 95 adapters 34 us and 23, 5684 of 25 35 and 30, 84 of one 6
+  // and 8, 2481 of two 42 and 155 (then a row at a time).  bf16 with eight and with two: 1027 rows of 7 adapters 9 us and 18, 399 of 36 23 and 13.
+  const bool tall = T_rows >= 64 * (int64_t)a.G && (sizeof(T) == 2 || T_rows >= 400 * (int64_t)a.G || (int64_t)blocks * cdiv(a.r, 16) <= 512);
   if (sizeof(T) == 4) {
     if (tall) hipLaunchKernelGGL(adapter_outer_f32_kernel<16>, dim3(blocks, cdiv(a.r, 16)), dim3(1024), 0, st, a);
     else hipLaunchKernelGGL(adapter_outer_f32_kernel<4>, dim3(blocks, cdiv(a.r, 16)), dim3(256), 0, st, a);
