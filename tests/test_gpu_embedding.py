@@ -169,3 +169,25 @@ def test_module_feeds_film_parameters():
     g = emb.weight.grad
     assert torch.isfinite(g).all() and g[2].abs().max() > 0 and g[6].abs().max() > 0
     assert not g[[0, 1, 3, 4, 5]].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D,offset,extra", [(500, 0, 0), (500, 4, 0), (634, 0, 6), (634, 2, 10), (96, 2, 8), (96, 1, 7), (1028, 0, 4), (2054, 0, 2)])
+def test_every_width_of_loads(D, offset, extra, dtype):
+    """Row lengths, strides and starts that allow loads of 16 bytes, of half, a quarter, an eighth of that, in tables and in upstream
+    gradients that are views of wider ones."""
+    ids, _, _ = _inputs((700,), 90, 8, dtype, torch.int64, "any")
+    g = torch.Generator().manual_seed(D + offset)
+    wide = torch.randn(90, D + offset + extra, generator=g).to(dtype).cuda()
+    table = wide[:, offset:offset + D].requires_grad_(True)
+    dout = torch.randn(700, D + offset + extra, generator=g).to(dtype).cuda()[:, offset:offset + D]
+    _check(ids, table, 3.0, dout)
+
+
+def test_padding_is_zero_whatever_the_scale():
+    from unet_amd.embedding import scaled_embedding
+    table = torch.ones(3, 40, device="cuda", requires_grad=True)
+    out = scaled_embedding(torch.tensor([-1, 1, 3], device="cuda"), table, float("inf"))
+    assert torch.equal(out[0], torch.zeros(40, device="cuda")) and torch.equal(out[2], out[0]) and torch.isinf(out[1]).all()
+    (grad,) = torch.autograd.grad(out, (table,), torch.ones_like(out))
+    assert torch.equal(grad[0], torch.zeros(40, device="cuda")) and torch.equal(grad[2], grad[0]) and torch.isinf(grad[1]).all()

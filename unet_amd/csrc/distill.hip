@@ -318,7 +318,7 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
   if (fix_at) *fix_at = from_f32<T>(fix);
 }
 
-// any row length, the logits read once for the maximum, once for the sum and once for the gradient; with GRAD_ONLY, the gradient alone, from
+// any row length, the logits read once for the maximum and the sum and once for the gradient; with GRAD_ONLY, the gradient alone, from
 // the maxima and sums of an earlier pass.  fmaxf drops a NaN; the sum brings it back
 template <typename T, int NT, bool GRAD_ONLY>
 __global__ __launch_bounds__(NT) void distill_wide_kernel(DistillArgs a) {
@@ -367,21 +367,28 @@ __global__ __launch_bounds__(NT) void distill_wide_kernel(DistillArgs a) {
     }
     const bool live = w != 0.f && !(ts == 0.f);
     if (!GRAD_ONLY && live) {
-      m = -INFINITY;
+      float mk = kFloor;                                  // as in rows_kernel: a thread rescales its sum when its maximum grows
+#pragma unroll 4
       for (int v = tid; v < nv; v += NT) {
         const Vec r = load_row_vec<T>(z, off, a.V, v);
+        float f[E], mn = mk;
 #pragma unroll
-        for (int e = 0; e < E; ++e) m = fmaxf(m, to_f32(r[e]));
+        for (int e = 0; e < E; ++e) { f[e] = to_f32(r[e]); mn = fmaxf(mn, f[e]); }
+        const float mc = mul_rn(mn, c);
+        s *= __builtin_amdgcn_exp2f(mul_rn(mk, c) - mc);
+#pragma unroll
+        for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f(fmaf(f[e], c, -mc));
+        mk = mn;
       }
-      m = all_max<NT>(m, red);
-      const Expo x(m, c);
-      for (int v = tid; v < nv; v += NT) {
-        const Vec r = load_row_vec<T>(z, off, a.V, v);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const int i = v * E + e - off;
-          s += i >= 0 && i < a.V ? __builtin_amdgcn_exp2f(x.at(to_f32(r[e]))) : 0.f;
-        }
+      m = all_max<NT>(mk, red);
+      s = mul_rn(s, __builtin_amdgcn_exp2f(mul_rn(mk, c) - mul_rn(m, c)));
+      if (!(fabsf(m) < kFar) || !(fabsf(c) < 1e6f)) {     // products that overflow: the row again, by differences
+        mk = -INFINITY;
+        for (int v = tid; v < a.V; v += NT) mk = fmaxf(mk, to_f32(z[v]));
+        m = all_max<NT>(mk, red);
+        const Expo x(m, c);
+        s = 0.f;
+        for (int v = tid; v < a.V; v += NT) s += __builtin_amdgcn_exp2f(x.at(to_f32(z[v])));
       }
       s = all_sum<NT>(s, red);
     }
@@ -499,12 +506,17 @@ static int distill_launch(const DistillArgs& a, hipStream_t st) {
   // another: the latter wins nearly everywhere.  256 MB of bf16 logits with / without a gradient: rows of 1000 by one wave 190 / 91 us, by four
   // 643 / 450; of 2000 by one 151 / 64, by two 212 / 122; of 16000 by 256 threads 117 / 50, by 512 119 / 63; of 32000 by 256 115 / 51, by 512
   // 111 / 52; of 24000 without a gradient 50 and 58; of 50000 by 512 118 / 50, by 1024 131 / 62.
-  if (a.K <= 64) {                                      // (a pair per thread)
+  if (a.K <= 64) {                                      // (one pair per thread)
     if (nv <= 64) return rows_launch<T, 64, 1>(a, 32, st);
     if (nv <= 128) return rows_launch<T, 64, 2>(a, 32, st);
     if (nv <= 256) return rows_launch<T, 64, 4>(a, 28, st);
     if (nv <= 512) return rows_launch<T, 64, 8>(a, 20, st);
     if (nv <= 1024) return rows_launch<T, 64, 16>(a, 16, st);
+  }
+  if (a.K <= 128) {
+    if (nv <= 256) return rows_launch<T, 128, 2>(a, 16, st);
+    if (nv <= 512) return rows_launch<T, 128, 4>(a, 14, st);
+    if (nv <= 1024) return rows_launch<T, 128, 8>(a, 10, st);
   }
   if (nv <= 256) return rows_launch<T, 256, 1>(a, 8, st);
   if (nv <= 512) return rows_launch<T, 256, 2>(a, 8, st);

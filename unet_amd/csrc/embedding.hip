@@ -20,10 +20,22 @@ static inline int embed_run(int64_t n) {
 }
 constexpr int64_t kMaxRows = 1 << 24;      // the gradient's grid gives every row of the table up to 128 threads of a 2^32 limit
 
-template <typename T, typename I, bool VEC>
+// E elements as one load or store
+template <typename T, int E> struct Piece { typedef __attribute__((ext_vector_type(E))) T type; };
+template <typename T> struct Piece<T, 1> { typedef T type; };
+template <typename T, int E> __device__ __forceinline__ float piece_get(const typename Piece<T, E>::type& p, int e) {
+  if constexpr (E == 1) return to_f32(p);
+  else return to_f32(p[e]);
+}
+template <typename T, int E> __device__ __forceinline__ void piece_set(typename Piece<T, E>::type& p, int e, float v) {
+  if constexpr (E == 1) p = from_f32<T>(v);
+  else p[e] = from_f32<T>(v);
+}
+
+template <typename T, typename I, int E>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* __restrict__ table, int64_t ld, const I* __restrict__ ids, int64_t n,
                                                         int64_t rows, int dim, float scale, T* __restrict__ out) {
-  constexpr int E = VEC ? 16 / (int)sizeof(T) : 1;
+  typedef typename Piece<T, E>::type P;
   const int pieces = dim / E;
   const int64_t total = n * pieces;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
@@ -33,15 +45,12 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* __restrict__ ta
     const bool ok = id >= 0 && id < rows;
     const T* src = table + (ok ? id : 0) * ld + c;
     T* dst = out + t * dim + c;
-    if constexpr (VEC) {
-      typename Elem<T>::Vec v = {};
-      if (ok) v = *reinterpret_cast<const typename Elem<T>::Vec*>(src);
+    P v = {};
+    if (ok) v = *reinterpret_cast<const P*>(src);
+    const float by = ok ? scale : 0.f;                     // (padding stays 0 whatever the scale is)
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[e] = from_f32<T>(to_f32(v[e]) * scale);
-      *reinterpret_cast<typename Elem<T>::Vec*>(dst) = v;
-    } else {
-      *dst = ok ? from_f32<T>(to_f32(*src) * scale) : from_f32<T>(0.f);
-    }
+    for (int e = 0; e < E; ++e) piece_set<T, E>(v, e, piece_get<T, E>(v, e) * by);
+    *reinterpret_cast<P*>(dst) = v;
   }
 }
 
@@ -57,10 +66,9 @@ struct EmbedBwdArgs {
 };
 
 // Columns of a thread: NC pieces of E elements, GROUP * E apart, from column c on.  Group = GROUP threads that share a row.
-template <typename T, bool VEC, int GROUP, int NC>
+template <typename T, int E, int GROUP, int NC>
 struct RowSum {
-  static constexpr int E = VEC ? 16 / (int)sizeof(T) : 1;
-  typedef std::conditional_t<VEC, typename Elem<T>::Vec, T> Piece;
+  typedef typename Piece<T, E>::type P;
   float acc[NC][E];
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -68,21 +76,17 @@ struct RowSum {
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[k][e] = 0.f;
   }
-  static __device__ __forceinline__ void load(Piece (&x)[NC], const T* __restrict__ row, int c, int dim) {
+  static __device__ __forceinline__ void load(P (&x)[NC], const T* __restrict__ row, int c, int dim) {
 #pragma unroll
     for (int k = 0; k < NC; ++k)
-      if (c + k * GROUP * E < dim) x[k] = *reinterpret_cast<const Piece*>(row + c + k * GROUP * E);
+      if (c + k * GROUP * E < dim) x[k] = *reinterpret_cast<const P*>(row + c + k * GROUP * E);
   }
-  __device__ __forceinline__ void add(const Piece (&x)[NC], int c, int dim) {
+  __device__ __forceinline__ void add(const P (&x)[NC], int c, int dim) {
 #pragma unroll
     for (int k = 0; k < NC; ++k)
       if (c + k * GROUP * E < dim) {
-        if constexpr (VEC) {
 #pragma unroll
-          for (int e = 0; e < E; ++e) acc[k][e] += to_f32(x[k][e]);
-        } else {
-          acc[k][0] += to_f32(x[k]);
-        }
+        for (int e = 0; e < E; ++e) acc[k][e] += piece_get<T, E>(x[k], e);
       }
   }
   // += dout rows perm[a .. b), in that order, U of them in flight
@@ -90,7 +94,7 @@ struct RowSum {
     constexpr int U = NC == 1 ? 8 : 4;
     const T* dout = (const T*)q.dout;
     for (int i = a; i < b; i += U) {
-      Piece x[U][NC];
+      P x[U][NC];
       int t[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) t[u] = q.perm[std::min(i + u, b - 1)];
@@ -102,19 +106,15 @@ struct RowSum {
         if (i + u < b) add(x[u], c, q.dim);
     }
   }
-  __device__ __forceinline__ void put(const EmbedBwdArgs& q, int64_t v, int c) const {
+  __device__ __forceinline__ void put(const EmbedBwdArgs& q, int64_t v, int c, float scale) const {
     T* dst = (T*)q.dtable + v * q.dim + c;
 #pragma unroll
     for (int k = 0; k < NC; ++k)
       if (c + k * GROUP * E < q.dim) {
-        if constexpr (VEC) {
-          typename Elem<T>::Vec o;
+        P o;
 #pragma unroll
-          for (int e = 0; e < E; ++e) o[e] = from_f32<T>(acc[k][e] * q.scale);
-          *reinterpret_cast<typename Elem<T>::Vec*>(dst + k * GROUP * E) = o;
-        } else {
-          dst[k * GROUP] = from_f32<T>(acc[k][0] * q.scale);
-        }
+        for (int e = 0; e < E; ++e) piece_set<T, E>(o, e, acc[k][e] * scale);
+        *reinterpret_cast<P*>(dst + k * GROUP * E) = o;
       }
   }
 };
@@ -123,10 +123,10 @@ struct RowSum {
 // rows are what keeps memory busy); the others take the runs of long rows
 constexpr int kRows = 4;
 
-template <typename T, bool VEC, int GROUP, int NC>
+template <typename T, int E, int GROUP, int NC>
 __global__ __launch_bounds__(256) void embed_bwd_kernel(EmbedBwdArgs q) {
-  typedef RowSum<T, VEC, GROUP, NC> Sum;
-  constexpr int E = Sum::E, STEP = GROUP * E * NC;
+  typedef RowSum<T, E, GROUP, NC> Sum;
+  constexpr int STEP = GROUP * E * NC;
   const int sub = threadIdx.x / GROUP, li = threadIdx.x % GROUP;
   const int64_t row_blocks = gridDim.x - q.run_blocks;
   if ((int64_t)blockIdx.x < row_blocks) {
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(256) void embed_bwd_kernel(EmbedBwdArgs q) {
 #pragma unroll
     for (int i = 0; i < kRows; ++i) first[i] = en[i] > st[i] ? q.perm[st[i]] : -1;
     for (int c = li * E; c < q.dim; c += STEP) {
-      typename Sum::Piece x[kRows][NC];
+      typename Sum::P x[kRows][NC];
 #pragma unroll
       for (int i = 0; i < kRows; ++i)
         if (first[i] >= 0) Sum::load(x[i], (const T*)q.dout + (int64_t)first[i] * q.ld, c, q.dim);
@@ -154,7 +154,7 @@ __global__ __launch_bounds__(256) void embed_bwd_kernel(EmbedBwdArgs q) {
           s.add(x[i], c, q.dim);
           s.rows(q, st[i] + 1, en[i], c);
         }
-        s.put(q, v0 + i, c);
+        s.put(q, v0 + i, c, first[i] >= 0 ? q.scale : 0.f);
       }
     }
   } else {
@@ -187,10 +187,10 @@ __global__ __launch_bounds__(256) void embed_bwd_kernel(EmbedBwdArgs q) {
 
 // The long row that begins in a run (its last one) = that run's last part + the first parts of the runs it goes on into.  One run per
 // block: its 512 / GROUP groups take every so many parts and add up through LDS, in the order of the groups.
-template <typename T, bool VEC, int GROUP, int NC>
+template <typename T, int E, int GROUP, int NC>
 __global__ __launch_bounds__(512) void embed_join_kernel(EmbedBwdArgs q) {
-  typedef RowSum<T, VEC, GROUP, NC> Sum;
-  constexpr int E = Sum::E, STEP = GROUP * E * NC, SUBS = 512 / GROUP;
+  typedef RowSum<T, E, GROUP, NC> Sum;
+  constexpr int STEP = GROUP * E * NC, SUBS = 512 / GROUP;
   __shared__ float part[SUBS][GROUP][NC * E];
   const int sub = threadIdx.x / GROUP, li = threadIdx.x % GROUP;
   const int64_t run = blockIdx.x, e0 = run * q.run, e1 = std::min<int64_t>(q.n, e0 + q.run);
@@ -222,7 +222,7 @@ __global__ __launch_bounds__(512) void embed_join_kernel(EmbedBwdArgs q) {
         for (int k = 0; k < NC; ++k)
 #pragma unroll
           for (int e = 0; e < E; ++e) s.acc[k][e] += part[o][li][k * E + e];
-      s.put(q, v, c);
+      s.put(q, v, c, q.scale);
     }
     __syncthreads();
   }
@@ -242,48 +242,64 @@ static EmbedWs embed_ws(int64_t n, int64_t rows, int dim) {
   return w;
 }
 
-template <typename T, bool VEC, int GROUP, int NC>
+template <typename T, int E, int GROUP, int NC>
 static int embed_bwd_launch(EmbedBwdArgs q, hipStream_t st) {
   const int per = 256 / GROUP;
   q.run = embed_run(q.n);
   const int64_t runs = q.n > q.run ? cdiv64(q.n, q.run) : 0;
   q.run_blocks = cdiv64(runs, per);
   const int64_t blocks = cdiv64(q.rows, per * kRows) + q.run_blocks;
-  hipLaunchKernelGGL((embed_bwd_kernel<T, VEC, GROUP, NC>), dim3((unsigned)blocks), dim3(256), 0, st, q);
+  hipLaunchKernelGGL((embed_bwd_kernel<T, E, GROUP, NC>), dim3((unsigned)blocks), dim3(256), 0, st, q);
   SX_LAUNCH_CHECK("embed_bwd");
   if (runs) {
-    hipLaunchKernelGGL((embed_join_kernel<T, VEC, GROUP, NC>), dim3((unsigned)runs), dim3(512), 0, st, q);
+    hipLaunchKernelGGL((embed_join_kernel<T, E, GROUP, NC>), dim3((unsigned)runs), dim3(512), 0, st, q);
     SX_LAUNCH_CHECK("embed_join");
   }
   return SX_OK;
 }
 
-template <typename T, bool VEC>
+template <typename T, int E>
 static int embed_bwd_pick(const EmbedBwdArgs& q, hipStream_t st) {
-  const int pieces = q.dim / (VEC ? 16 / (int)sizeof(T) : 1);
-  if (pieces <= 16) return embed_bwd_launch<T, VEC, 16, 1>(q, st);
-  if (pieces <= 64) return embed_bwd_launch<T, VEC, 64, 1>(q, st);
-  if (pieces <= 128) return embed_bwd_launch<T, VEC, 128, 1>(q, st);
-  return embed_bwd_launch<T, VEC, 128, 4>(q, st);
+  const int pieces = q.dim / E;
+  if (pieces <= 16) return embed_bwd_launch<T, E, 16, 1>(q, st);
+  if (pieces <= 64) return embed_bwd_launch<T, E, 64, 1>(q, st);
+  if (pieces <= 128) return embed_bwd_launch<T, E, 128, 1>(q, st);
+  return embed_bwd_launch<T, E, 128, 4>(q, st);
+}
+
+// elements of the widest load, up to 16 bytes, that rows of this length and stride from these addresses allow
+static int embed_width(int size, int dim, int64_t ld, const void* a, const void* b) {
+  int e = 16 / size;
+  while (e > 1 && (dim % e || ld % e || ((uintptr_t)a | (uintptr_t)b) % (e * size))) e /= 2;
+  return e;
 }
 
 template <typename T>
 static int embed_bwd(const EmbedBwdArgs& q, hipStream_t st) {
-  constexpr int E = 16 / (int)sizeof(T);
-  const bool vec = q.dim % E == 0 && q.ld % E == 0 && (uintptr_t)q.dout % 16 == 0 && (uintptr_t)q.dtable % 16 == 0;
-  return vec ? embed_bwd_pick<T, true>(q, st) : embed_bwd_pick<T, false>(q, st);
+  switch (embed_width(sizeof(T), q.dim, q.ld, q.dout, q.dtable)) {
+    case 1: return embed_bwd_pick<T, 1>(q, st);
+    case 2: return embed_bwd_pick<T, 2>(q, st);
+    case 4: return embed_bwd_pick<T, 4>(q, st);
+    default: return embed_bwd_pick<T, 16 / (int)sizeof(T)>(q, st);
+  }
+}
+
+template <typename T, typename I, int E>
+static int embed_fwd_launch(const void* table, int64_t ld, const void* ids, int64_t n, int64_t rows, int dim, float scale, void* out, hipStream_t st) {
+  const unsigned blocks = (unsigned)std::max<int64_t>(1, std::min<int64_t>(cdiv64(n * (dim / E), 256), 256 * 32));
+  hipLaunchKernelGGL((embed_fwd_kernel<T, I, E>), dim3(blocks), dim3(256), 0, st, (const T*)table, ld, (const I*)ids, n, rows, dim, scale, (T*)out);
+  SX_LAUNCH_CHECK("embed_fwd");
+  return SX_OK;
 }
 
 template <typename T, typename I>
 static int embed_fwd(const void* table, int64_t ld, const void* ids, int64_t n, int64_t rows, int dim, float scale, void* out, hipStream_t st) {
-  constexpr int E = 16 / (int)sizeof(T);
-  const bool vec = dim % E == 0 && ld % E == 0 && (uintptr_t)table % 16 == 0 && (uintptr_t)out % 16 == 0;
-  const int64_t total = n * (vec ? dim / E : dim);
-  const unsigned blocks = (unsigned)std::max<int64_t>(1, std::min<int64_t>(cdiv64(total, 256), 256 * 32));
-  if (vec) hipLaunchKernelGGL((embed_fwd_kernel<T, I, true>), dim3(blocks), dim3(256), 0, st, (const T*)table, ld, (const I*)ids, n, rows, dim, scale, (T*)out);
-  else hipLaunchKernelGGL((embed_fwd_kernel<T, I, false>), dim3(blocks), dim3(256), 0, st, (const T*)table, ld, (const I*)ids, n, rows, dim, scale, (T*)out);
-  SX_LAUNCH_CHECK("embed_fwd");
-  return SX_OK;
+  switch (embed_width(sizeof(T), dim, ld, table, out)) {
+    case 1: return embed_fwd_launch<T, I, 1>(table, ld, ids, n, rows, dim, scale, out, st);
+    case 2: return embed_fwd_launch<T, I, 2>(table, ld, ids, n, rows, dim, scale, out, st);
+    case 4: return embed_fwd_launch<T, I, 4>(table, ld, ids, n, rows, dim, scale, out, st);
+    default: return embed_fwd_launch<T, I, 16 / (int)sizeof(T)>(table, ld, ids, n, rows, dim, scale, out, st);
+  }
 }
 
 static int embed_check(const char* who, int dtype, int64_t n, int64_t rows, int dim, int64_t ld) {
