@@ -191,3 +191,23 @@ def test_padding_is_zero_whatever_the_scale():
     assert torch.equal(out[0], torch.zeros(40, device="cuda")) and torch.equal(out[2], out[0]) and torch.isinf(out[1]).all()
     (grad,) = torch.autograd.grad(out, (table,), torch.ones_like(out))
     assert torch.equal(grad[0], torch.zeros(40, device="cuda")) and torch.equal(grad[2], grad[0]) and torch.isinf(grad[1]).all()
+
+
+@pytest.mark.parametrize("n,V", [(16384, 1), (50000, 20), (50000, 300000), (300001, 70), (17_000_000, 5)])
+def test_many_ids(n, V):
+    """More ids of one row than a block's list holds, on its own or beside rare ones; more than an entry of a list can number.  Gradients of
+    ones are counts: whole numbers below 2^24, exact."""
+    from unet_amd.embedding import scaled_embedding
+    g = torch.Generator().manual_seed(n)
+    ids = torch.where(torch.rand(n, generator=g) < 0.8, torch.tensor(V // 2), torch.randint(-1, V + 1, (n,), generator=g)).to(torch.int32)
+    table = torch.zeros(V, 1, device="cuda", requires_grad=True)
+    out = scaled_embedding(ids.cuda(), table)
+    (grad,) = torch.autograd.grad(out, (table,), torch.ones_like(out))
+    ok = (ids >= 0) & (ids < V)
+    assert torch.equal(grad[:, 0].cpu().double(), torch.bincount(ids[ok].long(), minlength=V).double())
+    if n < 10 ** 6:
+        w = torch.randn(n, 1, generator=g)
+        a, b = (torch.autograd.grad(scaled_embedding(ids.cuda(), table), (table,), w.cuda())[0] for _ in range(2))
+        want = torch.zeros(V, 1, dtype=torch.float64).index_add_(0, ids[ok].long(), w[ok].double())
+        size = torch.zeros(V, 1, dtype=torch.float64).index_add_(0, ids[ok].long(), w[ok].double().abs())
+        assert torch.equal(a, b) and bool(((a.cpu().double() - want).abs() <= 1.01 * (n * U * size + U * want.abs()) + 1e-38).all())

@@ -5,10 +5,10 @@
 // wave owns a contiguous part of the ids, and each (wave, bucket) has its own counter, so an entry's place is the waves before, the
 // earlier entries of its own wave and its rank among the lanes -- no atomic whose order could show.
 //
-// Bound by latencies (a launch of this size alone is 4 us): 1024 ids 10 us, 16384 int64 ids over 32768 buckets 13.4 us evenly spread, 14.8 us
-// with most of them in few buckets, 15 to 20 us all in one.  With every id of the block handled in place, 64 to a step whatever their
-// number, the same were 14, 17, 22 and 32 us.  Beyond kSortPart ids per wave the list is made twice: 65536 ids 57 us, half of it each
-// block's passes over ids that are not its own.
+// Bound by latencies (a launch of this size alone is 4 us): 1024 ids 9 us, 16384 int64 ids over 32768 buckets 13 us evenly spread, 15 us with
+// most of them in few buckets, 15 to 20 us all in one, 65536 45 us.  With every id of the block handled in place, 64 to a step whatever
+// their number, the same were 14, 17, 22, 32 and 69 us.  Only a wave whose list cannot hold what the block owns of its part (16 million ids
+// and more, or nearly all of them in one block's buckets) reads its part again.
 #include "sort_ids.h"
 #include <algorithm>
 #include <atomic>
@@ -17,8 +17,7 @@ namespace sx {
 
 constexpr int kSortWaves = 16;          // 1024 threads
 constexpr int kSortBuckets = 1024;      // buckets per block: one per thread in the scan, 64 KB of counters
-constexpr int kSortPart = 1024;         // ids that a wave goes through at a time, and its list's entries: 64 KB for all
-constexpr int kSortLds = kSortWaves * (kSortBuckets + kSortPart + 2) * 4;
+constexpr int kSortLds = 160 * 1024;    // counters, 2 * kSortWaves sums, and the rest for the lists
 
 template <typename I>
 __global__ __launch_bounds__(1024) void sort_ids_kernel(const I* __restrict__ ids, int64_t n, int rows, int bits, int* __restrict__ perm,
@@ -26,19 +25,19 @@ __global__ __launch_bounds__(1024) void sort_ids_kernel(const I* __restrict__ id
   extern __shared__ int lds[];
   constexpr int U = 8;                                     // loads in flight per lane
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  int* const cnt = lds;                                    // [wave][bucket]
-  int* const mycnt = lds + wid * kSortBuckets;
-  int* const list = lds + kSortWaves * kSortBuckets + wid * kSortPart;      // this wave's: entry << 10 | bucket, both within the part / block
-  int(*const red)[kSortWaves] = reinterpret_cast<int(*)[kSortWaves]>(lds + kSortWaves * (kSortBuckets + kSortPart));      // [2]
+  const int buckets = 1 << bits, cap = ((kSortLds / 4 - 2 * kSortWaves) / kSortWaves - buckets) & ~63;      // cap: entries of a wave's list
+  int(*const red)[kSortWaves] = reinterpret_cast<int(*)[kSortWaves]>(lds);      // [2]
+  int* const cnt = lds + 2 * kSortWaves;                   // [wave][bucket]
+  int* const mycnt = cnt + wid * buckets;
+  int* const list = cnt + kSortWaves * buckets + wid * cap;      // this wave's: entry << 10 | bucket, within what was gathered / the block
   const int me = blockIdx.x, first = me << bits;
-  const bool mine = tid < (1 << bits) && first + tid <= rows;      // thread = one of the block's buckets
+  const bool mine = tid < buckets && first + tid <= rows;      // thread = one of the block's buckets
   const int64_t seg = (n + 1023) / 1024 * 64;              // this wave's part, a multiple of the lanes
   const int64_t s0 = std::min<int64_t>(n, wid * seg), s1 = std::min<int64_t>(n, s0 + seg);
-  for (int w = 0; w < kSortWaves; ++w) cnt[w * kSortBuckets + tid] = 0;
+  for (int i = tid; i < kSortWaves * buckets; i += 1024) cnt[i] = 0;
   int below = 0, len = 0;
-  // the block's own ids among kSortPart from t0 on -> list, in their order
-  auto gather = [&](int64_t t0, bool count) {
-    const int part = (int)std::min<int64_t>(kSortPart, s1 - t0);
+  // the block's own ids among the `part` from t0 on -> list, in their order; len: how many there are, more than cap if they did not fit
+  auto gather = [&](int64_t t0, int part, bool count) {
     len = 0;
     for (int p = 0; p < part; p += 64 * U) {
       I id[U];
@@ -51,15 +50,13 @@ __global__ __launch_bounds__(1024) void sort_ids_kernel(const I* __restrict__ id
         const bool own = in && b >> bits == me;
         if (count) below += in && b < first ? 1 : 0;
         const unsigned long long all = __ballot(own);
-        if (own) list[len + __popcll(all & ((1ull << lane) - 1))] = (p + u * 64 + lane) << 10 | (b - first);
+        const int at = len + __popcll(all & ((1ull << lane) - 1));
+        if (own && at < cap) list[at] = (p + u * 64 + lane) << 10 | (b - first);
         len += __popcll(all);
       }
     }
   };
-  __syncthreads();
-  const bool once = seg <= kSortPart;                      // then the list stays from here to the placing
-  for (int64_t t0 = s0; t0 < s1; t0 += kSortPart) {
-    gather(t0, true);
+  auto tally = [&]() {
     for (int i = lane; i - lane < len; i += 64) {
       const bool in = i < len;
       const int r = in ? list[i] & (kSortBuckets - 1) : -1, r0 = __builtin_amdgcn_readfirstlane(r);
@@ -70,7 +67,22 @@ __global__ __launch_bounds__(1024) void sort_ids_kernel(const I* __restrict__ id
         atomicAdd(&mycnt[r], 1);
       }
     }
+  };
+  // each(f): f for this wave's ids, whole if its list holds the block's own of them, else cap at a time
+  bool whole = false;
+  auto each = [&](bool again, auto&& f) {
+    if (whole) { f(s0); return; }
+    for (int64_t t0 = s0; t0 < s1; t0 += cap) {
+      gather(t0, (int)std::min<int64_t>(cap, s1 - t0), !again && s1 - s0 > (1 << 20));
+      f(t0);
+    }
+  };
+  __syncthreads();
+  if (s1 - s0 <= 1 << 20) {                                // (an entry has 22 bits)
+    gather(s0, (int)(s1 - s0), true);
+    whole = len <= cap;
   }
+  each(false, [&](int64_t) { tally(); });
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) below += __shfl_xor(below, o, 64);
   if (lane == 0) red[0][wid] = below;
@@ -78,7 +90,7 @@ __global__ __launch_bounds__(1024) void sort_ids_kernel(const I* __restrict__ id
   // exclusive scan over this block's buckets, one per thread
   int tot = 0;
   if (mine)
-    for (int w = 0; w < kSortWaves; ++w) tot += cnt[w * kSortBuckets + tid];
+    for (int w = 0; w < kSortWaves; ++w) tot += cnt[w * buckets + tid];
   int inc = tot;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -97,14 +109,13 @@ __global__ __launch_bounds__(1024) void sort_ids_kernel(const I* __restrict__ id
     start[first + tid] = base;
     end[first + tid] = base + tot;
     for (int w = 0; w < kSortWaves; ++w) {
-      const int c = cnt[w * kSortBuckets + tid];
-      cnt[w * kSortBuckets + tid] = base;
+      const int c = cnt[w * buckets + tid];
+      cnt[w * buckets + tid] = base;
       base += c;
     }
   }
   __syncthreads();
-  for (int64_t t0 = s0; t0 < s1; t0 += kSortPart) {
-    if (!once) gather(t0, false);
+  each(true, [&](int64_t t0) {
     for (int i = lane; i - lane < len; i += 64) {
       const bool in = i < len;
       const int e = in ? list[i] : -1, r = e & (kSortBuckets - 1);
@@ -124,7 +135,7 @@ __global__ __launch_bounds__(1024) void sort_ids_kernel(const I* __restrict__ id
         key[p] = first + r;
       }
     }
-  }
+  });
 }
 
 template <typename I>
