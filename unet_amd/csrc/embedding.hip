@@ -11,11 +11,13 @@
 
 namespace sx {
 
-// Entries a group sums in a row: about 1024 runs, 16 entries at least.  A group's time is a chain of memory latencies, eight rows at a
-// time: 16384 tokens took 48 us in runs of 64.
-static inline int embed_run(int64_t n) {
-  int run = 16;
-  while ((int64_t)run * 1024 < n) run *= 2;
+// Entries a group of threads sums in a row: about 1024 runs, more for small groups, kMinRun entries at least.  A group's time
+// is a chain of memory latencies, eight rows at a time (16384 tokens of 1024 bf16: 18 us in runs of 16, 48 us in runs of 64), that of a
+// row's join grows with its runs.
+constexpr int kMinRun = 16;
+static inline int embed_run(int64_t n, int group) {
+  int run = kMinRun;
+  while ((int64_t)run * (group >= 64 ? 1024 : 4096) < n) run *= 2;
   return run;
 }
 constexpr int64_t kMaxRows = 1 << 24;      // the gradient's grid gives every row of the table up to 128 threads of a 2^32 limit
@@ -119,34 +121,33 @@ struct RowSum {
   }
 };
 
-// Blocks [0, gridDim.x - run_blocks) take the rows of the table, kRows per group (most of them have no token or one: the loads of several
-// rows are what keeps memory busy); the others take the runs of long rows
-constexpr int kRows = 4;
-
-template <typename T, int E, int GROUP, int NC>
+// Blocks [0, gridDim.x - run_blocks) take the rows of the table, ROWS per group; the others take the runs of long rows.  Where most rows have
+// no token or one the loads of four rows are what keeps memory busy; where they have many, four after another take four times as long
+// (65000 tokens, 1000 rows of 500 bf16: 47 us by four, 20 by one)
+template <typename T, int E, int GROUP, int NC, int ROWS>
 __global__ __launch_bounds__(256) void embed_bwd_kernel(EmbedBwdArgs q) {
   typedef RowSum<T, E, GROUP, NC> Sum;
   constexpr int STEP = GROUP * E * NC;
   const int sub = threadIdx.x / GROUP, li = threadIdx.x % GROUP;
   const int64_t row_blocks = gridDim.x - q.run_blocks;
   if ((int64_t)blockIdx.x < row_blocks) {
-    const int64_t v0 = (blockIdx.x * (int64_t)(256 / GROUP) + sub) * kRows;
+    const int64_t v0 = (blockIdx.x * (int64_t)(256 / GROUP) + sub) * ROWS;
     if (v0 >= q.rows) return;
-    int st[kRows], en[kRows], first[kRows];
+    int st[ROWS], en[ROWS], first[ROWS];
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
+    for (int i = 0; i < ROWS; ++i) {
       st[i] = q.start[std::min<int64_t>(v0 + i, q.rows)];
       en[i] = q.end[std::min<int64_t>(v0 + i, q.rows)];
     }
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) first[i] = en[i] > st[i] ? q.perm[st[i]] : -1;
+    for (int i = 0; i < ROWS; ++i) first[i] = en[i] > st[i] ? q.perm[st[i]] : -1;
     for (int c = li * E; c < q.dim; c += STEP) {
-      typename Sum::P x[kRows][NC];
+      typename Sum::P x[ROWS][NC];
 #pragma unroll
-      for (int i = 0; i < kRows; ++i)
+      for (int i = 0; i < ROWS; ++i)
         if (first[i] >= 0) Sum::load(x[i], (const T*)q.dout + (int64_t)first[i] * q.ld, c, q.dim);
 #pragma unroll
-      for (int i = 0; i < kRows; ++i) {
+      for (int i = 0; i < ROWS; ++i) {
         if (v0 + i >= q.rows || en[i] - st[i] > q.run) continue;
         Sum s;
         s.clear();
@@ -202,14 +203,24 @@ __global__ __launch_bounds__(512) void embed_join_kernel(EmbedBwdArgs q) {
   for (int c = li * E; c - li * E < q.dim; c += STEP) {
     Sum s;
     s.clear();
-#pragma unroll 4
-    for (int64_t r = run + sub; r <= last; r += SUBS) {
-      const float* p = q.part + (r * 2 + (r == run ? 1 : 0)) * q.dim + c;
+    constexpr int U = NC * E <= 8 ? 8 : 4;              // parts in flight; no branch around a load, columns behind the last read the first
+    for (int64_t r0 = run + sub; r0 <= last; r0 += SUBS * U) {
+      float x[U][NC][E];
 #pragma unroll
-      for (int k = 0; k < NC; ++k)
-        if (c + k * GROUP * E < q.dim)
+      for (int u = 0; u < U; ++u) {
+        const int64_t r = std::min(r0 + u * SUBS, last);
+        const float* p = q.part + (r * 2 + (r == run ? 1 : 0)) * q.dim;
 #pragma unroll
-          for (int e = 0; e < E; ++e) s.acc[k][e] += p[k * GROUP * E + e];
+        for (int k = 0; k < NC; ++k)
+#pragma unroll
+          for (int e = 0; e < E; ++e) x[u][k][e] = p[(c + k * GROUP * E < q.dim ? c + k * GROUP * E : 0) + e];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int k = 0; k < NC; ++k)
+#pragma unroll
+          for (int e = 0; e < E; ++e) s.acc[k][e] += r0 + u * SUBS <= last ? x[u][k][e] : 0.f;
     }
 #pragma unroll
     for (int k = 0; k < NC; ++k)
@@ -236,8 +247,7 @@ static EmbedWs embed_ws(int64_t n, int64_t rows, int dim) {
   w.key = o; o = align_up(o + (size_t)n * 4, 256);
   w.start = o; o = align_up(o + (size_t)(rows + 1) * 4, 256);
   w.end = o; o = align_up(o + (size_t)(rows + 1) * 4, 256);
-  const int run = embed_run(n);
-  w.part = o; o = align_up(o + (n > run ? (size_t)cdiv64(n, run) * 2 * (size_t)dim * 4 : 0), 256);
+  w.part = o; o = align_up(o + (n > kMinRun ? (size_t)cdiv64(n, kMinRun) * 2 * (size_t)dim * 4 : 0), 256);
   w.total = o;
   return w;
 }
@@ -245,11 +255,13 @@ static EmbedWs embed_ws(int64_t n, int64_t rows, int dim) {
 template <typename T, int E, int GROUP, int NC>
 static int embed_bwd_launch(EmbedBwdArgs q, hipStream_t st) {
   const int per = 256 / GROUP;
-  q.run = embed_run(q.n);
+  q.run = embed_run(q.n, GROUP);
   const int64_t runs = q.n > q.run ? cdiv64(q.n, q.run) : 0;
   q.run_blocks = cdiv64(runs, per);
-  const int64_t blocks = cdiv64(q.rows, per * kRows) + q.run_blocks;
-  hipLaunchKernelGGL((embed_bwd_kernel<T, E, GROUP, NC>), dim3((unsigned)blocks), dim3(256), 0, st, q);
+  const int by = q.n > 2 * q.rows ? 1 : 4;
+  const dim3 grid((unsigned)(cdiv64(q.rows, per * by) + q.run_blocks));
+  if (by == 1) hipLaunchKernelGGL((embed_bwd_kernel<T, E, GROUP, NC, 1>), grid, dim3(256), 0, st, q);
+  else hipLaunchKernelGGL((embed_bwd_kernel<T, E, GROUP, NC, 4>), grid, dim3(256), 0, st, q);
   SX_LAUNCH_CHECK("embed_bwd");
   if (runs) {
     hipLaunchKernelGGL((embed_join_kernel<T, E, GROUP, NC>), dim3((unsigned)runs), dim3(512), 0, st, q);
