@@ -423,7 +423,7 @@ int sx_adapter_backward(int dtype, int64_t T, int K, int N, int r, int G, const 
  *                         d loss / d logits (for mean = 0: of the plain sum).  row_stats (nullable) [4][N]: kept for the call below.
  *   sx_distill_backward : dlogits = g[t * g_stride] * (the same gradient), from the logits and row_stats of the forward call.
  *                         ready != 0: dlogits still is what that forward call wrote; rows with g = 1 are then left as they are.
- * 0 < tau < inf; N < 2^22.
+ * 2^-126 <= tau < inf; N < 2^22; V, K <= 2^30.
  * --------------------------------------------------------------------------------------------- */
 int sx_distill_forward(int dtype, int64_t N, int V, int K, const void* logits, int64_t ld, int top_dtype, const void* top,
                        const void* idx, int idx64, float tau, const float* weights, int mean, float* row_loss,

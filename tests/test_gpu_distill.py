@@ -327,3 +327,25 @@ def _check_rows(z, top, idx, w, g):
     E = (6 * A + z.shape[1] / 64 + 64) * U
     assert bool(((grad.double() - c * (q - sp)).abs() <= c.abs() * E * (q + sp) + 1.01 * 2 * U * (c * (q - sp)).abs() + 1e-38).all())
     assert bool(((loss.detach().double() - want).abs() <= w.double() * (2 * E + E * d.abs().amax(1) + 8 * U * (A + math.log(z.shape[1]))) + U * want.abs()).all())
+
+
+@pytest.mark.parametrize("tau", [1e-4, 1e-20])
+def test_temperatures_near_zero(tau):
+    """Both distributions are one-hot: the loss is tau * (z_max - z at the teacher's best), the gradient tau * (one-hot - one-hot) / rows.  Each is a
+    difference, a product by 1 / tau and two by tau: at most 8 u of itself."""
+    z, top, idx = _inputs((4,), 300, 5)
+    with torch.no_grad():
+        z.mul_(16).round_()                                # gaps of whole numbers, not ties
+        z[:, 7] = 200.0
+        top.copy_(torch.arange(5.0).expand(4, 5))
+    from unet_amd.losses import distillation_loss
+    loss = distillation_loss(z, top, idx, temperature=tau)
+    (grad,) = torch.autograd.grad(loss, (z,))
+    zd, best = z.detach().double().cpu(), idx[:, 4].cpu()
+    t = float(torch.tensor(tau, dtype=torch.float32))
+    want = (t * (200.0 - zd.gather(1, best[:, None])[:, 0])).mean()
+    wg = torch.zeros(4, 300, dtype=torch.float64)
+    wg[:, 7] += t / 4
+    wg.scatter_add_(1, best[:, None], torch.full((4, 1), -t / 4, dtype=torch.float64))
+    assert abs(float(loss.detach()) - float(want)) <= 8 * U * float(want)
+    assert bool(((grad.cpu().double() - wg).abs() <= 8 * U * wg.abs()).all())

@@ -102,3 +102,18 @@ def test_adapter_c_entry_refusals():
     for kw in (dict(dt=9), dict(T=0), dict(x=None), dict(w=None), dict(A=None), dict(B=None), dict(dy=None), dict(kept=None), dict(ws=None), dict(ldx=15),
                dict(ldw=15), dict(ldd=7), dict(ldd=9), dict(dy=odd), dict(nk=nk - 1), dict(nw=nb - 1), dict(kept=odd), dict(ws=odd)):
         _bad(bwd(**kw))
+
+
+def test_temperatures_and_sizes_out_of_reach_are_refused():
+    """A temperature whose reciprocal is infinite in 32 bits, or that is infinite there itself; rows that 32-bit positions cannot number."""
+    from unet_amd import _lib as L
+    from unet_amd.losses import distillation_loss
+    z = torch.zeros(2, 5)
+    for t in (1e-40, 1e39):
+        with pytest.raises(ValueError, match="temperature"):
+            distillation_loss(z, z, torch.zeros(2, 5, dtype=torch.int64), temperature=t)
+    lib, P = L.lib(), 4096
+    for kw in (dict(V=(1 << 30) + 1), dict(K=(1 << 30) + 1), dict(tau=1e-40)):
+        a = dict(V=10, K=2, tau=1.0)
+        a.update(kw)
+        assert lib.sx_distill_forward(0, 3, a["V"], a["K"], P, 1 << 31, 0, P, P, 1, a["tau"], None, 1, P, None, P, None, None, 10, None) < 0

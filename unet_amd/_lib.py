@@ -7,6 +7,7 @@ shape, matching the reference's error conventions) or RuntimeError (HIP failure)
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 
 import torch
@@ -207,6 +208,12 @@ def launch(name, device, *args):
         with torch.cuda.device(i):
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     return rc if rc >= 0 else check(rc, name)
+
+
+@functools.lru_cache(maxsize=1024)
+def size_of(name, *args):
+    """Bytes that the entry point `name` answers with for these sizes (its answer depends on nothing else)."""
+    return check(getattr(_lib or lib(), name)(*args), name)
 
 
 def once(who):

@@ -22,7 +22,6 @@ def _factors(A, B):
 
 def _project(x, weight, bias, A, B, ids, scales, keep):
     """(y, what the backward pass needs of it if `keep`)"""
-    lib = L.lib()
     N, K = weight.shape
     G, r = A.shape[:2]
     dt, dev = L.dtype_code(x, "adapter_linear"), x.device
@@ -31,8 +30,8 @@ def _project(x, weight, bias, A, B, ids, scales, keep):
     T = x2.shape[0]
     Ad, Bd = _factors(A, B)
     y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=dev)
-    nk = L.check(lib.sx_adapter_kept_bytes(dt, T, r, G), "sx_adapter_kept_bytes") if keep else 0
-    nw = L.check(lib.sx_adapter_workspace_bytes(dt, T, K, N, r, G, L.SX_ADAPTER_FORWARD if keep else L.SX_ADAPTER_ALONE), "sx_adapter_workspace_bytes")
+    nk = L.size_of("sx_adapter_kept_bytes", dt, T, r, G) if keep else 0
+    nw = L.size_of("sx_adapter_workspace_bytes", dt, T, K, N, r, G, L.SX_ADAPTER_FORWARD if keep else L.SX_ADAPTER_ALONE)
     kept = torch.empty(nk, dtype=torch.uint8, device=dev) if keep else None
     ws = torch.empty(nw, dtype=torch.uint8, device=dev)
     L.launch("sx_adapter_forward", dev, dt, T, K, N, r, G, L.addr(x2), ldx, L.addr(w), ldw, L.addr(bias), L.addr(Ad), L.addr(Bd), L.addr(scales),
@@ -68,7 +67,7 @@ class _AdapterFn(torch.autograd.Function):
         w, ldw = L.rows_2d(weight, K)
         d2, ldd = L.rows_2d(dy, N, aligned=True)
         Ad, Bd = A.contiguous(), B.contiguous()
-        nw = L.check(L.lib().sx_adapter_workspace_bytes(dt, T, K, N, r, G, L.SX_ADAPTER_BACKWARD), "sx_adapter_workspace_bytes")
+        nw = L.size_of("sx_adapter_workspace_bytes", dt, T, K, N, r, G, L.SX_ADAPTER_BACKWARD)
         ws = torch.empty(nw, dtype=torch.uint8, device=dev)
         L.launch("sx_adapter_backward", dev, dt, T, K, N, r, G, L.addr(x2), ldx, L.addr(w), ldw, L.addr(Ad), L.addr(Bd), L.addr(scales), L.addr(d2), ldd,
                  L.addr(kept), kept.numel(), L.addr(dx), L.addr(dA), L.addr(dB), L.addr(ws), nw)

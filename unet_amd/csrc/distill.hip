@@ -88,12 +88,13 @@ __device__ __forceinline__ float mul_rn(float a, float b) {
 
 // exponent of 2 of a logit relative to the row's maximum.  z * c - m * c in one fma: m * c is rounded, but alike for all of the row (and
 // sums move from one maximum to another by the difference of the rounded products).
-// Beyond kFar (a row whose every logit is the type's lowest value) m * c could overflow: the difference is taken first.
-constexpr float kFar = 1e30f;
+// Beyond kFar (a row whose every logit is the type's lowest value) or kSharp (a temperature near zero) m * c could overflow: the difference
+// is taken first.
+constexpr float kFar = 1e30f, kSharp = 2e6f;
 struct Expo {
   float c, m, mc;
   bool far;
-  __device__ __forceinline__ Expo(float m_, float c_) : c(c_), m(m_), mc(mul_rn(m_, c_)), far(!(fabsf(m_) < kFar)) {}
+  __device__ __forceinline__ Expo(float m_, float c_) : c(c_), m(m_), mc(mul_rn(m_, c_)), far(!(fabsf(m_) < kFar && c_ < kSharp)) {}
   __device__ __forceinline__ float at(float z) const { return far ? (z - m) * c : fmaf(z, c, -mc); }
 };
 
@@ -382,7 +383,7 @@ __global__ __launch_bounds__(NT) void distill_wide_kernel(DistillArgs a) {
       }
       m = all_max<NT>(mk, red);
       s = mul_rn(s, __builtin_amdgcn_exp2f(mul_rn(mk, c) - mul_rn(m, c)));
-      if (!(fabsf(m) < kFar) || !(fabsf(c) < 1e6f)) {     // products that overflow: the row again, by differences
+      if (!(fabsf(m) < kFar && c < kSharp)) {     // products that overflow: the row again, by differences
         mk = -INFINITY;
         for (int v = tid; v < a.V; v += NT) mk = fmaxf(mk, to_f32(z[v]));
         m = all_max<NT>(mk, red);
@@ -529,8 +530,8 @@ static int distill_launch(const DistillArgs& a, hipStream_t st) {
 
 static int distill_check(const char* who, int dtype, int64_t N, int V, int K, int64_t ld, int top_dtype, float tau) {
   SX_REQUIRE((dtype == SX_F32 || dtype == SX_BF16) && (top_dtype == SX_F32 || top_dtype == SX_BF16), "%s: dtypes %d / %d are neither fp32 nor bf16", who, dtype, top_dtype);
-  SX_REQUIRE(N >= 0 && N < (1 << 22) && V > 0 && K > 0 && ld >= V, "%s: bad sizes N=%lld V=%d K=%d ld=%lld", who, (long long)N, V, K, (long long)ld);
-  SX_REQUIRE(tau > 0.f && tau < INFINITY, "%s: the temperature must be positive and finite, got %g", who, (double)tau);
+  SX_REQUIRE(N >= 0 && N < (1 << 22) && V > 0 && V <= (1 << 30) && K > 0 && K <= (1 << 30) && ld >= V, "%s: bad sizes N=%lld V=%d K=%d ld=%lld", who, (long long)N, V, K, (long long)ld);
+  SX_REQUIRE(tau >= 1.17549435e-38f && tau < INFINITY, "%s: the temperature must be positive, normal and finite, got %g", who, (double)tau);      // 1 / tau is finite
   return SX_OK;
 }
 

@@ -36,7 +36,7 @@ class _EmbeddingFn(torch.autograd.Function):
         n, dev = i.numel(), dout.device
         d, ld = L.rows_2d(dout, D)
         grad = torch.empty(V, D, dtype=dtype, device=dev)
-        nb = L.check(L.lib().sx_embedding_workspace_bytes(n, V, D), "sx_embedding_workspace_bytes")
+        nb = L.size_of("sx_embedding_workspace_bytes", n, V, D)
         ws = torch.empty(nb, dtype=torch.uint8, device=dev)
         L.launch("sx_embedding_backward", dev, L.dtype_code(grad, "scaled_embedding"), n, V, D, L.addr(d), ld, L.addr(i),
                  L.ids_flag(i, "scaled_embedding"), scale, L.addr(grad), L.addr(ws), nb)

@@ -213,8 +213,8 @@ def distillation_loss(logits, top_logits, top_idx, *, temperature=1.0, weights=N
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"Unknown reduction={reduction}")
     tau = float(temperature)
-    if not 0.0 < tau < float("inf"):
-        raise ValueError(f"{who}: temperature must be positive and finite, got {temperature}")
+    if not 2.0 ** -126 <= tau < 2.0 ** 128:
+        raise ValueError(f"{who}: temperature must be positive and finite (normal in 32 bits), got {temperature}")
     for t in (logits, top_logits, top_idx):
         _require_cuda(t, who)
     if logits.dim() < 1 or logits.shape[-1] < 1:
