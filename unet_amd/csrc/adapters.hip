@@ -13,6 +13,11 @@
 //           meets, with h (dh) as an operand: the adapter's share goes through the same accumulators and is rounded once, with
 //           the product.  bf16 MFMA takes h as two bf16 parts (adapters.h).
 //   outer   dA and dB: sums over an adapter's rows
+//
+// Measured at 4096 x 2048 -> 4096 bf16, four adapters of rank 32: sort 7, shrink 14 (forward, 17 MB of x, 1.2 TB/s) and 24 us (backward, 34 MB
+// of dy, 1.4 TB/s; bound by the latencies of 256 blocks, one a CU), project 74 and 72, pack 9 (34 MB, 3.7 TB/s), outer 21 (50 MB, 2.4
+// TB/s; each gathered row's 128-byte pieces once per block of columns).  At 8192 x 4096 -> 4096, rank 16: sort 8.6, shrink 25 (67 MB, 2.7 TB/s),
+// project 244.
 #include "adapters.h"
 #include "sort_ids.h"
 #include <algorithm>
