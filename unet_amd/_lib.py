@@ -193,6 +193,18 @@ def torch_clone(t):
     return t.clone(memory_format=torch.contiguous_format)
 
 
+def packed(t, aligned=False):
+    """Contiguous tensor; aligned: one whose last dimension is a whole number of 16-byte pieces also starts on 16 bytes."""
+    if not t.is_contiguous():
+        return torch_clone(t)
+    return torch_clone(t) if aligned and t.data_ptr() % 16 and t.shape[-1] * t.element_size() % 16 == 0 else t
+
+
+def plain_f32(t):
+    """Contiguous float32 without a history, the tensor itself where it is that."""
+    return t if t.dtype == torch.float32 and not t.requires_grad and t.is_contiguous() else t.detach().float().contiguous()
+
+
 def addr(t):
     """Device address of a tensor as an int (None stays None): what a c_void_p argument takes without an object around it."""
     return None if t is None else t.data_ptr()

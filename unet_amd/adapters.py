@@ -16,10 +16,6 @@ from . import _lib as L
 MAX_RANK = 128
 
 
-def _factors(A, B):
-    return L.rows_2d(A.contiguous(), A.shape[2], aligned=True)[0], L.rows_2d(B.contiguous(), B.shape[2], aligned=True)[0]
-
-
 def _project(x, weight, bias, A, B, ids, scales, keep):
     """(y, what the backward pass needs of it if `keep`)"""
     N, K = weight.shape
@@ -28,7 +24,7 @@ def _project(x, weight, bias, A, B, ids, scales, keep):
     x2, ldx = L.rows_2d(x, K, aligned=True)
     w, ldw = L.rows_2d(weight, K, aligned=True)
     T = x2.shape[0]
-    Ad, Bd = _factors(A, B)
+    Ad, Bd = L.packed(A, aligned=True), L.packed(B, aligned=True)
     y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=dev)
     nk = L.size_of("sx_adapter_kept_bytes", dt, T, r, G) if keep else 0
     nw = L.size_of("sx_adapter_workspace_bytes", dt, T, K, N, r, G, L.SX_ADAPTER_FORWARD if keep else L.SX_ADAPTER_ALONE)
@@ -42,7 +38,7 @@ def _project(x, weight, bias, A, B, ids, scales, keep):
 class _AdapterFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, A, B, ids, scales):
-        y, kept = _project(x.detach(), weight, bias, A.detach(), B.detach(), ids, scales, True)
+        y, kept = _project(x, weight, bias, A, B, ids, scales, True)
         ctx.save_for_backward(x, weight, A, B, scales, kept)
         return y
 
@@ -66,7 +62,7 @@ class _AdapterFn(torch.autograd.Function):
             return dx, None, None, dA, dB, None, None
         w, ldw = L.rows_2d(weight, K)
         d2, ldd = L.rows_2d(dy, N, aligned=True)
-        Ad, Bd = A.contiguous(), B.contiguous()
+        Ad, Bd = L.packed(A), L.packed(B)
         nw = L.size_of("sx_adapter_workspace_bytes", dt, T, K, N, r, G, L.SX_ADAPTER_BACKWARD)
         ws = torch.empty(nw, dtype=torch.uint8, device=dev)
         L.launch("sx_adapter_backward", dev, dt, T, K, N, r, G, L.addr(x2), ldx, L.addr(w), ldw, L.addr(Ad), L.addr(Bd), L.addr(scales), L.addr(d2), ldd,
@@ -110,9 +106,7 @@ def adapter_linear(x, weight, bias, A, B, ids, *, scales=None):
         raise ValueError(f"{who}: ids must be {lead} or one per leading index of it, got {tuple(ids.shape)}")
     if ids.dim() < len(lead):
         ids = ids.reshape(tuple(ids.shape) + (1,) * (len(lead) - ids.dim())).expand(lead)
-    if scales is not None:
-        scales = scales.detach().float().contiguous()
-    args = (x, weight, None if bias is None else bias.contiguous(), A, B, ids.contiguous(), scales)
+    args = (x, weight, None if bias is None else L.packed(bias), A, B, L.packed(ids), None if scales is None else L.plain_f32(scales))
     return _AdapterFn.apply(*args) if L.wants_grad(x, A, B) else _project(*args, False)[0]
 
 

@@ -12,7 +12,7 @@ from . import _lib as L
 def _lookup(ids, table, scale):
     """(flat ids, output)"""
     V, D = table.shape
-    i = ids.contiguous()
+    i = L.packed(ids)
     t, ld = L.rows_2d(table, D)
     out = torch.empty(*ids.shape, D, dtype=table.dtype, device=table.device)
     L.launch("sx_embedding_forward", table.device, L.dtype_code(table, "scaled_embedding"), i.numel(), V, D, L.addr(t), ld, L.addr(i),
@@ -23,7 +23,7 @@ def _lookup(ids, table, scale):
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, table, scale):
-        i, out = _lookup(ids, table.detach(), scale)
+        i, out = _lookup(ids, table, scale)
         ctx.save_for_backward(i)
         ctx.meta = (*table.shape, scale, table.dtype)
         return out

@@ -175,7 +175,7 @@ def _distill(logits, top, idx, weights, tau, reduction, need):
 class _DistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, top, idx, weights, tau, reduction):
-        loss, keep, ctx.d = _distill(logits.detach(), top, idx, weights, tau, reduction, True)
+        loss, keep, ctx.d = _distill(logits, top, idx, weights, tau, reduction, True)
         ctx.save_for_backward(logits, top, idx, weights, keep)
         ctx.meta = (tau, reduction)
         return loss
@@ -194,7 +194,7 @@ class _DistillFn(torch.autograd.Function):
         if not ready:
             d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         z, ld = L.rows_2d(logits, V)
-        g = g.float().contiguous()
+        g = L.plain_f32(g)
         L.launch("sx_distill_backward", logits.device, L.dtype_code(logits, who), z.shape[0], V, K, L.addr(z), ld, L.dtype_code(top, who), L.addr(top),
                  L.addr(idx), L.ids_flag(idx, who), tau, L.addr(weights), 1 if reduction == "mean" else 0, L.addr(keep) + 4, L.addr(keep), L.addr(g),
                  1 if reduction == "none" else 0, 1 if ready else 0, L.addr(d), V)
@@ -228,11 +228,11 @@ def distillation_loss(logits, top_logits, top_idx, *, temperature=1.0, weights=N
     if weights is not None:
         if tuple(weights.shape) != lead:
             raise ValueError(f"{who}: weights must be {lead}, got {tuple(weights.shape)}")
-        weights = weights.detach().to(device=logits.device, dtype=torch.float32).contiguous()
-    top = top_logits.detach().contiguous()
+        weights = L.plain_f32(weights if weights.device == logits.device else weights.to(logits.device))
+    top, idx = L.packed(top_logits.detach() if top_logits.requires_grad else top_logits), L.packed(top_idx)
     if L.wants_grad(logits):
-        return _DistillFn.apply(logits, top, top_idx.contiguous(), weights, tau, reduction)
-    return _distill(logits, top, top_idx.contiguous(), weights, tau, reduction, False)[0]
+        return _DistillFn.apply(logits, top, idx, weights, tau, reduction)
+    return _distill(logits, top, idx, weights, tau, reduction, False)[0]
 
 
 def edge_weights(mask_np: np.ndarray, sigma_px: float = 3.0) -> np.ndarray:
