@@ -349,3 +349,32 @@ def test_temperatures_near_zero(tau):
     wg.scatter_add_(1, best[:, None], torch.full((4, 1), -t / 4, dtype=torch.float64))
     assert abs(float(loss.detach()) - float(want)) <= 8 * U * float(want)
     assert bool(((grad.cpu().double() - wg).abs() <= 8 * U * wg.abs()).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V,K", [(700, 65), (3000, 100), (6000, 128), (40, 129), (1500, 200), (2500, 256), (5000, 256), (12000, 200), (20000, 64), (30000, 257)])
+def test_pairs_per_thread(V, K, dtype):
+    """Every size of block that the pairs can ask for, with rows that fill one to sixteen vectors a thread."""
+    for red, g in (("mean", None), ("none", torch.tensor([0.5, 1.0, -3.0]).cuda())):
+        z, top, idx = _inputs((3,), V, K, dtype, torch.bfloat16, torch.int32, seed=K)
+        idx[1, ::3] = -1
+        _check(z, top, idx, 1.25, None, red, g)
+
+
+@pytest.mark.parametrize("V", [100, 900, 1800, 3700, 7000, 15000, 30000, 60000, 120000])
+def test_loss_without_a_gradient(V):
+    """The loss alone is what it is beside a gradient, for rows of every size class and more rows than blocks hold at once."""
+    from unet_amd.losses import distillation_loss
+    N = 600 if V > 5000 else 9000
+    z, top, idx = _inputs((N,), V, 8, torch.bfloat16, seed=V) if V <= 5000 else (torch.randn(N, V, device="cuda").to(torch.bfloat16).requires_grad_(True),
+                                                                                 torch.randn(N, 8, device="cuda"), torch.randint(0, V, (N, 8), device="cuda"))
+    alone = distillation_loss(z.detach(), top, idx, reduction="none")
+    q = torch.log_softmax(z.detach().double(), 1)
+    p = torch.softmax(top.double(), 1)
+    d = torch.log(p) - q.gather(1, idx)
+    E = (6 * 60.0 + V / 64 + 64) * U
+    tol = 2 * E + E * d.abs().amax(1) + 8 * U * (60.0 + math.log(V))
+    want = (p * d).sum(1)
+    assert bool(((alone.double() - want).abs() <= tol + U * want.abs()).all())
+    total = distillation_loss(z, top, idx, reduction="sum")
+    assert abs(float(total.detach()) - float(want.sum())) <= float(tol.sum() + N * U * want.abs().sum())
