@@ -331,3 +331,59 @@ def test_module_starts_as_the_shared_projection_and_trains_its_adapters_alone():
     assert (y.detach().double() - ref).abs().max() <= 52 * U * (x.abs().double() @ lin.weight.detach().abs().double().t() + 1).max()
     y.square().sum().backward()
     assert m.B.grad.abs().max() > 0 and not m.A.grad.any() and lin.weight.grad is None and lin.bias.grad is None
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,K,N,r,G,kind", [(84, 2880, 128, 8, 1, "segments"), (399, 64, 2112, 24, 36, "random"), (250, 4000, 100, 33, 20, "random"),
+                                            (1022, 1300, 136, 5, 2, "random"), (70, 19, 20, 19, 118, "random"), (1500, 200, 1950, 40, 90, "random"),
+                                            (530, 2050, 330, 128, 33, "segments")])
+def test_reductions_in_parts_and_seldom_shared_adapters(T, K, N, r, G, kind, dtype):
+    """Few tiles with a long reduction in either direction, fragments of many adapters, rows that come one by one."""
+    _check(_inputs(T, K, N, r, G, dtype, kind))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("K,N,G", [(96, 80, 12), (3200, 64, 2), (64, 3200, 30)])
+def test_nan_stays_in_its_row_and_adapter_in_parts_too(K, N, G, dtype):
+    from unet_amd.adapters import adapter_linear
+    i = _inputs(100, K, N, 8, G, dtype)
+    ids = i["ids"].cpu()
+    with torch.no_grad():
+        i["A"][1] = float("nan")
+        i["B"][1, :, 3] = float("inf")
+        row = int((ids != 1).nonzero()[5])
+        i["x"][row] = float("nan")
+    y, dx, dA, dB = _call(i)
+    bad = (ids == 1)
+    bad[row] = True
+    assert torch.isnan(y.cpu()[bad]).all() and torch.isfinite(y.cpu()[~bad]).all()
+    bad[row] = False                                       # dx of the NaN row does not depend on it
+    assert torch.isfinite(dx.cpu()[~bad]).all()
+    sound = torch.ones(G, dtype=torch.bool)
+    sound[1] = False
+    if ids[row] >= 0 and ids[row] < G:
+        sound[ids[row]] = False
+    assert torch.isfinite(dA.cpu()[sound]).all() and torch.isfinite(dB.cpu()[sound]).all()
+
+
+@pytest.mark.parametrize("K,N,G", [(2816, 128, 1), (256, 256, 16)])
+def test_parts_have_the_same_bits_in_a_replayed_graph(K, N, G):
+    from unet_amd.adapters import adapter_linear
+    i = _inputs(200, K, N, 8, G, torch.float32)
+    a = {k: (v.detach() if torch.is_tensor(v) else v) for k, v in i.items()}
+    with torch.no_grad():
+        want = adapter_linear(a["x"], a["w"], a["b"], a["A"], a["B"], a["ids"], scales=a["sc"])
+        graph = torch.cuda.CUDAGraph()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            adapter_linear(a["x"], a["w"], a["b"], a["A"], a["B"], a["ids"], scales=a["sc"])
+        torch.cuda.current_stream().wait_stream(side)
+        with torch.cuda.graph(graph):
+            y = adapter_linear(a["x"], a["w"], a["b"], a["A"], a["B"], a["ids"], scales=a["sc"])
+        for _ in range(3):
+            y.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, want)
+            torch.randn(1 << 20, device="cuda").sum()
