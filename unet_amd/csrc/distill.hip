@@ -19,7 +19,6 @@
 // by what a row costs besides (five sums over the lanes, the pairs): rows of 4000 128 us, of 1000 190 us.
 #include "sx_common.h"
 #include <algorithm>
-#include <type_traits>
 
 namespace sx {
 
@@ -158,11 +157,6 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
     den = *a.den;
   }
   const unsigned my = tid * 16u;                        // bytes: with the block's own base in scalar registers, one offset for all vectors
-  auto vec_at = [](auto* base, unsigned off) {
-    typedef std::conditional_t<std::is_const_v<std::remove_pointer_t<decltype(base)>>, const Vec, Vec> V1;
-    typedef std::conditional_t<std::is_const_v<V1>, const char, char> C1;
-    return reinterpret_cast<V1*>(reinterpret_cast<C1*>(base) + off);
-  };
   // vector k of a row, from its descriptor: behind the last one the load is not made, with no branch around it (a branch would leave the
   // number of loads in flight open, and a wait for one would be a wait for all)
   auto row_desc = [](const T* z, int nh, int nb) { return __builtin_amdgcn_make_buffer_rsrc((void*)(z + nh), 0, nb * 16, 0x00020000); };
@@ -305,7 +299,7 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
         if (live)
 #pragma unroll
           for (int e = 0; e < E; ++e) o[e] = from_f32<T>(gs * __builtin_amdgcn_exp2f(fmaf(to_f32(r[k][e]), c, -mc)));
-        *vec_at(dz + nh + k * NT * E, my) = o;
+        *reinterpret_cast<Vec*>(reinterpret_cast<char*>(dz + nh + k * NT * E) + my) = o;
       }
       if (GRAD) r[k] = load_vec(dn, k);
       __builtin_amdgcn_sched_barrier(0);

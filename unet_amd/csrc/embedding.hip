@@ -10,7 +10,6 @@
 // TB/s) behind a sort of 15 and before a join of 5.4.  5003 tokens of 9973 x 331 fp32 (4-byte loads): 6, 16, 7.4 and 4 us.
 #include "sort_ids.h"
 #include <algorithm>
-#include <type_traits>
 
 namespace sx {
 
