@@ -544,8 +544,11 @@ extern "C" int sx_distill_forward(int dtype, int64_t N, int V, int K, const void
   a.weights = weights; a.den_host = mean ? fmaxf((float)N, 1e-8f) : 1.f; a.row_loss = row_loss;
   a.row_stats = row_stats; a.dz = dlogits; a.lddz = ldd;
   if (mean && weights) {
-    if (N > 0 && N <= 16384 && rows_fit(a, dtype)) {
-      a.den_out = den;                                  // few enough weights for every block to add up itself
+    // few enough weights for every block to add up itself, sixteen a thread: 8192 rows of 1000 with a wave each 40 us, with a launch for
+    // the sum 17
+    const int64_t few = V <= 1024 * (16 / (int)dtype_size(dtype)) ? 1024 : V <= 8192 * (16 / (int)dtype_size(dtype)) ? 4096 : 16384;
+    if (N > 0 && N <= few && rows_fit(a, dtype)) {
+      a.den_out = den;
     } else {
       hipLaunchKernelGGL(distill_den_kernel, dim3(1), dim3(1024), 0, st, weights, N, den);
       SX_LAUNCH_CHECK("distill_den");
