@@ -378,3 +378,18 @@ def test_loss_without_a_gradient(V):
     assert bool(((alone.double() - want).abs() <= tol + U * want.abs()).all())
     total = distillation_loss(z, top, idx, reduction="sum")
     assert abs(float(total.detach()) - float(want.sum())) <= float(tol.sum() + N * U * want.abs().sum())
+
+
+@pytest.mark.parametrize("N", [1, 3, 4097, 20001, 300007])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_sums_over_many_rows(N, shift):
+    """The mean's two sums, from 16-byte boundaries and off them: the same as of the rows' losses and of the weights."""
+    from unet_amd.losses import distillation_loss
+    z, top, idx = _inputs((N,), 9, 2, seed=N)
+    w = torch.rand(N + shift, generator=torch.Generator().manual_seed(N)).cuda()[shift:]
+    rows = distillation_loss(z.detach(), top, idx, weights=w, reduction="none").double()
+    for red, want in (("mean", rows.sum() / w.double().sum()), ("sum", rows.sum())):
+        got = distillation_loss(z.detach(), top, idx, weights=w, reduction=red)
+        # a thread adds n / 4096 terms, ten joins and a division behind them, in either sum; all terms are positive
+        assert abs(float(got) - float(want)) <= 2 * (N / 4096 + 16) * U * float(want)
+        assert torch.equal(got, distillation_loss(z.detach(), top, idx, weights=w, reduction=red))
