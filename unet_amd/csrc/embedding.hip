@@ -124,8 +124,9 @@ struct RowSum {
 };
 
 // Blocks [0, gridDim.x - run_blocks) take the rows of the table, ROWS per group; the others take the runs of long rows.  Where most rows have
-// no token or one the loads of four rows are what keeps memory busy; where they have many, four after another take four times as long
-// (65000 tokens, 1000 rows of 500 bf16: 47 us by four, 20 by one)
+// no token or one the loads of four rows are what keeps memory busy; where they have several, four after another take longer.  Row length 1024
+// in bf16, 16384 tokens evenly and unevenly spread, by four and by one: 32768 rows 19 and 22 us, 16384 rows 16.0 and 15.7, 4000 rows 12.8 and
+// 9.1, uneven 17 and 12; 65000 tokens of 1000 rows of 500, 47 and 20
 template <typename T, int E, int GROUP, int NC, int ROWS>
 __global__ __launch_bounds__(256) void embed_bwd_kernel(EmbedBwdArgs q) {
   typedef RowSum<T, E, GROUP, NC> Sum;
@@ -260,7 +261,7 @@ static int embed_bwd_launch(EmbedBwdArgs q, hipStream_t st) {
   q.run = embed_run(q.n, GROUP);
   const int64_t runs = q.n > q.run ? cdiv64(q.n, q.run) : 0;
   q.run_blocks = cdiv64(runs, per);
-  const int by = q.n > 2 * q.rows ? 1 : 4;
+  const int by = q.n >= q.rows ? 1 : 4;
   const dim3 grid((unsigned)(cdiv64(q.rows, per * by) + q.run_blocks));
   if (by == 1) hipLaunchKernelGGL((embed_bwd_kernel<T, E, GROUP, NC, 1>), grid, dim3(256), 0, st, q);
   else hipLaunchKernelGGL((embed_bwd_kernel<T, E, GROUP, NC, 4>), grid, dim3(256), 0, st, q);
