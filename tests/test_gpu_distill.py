@@ -393,3 +393,51 @@ def test_sums_over_many_rows(N, shift):
         # a thread adds n / 4096 terms, ten joins and a division behind them, in either sum; all terms are positive
         assert abs(float(got) - float(want)) <= 2 * (N / 4096 + 16) * U * float(want)
         assert torch.equal(got, distillation_loss(z.detach(), top, idx, weights=w, reduction=red))
+
+
+FILLS = [-1e4, -1e9, -1e10, -1e12, -1e20, -1e29, -1e30, -3e38]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V,K", [(257, 6), (500, 9), (2001, 70), (500, 300), (9001, 300)])
+@pytest.mark.parametrize("fill", FILLS)
+def test_masked_vocabulary_of_any_fill(fill, V, K, dtype):
+    """Logits masked by a large negative number, at the head, at the tail, scattered, and all but one, so that threads meet only such
+    numbers, first, last or throughout; rows of a length that leaves loose elements; rows in registers and rows read twice (K = 300).  A
+    thread's maximum is then the fill, and the product with log2 e / tau has a rounding error of many powers of 2."""
+    for tau in (0.5, 1.0, 2.0, 1e-5):
+        z, top, idx = _inputs((5,), V, K, dtype)
+        live = torch.zeros(5, V, dtype=torch.bool)
+        live[0, V // 2:] = True
+        live[1, :V // 3] = True
+        live[2, torch.randperm(V, generator=torch.Generator().manual_seed(V))[:V // 10]] = True
+        live[3, V - 1] = True
+        live[4] = True
+        with torch.no_grad():
+            z[~live.cuda()] = fill
+            for r in range(5):
+                at = live[r].nonzero().view(-1).cuda()
+                idx[r] = at[idx[r] % at.numel()]
+        _check(z, top, idx, tau)
+        _check(z, top, idx, tau, None, "none", torch.tensor([0.5, -1.0, 1.0, 2.0, 3.0]).cuda())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("K", [6, 300])
+def test_rows_of_one_far_value_and_teachers_on_masked_entries(K, dtype):
+    """Whole rows at a far value, whose softmax is flat, and a teacher whose mass lies on masked entries: a large loss, no NaN."""
+    for V in (257, 4003):
+        z, top, idx = _inputs((8,), V, K, dtype)
+        with torch.no_grad():
+            for r, v in enumerate((1e7, -1e7, 1e10, -1e10, 1e20, -1e20)):
+                z[r] = v
+            z[6, 1:] = -1e10
+            z[7, :V // 2] = -1e20
+            idx[6], idx[7] = 1 + idx[6] % (V - 1), idx[7] % (V // 2)
+        for tau in (0.5, 1.0, 1.5):
+            _check(z, top, idx, tau, None, "none")
+            _check(z, top, idx, tau)
+    z, top, idx = _inputs((3,), 700, K, dtype)
+    with torch.no_grad():
+        z.mul_(1000.0)                                    # logits in the thousands at a temperature near zero
+    _check(z, top, idx, 1e-6)

@@ -86,14 +86,18 @@ __device__ __forceinline__ float mul_rn(float a, float b) {
 }
 
 // exponent of 2 of a logit relative to the row's maximum.  z * c - m * c in one fma: m * c is rounded, but alike for all of the row (and
-// sums move from one maximum to another by the difference of the rounded products).
-// Beyond kFar (a row whose every logit is the type's lowest value) or kSharp (a temperature near zero) m * c could overflow: the difference
-// is taken first.
-constexpr float kFar = 1e30f, kSharp = 2e6f;
+// sums move from one maximum to another by the difference of the rounded products).  What the maximum itself gets is that rounding's residual,
+// up to half a last place of m * c, in the place of 0: it has to stay far below the 128 where exp2 leaves 32 bits on either side, or the sum is
+// infinite or 0 (a masked logit of -1e10 at c = log2 e: 440).  So the form holds for |m * c| < 2^28, a residual of 8 at most, and beyond, rows
+// of far values or temperatures near zero, the difference is taken first.
+constexpr float kReach = 268435456.f;
+// the largest logits that the fma form takes; a thread's maximum starts at minus that, so that a set without a logit above it joins the others
+// as the little that it is beside any row maximum in reach
+__device__ __forceinline__ float logit_reach(float c) { return fminf(1e30f, kReach / c); }
 struct Expo {
   float c, m, mc;
   bool far;
-  __device__ __forceinline__ Expo(float m_, float c_) : c(c_), m(m_), mc(mul_rn(m_, c_)), far(!(fabsf(m_) < kFar && c_ < kSharp)) {}
+  __device__ __forceinline__ Expo(float m_, float c_, float reach) : c(c_), m(m_), mc(mul_rn(m_, c_)), far(!(fabsf(m_) < reach)) {}
   __device__ __forceinline__ float at(float z) const { return far ? (z - m) * c : fmaf(z, c, -mc); }
 };
 
@@ -130,9 +134,6 @@ __device__ __forceinline__ void store_row_vec(T* __restrict__ d, int off, int V,
 template <typename T>
 __device__ __forceinline__ int row_off(const T* z) { return (int)(((uintptr_t)z & 15) / sizeof(T)); }
 
-// a thread's maximum never goes below this, so that a set without a live logit joins the others as a sum of 0
-constexpr float kFloor = -kFar;
-
 // Row = nh elements up to the first 16-byte boundary, nb whole vectors, the rest.  Vector v belongs to thread v % NT, register v / NT; the
 // elements before and behind the vectors to threads 0, 1, ... one each.  Pair k belongs to thread k; the gradient at its index is
 // stored once more, over the plain q of the row's other elements, behind the next barrier that the block meets anyway.
@@ -145,7 +146,7 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
   __shared__ float pair_p[PAIRS];
   __shared__ int pair_i[PAIRS];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  const float it = 1.f / a.tau, c = it * kLog2e;
+  const float it = 1.f / a.tau, c = it * kLog2e, reach = logit_reach(c);
   float den = a.den_host;
   if (a.den_out) {
     float s = 0.f;
@@ -215,7 +216,7 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
     shape(zn, nhn, nbn);
     if (!onn) nbn = 0;
     const auto dn = row_desc(zn, nhn, nbn);
-    float m = kFloor, s = 0.f;
+    float m = -reach, s = 0.f;
     if (on && has_loose) {
       m = fmaxf(m, zl);
       s = __builtin_amdgcn_exp2f(fmaf(zl, c, -mul_rn(m, c)));
@@ -252,7 +253,7 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
       TS = wave_sum(lane < NW && any1 != 0.f ? mul_rn(red[3][ww], expf((tm1 - TM) * it)) : 0.f);
     }
     const bool live = on && any != 0.f;
-    const bool far = live && !(fabsf(M) < kFar);        // no logit above the floor, or products that overflow: the row again, by differences
+    const bool far = live && !(fabsf(M) < reach);       // the row again, by differences
     if (far) {
       float mk = -INFINITY;
       for (int v = tid; v < a.V; v += NT) mk = fmaxf(mk, to_f32(z[v]));
@@ -268,7 +269,7 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
       if (live && paired) {
         const float lt = (pt - TM) * it;
         p = expf(lt) / TS;
-        const Expo x(M, c);
+        const Expo x(M, c, reach);
         if (!(p == 0.f)) kl = p * ((lt - logf(TS)) - (x.at(zp) * kLn2 - logf(S)));
       }
       pair_i[tid] = pi;
@@ -285,7 +286,7 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
       if (a.row_stats) keep_stats(a, row, M, S, TM, TS);
     }
     if (GRAD && live && wid * 64 < a.K) {                 // the gradient at the pairs' indices, in the order of the pairs
-      const Expo x(M, c);
+      const Expo x(M, c, reach);
       fix = gs * __builtin_amdgcn_exp2f(x.at(zp));
       for (int j = 0; j < a.K; ++j) fix = pair_i[j] == pi ? fmaf(-gc, pair_p[j], fix) : fix;
       if (paired) fix_at = dz + pi;
@@ -323,7 +324,7 @@ __global__ __launch_bounds__(NT) void distill_wide_kernel(DistillArgs a) {
   __shared__ int64_t pair_i[NT];
   __shared__ float pair_p[NT];
   const int tid = threadIdx.x;
-  const float it = 1.f / a.tau, c = it * kLog2e;
+  const float it = 1.f / a.tau, c = it * kLog2e, reach = logit_reach(c);
   if (GRAD_ONLY && a.ready && a.g_stride == 0 && *a.g == 1.f) return;      // dz still holds the forward pass's gradient, which is this one
   for (int64_t row = blockIdx.x; row < a.N; row += gridDim.x) {
     const T* z = (const T*)a.z + row * a.ldz;
@@ -362,7 +363,7 @@ __global__ __launch_bounds__(NT) void distill_wide_kernel(DistillArgs a) {
     }
     const bool live = w != 0.f && !(ts == 0.f);
     if (!GRAD_ONLY && live) {
-      float mk = kFloor;                                  // as in rows_kernel: a thread rescales its sum when its maximum grows
+      float mk = -reach;                                  // as in rows_kernel: a thread rescales its sum when its maximum grows
 #pragma unroll 4
       for (int v = tid; v < nv; v += NT) {
         const Vec r = load_row_vec<T>(z, off, a.V, v);
@@ -377,17 +378,17 @@ __global__ __launch_bounds__(NT) void distill_wide_kernel(DistillArgs a) {
       }
       m = all_max<NT>(mk, red);
       s = mul_rn(s, __builtin_amdgcn_exp2f(mul_rn(mk, c) - mul_rn(m, c)));
-      if (!(fabsf(m) < kFar && c < kSharp)) {     // products that overflow: the row again, by differences
+      if (!(fabsf(m) < reach)) {                          // the row again, by differences
         mk = -INFINITY;
         for (int v = tid; v < a.V; v += NT) mk = fmaxf(mk, to_f32(z[v]));
         m = all_max<NT>(mk, red);
-        const Expo x(m, c);
+        const Expo x(m, c, reach);
         s = 0.f;
         for (int v = tid; v < a.V; v += NT) s += __builtin_amdgcn_exp2f(x.at(to_f32(z[v])));
       }
       s = all_sum<NT>(s, red);
     }
-    const Expo x(m, c);
+    const Expo x(m, c, reach);
     if constexpr (!GRAD_ONLY) {
       const float ls = logf(s), lts = logf(ts);
       float kl = 0.f;
