@@ -1,0 +1,61 @@
+"""GPU: the embedding, the adapters and the distillation loss under what torch puts around calls: forward mode, tracing, function
+transforms, second derivatives.  What an operator has no rule for is refused, never answered wrongly."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+pytestmark = pytest.mark.gpu
+
+
+def _calls():
+    """name -> (function of its differentiable inputs alone, those inputs)"""
+    from unet_amd import adapter_linear, distillation_loss, scaled_embedding
+    g = torch.Generator().manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g).cuda()
+    ids = torch.randint(-1, 6, (11,), generator=g).cuda()
+    w, b, A, B, who = r(9, 8), r(9), r(3, 2, 8), r(3, 9, 2), torch.randint(-1, 3, (11,), generator=g).cuda()
+    top, idx = r(11, 4), torch.randint(0, 30, (11, 4), generator=g).cuda()
+    return {
+        "scaled_embedding": (lambda t: scaled_embedding(ids, t, 2.0), (r(6, 5),)),
+        "adapter_linear": (lambda x, a, c: adapter_linear(x, w, b, a, c, who), (r(11, 8), A, B)),
+        "adapter_linear, many rows": (lambda x, a, c: adapter_linear(x, w, b, a, c, who.repeat(9)), (r(99, 8), A, B)),
+        "distillation_loss": (lambda z: distillation_loss(z, top, idx), (r(11, 30),)),
+        "distillation_loss, per row": (lambda z: distillation_loss(z, top, idx, weights=torch.ones(11, device="cuda"), reduction="none"), (r(11, 30),)),
+    }
+
+
+NAMES = ["scaled_embedding", "adapter_linear", "adapter_linear, many rows", "distillation_loss", "distillation_loss, per row"]
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_forward_mode_is_refused_not_dropped(name):
+    fn, args = _calls()[name]
+    for at in range(len(args)):
+        with forward_ad.dual_level():
+            dual = [forward_ad.make_dual(a, torch.ones_like(a)) if i == at else a for i, a in enumerate(args)]
+            with pytest.raises((RuntimeError, NotImplementedError), match="jvp"):
+                fn(*dual)
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            torch.func.jvp(fn, args, tuple(torch.ones_like(a) for a in args))
+    with forward_ad.dual_level():
+        a = fn(*args)                                     # no tangent anywhere: the value
+    assert torch.equal(a, fn(*args))
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_a_trace_computes(name):
+    """Traced without gradients, replayed on other inputs."""
+    fn, args = _calls()[name]
+    with torch.no_grad():
+        traced = torch.jit.trace(fn, args, check_trace=False)
+        for k in (1.0, -0.5, 3.0):
+            other = tuple(a * k for a in args)
+            torch.full((1 << 16,), float("nan"), device="cuda")      # what a reused allocation may hold
+            assert torch.equal(traced(*other), fn(*other))
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_batched_transforms_are_refused(name):
+    fn, args = _calls()[name]
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(fn)(*(a.unsqueeze(0).repeat(2, *([1] * a.dim())) for a in args))

@@ -117,3 +117,25 @@ def test_temperatures_and_sizes_out_of_reach_are_refused():
         a = dict(V=10, K=2, tau=1.0)
         a.update(kw)
         assert lib.sx_distill_forward(0, 3, a["V"], a["K"], P, 1 << 31, 0, P, P, 1, a["tau"], None, 1, P, None, P, None, None, 10, None) < 0
+
+
+def test_what_looks_into_calls_is_seen():
+    """A direct call of the kernels would drop a tangent and leave nothing in a trace: forward mode, traces and function transforms are noticed."""
+    from torch.autograd import forward_ad
+    from unet_amd import _lib as L
+    t, p, seen = torch.ones(3), torch.ones(3, requires_grad=True), []
+
+    def f(x):
+        seen.append(L.by_autograd(x))
+        return x * 2
+    f(t)
+    f(p)
+    with torch.no_grad():
+        f(p)
+        torch.jit.trace(f, (t,), check_trace=False)
+    with forward_ad.dual_level():
+        f(t)
+    torch.func.vmap(f)(t)
+    torch.func.jvp(f, (t,), (t,))
+    f(t)
+    assert seen == [False, True, False, True, True, True, True, False]

@@ -11,6 +11,7 @@ import functools
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsolpex_hip.so")
@@ -236,6 +237,14 @@ def once(who):
 
 def wants_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def by_autograd(*tensors):
+    """Whether a call has to go through its autograd Function: one of its inputs wants a gradient, or something is at work that only sees
+    what passes through one -- forward mode (a Function without a jvp refuses a tangent, a plain call would drop it), a trace (a plain
+    call leaves nothing but the allocation of its output in it), a function transform."""
+    return (wants_grad(*tensors) or forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None
+            or torch._C._are_functorch_transforms_active())
 
 
 def ptr_table(tensors):

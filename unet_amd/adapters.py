@@ -38,7 +38,7 @@ def _project(x, weight, bias, A, B, ids, scales, keep):
 class _AdapterFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, A, B, ids, scales):
-        y, kept = _project(x, weight, bias, A, B, ids, scales, True)
+        y, kept = _project(x, weight, bias, A, B, ids, scales, any(ctx.needs_input_grad))
         ctx.save_for_backward(x, weight, A, B, scales, kept)
         return y
 
@@ -107,7 +107,7 @@ def adapter_linear(x, weight, bias, A, B, ids, *, scales=None):
     if ids.dim() < len(lead):
         ids = ids.reshape(tuple(ids.shape) + (1,) * (len(lead) - ids.dim())).expand(lead)
     args = (x, weight, None if bias is None else L.packed(bias), A, B, L.packed(ids), None if scales is None else L.plain_f32(scales))
-    return _AdapterFn.apply(*args) if L.wants_grad(x, A, B) else _project(*args, False)[0]
+    return _AdapterFn.apply(*args) if L.by_autograd(x, A, B) else _project(*args, False)[0]
 
 
 class AdapterLinear(nn.Module):

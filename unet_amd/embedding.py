@@ -58,7 +58,7 @@ def scaled_embedding(ids, table, scale=1.0):
         raise ValueError(f"{who}: ids are on {ids.device}, the table on {table.device}")
     L.ids_flag(ids, who)
     L.dtype_code(table, who)
-    return _EmbeddingFn.apply(ids, table, float(scale)) if L.wants_grad(table) else _lookup(ids, table, float(scale))[1]
+    return _EmbeddingFn.apply(ids, table, float(scale)) if L.by_autograd(table) else _lookup(ids, table, float(scale))[1]
 
 
 class ScaledEmbedding(nn.Module):

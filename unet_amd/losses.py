@@ -175,7 +175,7 @@ def _distill(logits, top, idx, weights, tau, reduction, need):
 class _DistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, top, idx, weights, tau, reduction):
-        loss, keep, ctx.d = _distill(logits, top, idx, weights, tau, reduction, True)
+        loss, keep, ctx.d = _distill(logits, top, idx, weights, tau, reduction, ctx.needs_input_grad[0])
         ctx.save_for_backward(logits, top, idx, weights, keep)
         ctx.meta = (tau, reduction)
         return loss
@@ -230,7 +230,7 @@ def distillation_loss(logits, top_logits, top_idx, *, temperature=1.0, weights=N
             raise ValueError(f"{who}: weights must be {lead}, got {tuple(weights.shape)}")
         weights = L.plain_f32(weights if weights.device == logits.device else weights.to(logits.device))
     top, idx = L.packed(top_logits.detach() if top_logits.requires_grad else top_logits), L.packed(top_idx)
-    if L.wants_grad(logits):
+    if L.by_autograd(logits):
         return _DistillFn.apply(logits, top, idx, weights, tau, reduction)
     return _distill(logits, top, idx, weights, tau, reduction, False)[0]
 
