@@ -1,4 +1,4 @@
-"""GPU: the embedding, the adapters and the distillation loss under what torch puts around calls: forward mode, tracing, function
+"""GPU: the embedding, the adapters, the distillation loss and the latent MLPs under what torch puts around calls: forward mode, tracing, function
 transforms, second derivatives.  What an operator has no rule for is refused, never answered wrongly."""
 import pytest
 import torch
@@ -10,21 +10,27 @@ pytestmark = pytest.mark.gpu
 def _calls():
     """name -> (function of its differentiable inputs alone, those inputs)"""
     from unet_amd import adapter_linear, distillation_loss, scaled_embedding
+    from unet_amd.latent import ParamToZ
     g = torch.Generator().manual_seed(1)
     r = lambda *s: torch.randn(*s, generator=g).cuda()
     ids = torch.randint(-1, 6, (11,), generator=g).cuda()
     w, b, A, B, who = r(9, 8), r(9), r(3, 2, 8), r(3, 9, 2), torch.randint(-1, 3, (11,), generator=g).cuda()
     top, idx = r(11, 4), torch.randint(0, 30, (11, 4), generator=g).cuda()
+    torch.manual_seed(2)
+    mlp = ParamToZ(4, 6, hidden=(16, 8)).cuda().eval()
+    for p in mlp.parameters():
+        p.requires_grad_(False)
     return {
         "scaled_embedding": (lambda t: scaled_embedding(ids, t, 2.0), (r(6, 5),)),
         "adapter_linear": (lambda x, a, c: adapter_linear(x, w, b, a, c, who), (r(11, 8), A, B)),
         "adapter_linear, many rows": (lambda x, a, c: adapter_linear(x, w, b, a, c, who.repeat(9)), (r(99, 8), A, B)),
         "distillation_loss": (lambda z: distillation_loss(z, top, idx), (r(11, 30),)),
         "distillation_loss, per row": (lambda z: distillation_loss(z, top, idx, weights=torch.ones(11, device="cuda"), reduction="none"), (r(11, 30),)),
+        "latent MLP": (mlp, (r(11, 4),)),
     }
 
 
-NAMES = ["scaled_embedding", "adapter_linear", "adapter_linear, many rows", "distillation_loss", "distillation_loss, per row"]
+NAMES = ["scaled_embedding", "adapter_linear", "adapter_linear, many rows", "distillation_loss", "distillation_loss, per row", "latent MLP"]
 
 
 @pytest.mark.parametrize("name", NAMES)

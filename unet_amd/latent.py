@@ -140,8 +140,7 @@ class _MLP(nn.Module):
     def forward(self, x):
         lead = x.shape[:-1]
         x2 = x.reshape(-1, x.shape[-1])
-        needs = torch.is_grad_enabled() and (x2.requires_grad or any(p.requires_grad for p in self.parameters()))
-        if needs:
+        if L.by_autograd(x2, *self.parameters()):
             out = _MLPFn.apply(self, x2, *self.parameters())
         else:
             out = self.hip_forward(x2, train=self.training).out
