@@ -65,3 +65,48 @@ def test_batched_transforms_are_refused(name):
     fn, args = _calls()[name]
     with pytest.raises(RuntimeError):
         torch.func.vmap(fn)(*(a.unsqueeze(0).repeat(2, *([1] * a.dim())) for a in args))
+@pytest.mark.parametrize("name", NAMES[:5])
+def test_second_derivatives_are_refused_where_they_are_taken(name):
+    """Under create_graph the first derivatives are what they are without it, beside a penalty on other gradients of the same graph; differentiating
+    them raises."""
+    fn, args = _calls()[name]
+    for wanted in range(len(args)):                       # one input at a time, then its gradients with all of them
+        leaves = [a.clone().requires_grad_(i == wanted or wanted == 0) for i, a in enumerate(args)]
+        live = [t for t in leaves if t.requires_grad]
+        plain = torch.autograd.grad(fn(*leaves).square().sum(), live)
+        grads = torch.autograd.grad(fn(*leaves).square().sum(), live, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(plain, grads))
+        for g in grads:
+            assert g.requires_grad
+            with pytest.raises(RuntimeError, match="not differentiable twice"):
+                torch.autograd.grad(g.sum(), live, retain_graph=True, allow_unused=True)
+    # a gradient penalty elsewhere in the graph
+    u = torch.randn(5, device="cuda", requires_grad=True)
+    leaves = [a.clone().requires_grad_(True) for a in args]
+    total = fn(*leaves).sum() + (u ** 3).sum()
+    gu, *rest = torch.autograd.grad(total, (u, *leaves), create_graph=True)
+    (gu.square().sum() + total).backward()
+    # 9 u^4 and u^3, each product and sum rounded
+    want = 36 * u.detach() ** 3 + 3 * u.detach() ** 2
+    assert bool(((u.grad - want).abs() <= 1e-5 * (36 * u.detach().abs() ** 3 + 3 * u.detach() ** 2)).all())
+    for leaf, g in zip(leaves, rest):
+        assert torch.equal(leaf.grad, g.detach())
+
+
+def test_a_first_derivative_of_the_distillation_depends_on_its_logits():
+    """The upstream gradient of a plain .backward(create_graph=True) needs no gradient itself, the result does: a penalty on it must not lose its
+    term in silence."""
+    from unet_amd import distillation_loss
+    z = torch.randn(3, 20, device="cuda", requires_grad=True)
+    top, idx = torch.randn(3, 2, device="cuda"), torch.zeros(3, 2, dtype=torch.int64, device="cuda")
+    (g,) = torch.autograd.grad(distillation_loss(z, top, idx), (z,), create_graph=True)
+    with pytest.raises(RuntimeError, match="not differentiable twice"):
+        (distillation_loss(z, top, idx) + g.square().sum()).backward()
+
+
+def test_gradients_that_depend_on_nothing_are_constants():
+    """The table's gradient is linear in the upstream one alone: with a constant one there is nothing to differentiate."""
+    from unet_amd import scaled_embedding
+    t = torch.randn(4, 3, device="cuda", requires_grad=True)
+    (g,) = torch.autograd.grad(scaled_embedding(torch.tensor([0, 2, 2], device="cuda"), t).sum(), (t,), create_graph=True)
+    assert not g.requires_grad and torch.equal(g[2], torch.full((3,), 2.0, device="cuda"))

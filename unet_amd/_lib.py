@@ -229,10 +229,24 @@ def size_of(name, *args):
     return check(getattr(_lib or lib(), name)(*args), name)
 
 
-def once(who):
-    """For the top of a backward pass that has no derivative of its own (cheaper than a decorator's context manager)."""
-    if torch.is_grad_enabled():
-        raise RuntimeError(f"{who}: not differentiable twice (create_graph=True)")
+class _NotTwice(torch.autograd.Function):
+    """A gradient as it is, with a derivative that raises."""
+    @staticmethod
+    def forward(ctx, who, grad, *sources):
+        ctx.who = who
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, g):
+        raise RuntimeError(f"{ctx.who}: not differentiable twice (create_graph=True)")
+
+
+def not_twice(who, grad, *sources):
+    """`grad`, which a kernel computed from `sources`: where one of them wants a gradient (a backward pass under create_graph), the first
+    derivative is had as ever, and only differentiating it raises."""
+    if grad is None or not wants_grad(*sources):
+        return grad
+    return _NotTwice.apply(who, grad, *sources)
 
 
 def wants_grad(*tensors):

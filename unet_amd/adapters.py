@@ -44,8 +44,12 @@ class _AdapterFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        L.once("adapter_linear")
         x, weight, A, B, scales, kept = ctx.saved_tensors
+        if torch.is_grad_enabled():
+            who = "adapter_linear"
+            with torch.no_grad():
+                dx, _, _, dA, dB, _, _ = _AdapterFn.backward(ctx, dy)
+            return (L.not_twice(who, dx, dy, A, B), None, None, L.not_twice(who, dA, dy, x, B), L.not_twice(who, dB, dy, x, A), None, None)
         need_x, _, _, need_a, need_b = ctx.needs_input_grad[:5]
         N, K = weight.shape
         G, r = A.shape[:2]

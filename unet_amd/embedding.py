@@ -30,7 +30,10 @@ class _EmbeddingFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout):
-        L.once("scaled_embedding")
+        if torch.is_grad_enabled():
+            with torch.no_grad():
+                grads = _EmbeddingFn.backward(ctx, dout)
+            return None, L.not_twice("scaled_embedding", grads[1], dout), None
         (i,) = ctx.saved_tensors
         V, D, scale, dtype = ctx.meta
         n, dev = i.numel(), dout.device

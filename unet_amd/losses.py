@@ -185,8 +185,11 @@ class _DistillFn(torch.autograd.Function):
         """Where the forward pass left the gradient for an upstream gradient of 1, that is it; for another one the gradient is computed
         again from the logits (one rounding), not scaled after its own."""
         who = "distillation_loss"
-        L.once(who)
         logits, top, idx, weights, keep = ctx.saved_tensors
+        if torch.is_grad_enabled():
+            with torch.no_grad():
+                grads = _DistillFn.backward(ctx, g)
+            return (L.not_twice(who, grads[0], g, logits), *grads[1:])
         tau, reduction = ctx.meta
         V, K = logits.shape[-1], top.shape[-1]
         d, ctx.d = ctx.d, None                     # the buffer is the caller's now: a second backward pass fills one of its own
