@@ -441,3 +441,33 @@ def test_rows_of_one_far_value_and_teachers_on_masked_entries(K, dtype):
     with torch.no_grad():
         z.mul_(1000.0)                                    # logits in the thousands at a temperature near zero
     _check(z, top, idx, 1e-6)
+
+
+def test_saved_tensor_hooks_see_the_gradient_buffer():
+    """The N x V gradient that the forward pass leaves is saved where hooks see it (offloading), a recomputed forward pass (checkpoint) works, and
+    a gradient that was changed in place does not keep a second backward pass from its own."""
+    from torch.utils.checkpoint import checkpoint
+    from unet_amd.losses import distillation_loss
+    for dtype in (torch.float32, torch.bfloat16):
+        z, top, idx = _inputs((6,), 777, 9, dtype)
+        (want,) = torch.autograd.grad(distillation_loss(z, top, idx), (z,))
+        big = []
+
+        def pack(t):
+            big.append(t.shape == z.shape and t.data_ptr() != z.data_ptr())
+            return t.cpu()
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t.cuda()):
+            loss = distillation_loss(z, top, idx)
+        assert sum(big) == 1
+        (a,) = torch.autograd.grad(loss, (z,), retain_graph=True)
+        assert torch.equal(a, want)
+        (b,) = torch.autograd.grad(loss, (z,), torch.tensor(2.0, device="cuda"))
+        assert bool(((b.float() - 2 * want.float()).abs() <= 2.02 * HALF[dtype] * 2 * want.float().abs() + 1e-9).all())
+        loss = checkpoint(lambda t: distillation_loss(t, top, idx), z, use_reentrant=False)
+        assert torch.equal(torch.autograd.grad(loss, (z,))[0], want)
+        loss = distillation_loss(z, top, idx)
+        (a,) = torch.autograd.grad(loss, (z,), retain_graph=True)
+        assert torch.equal(a, want)
+        a.zero_()
+        (b,) = torch.autograd.grad(loss, (z,))
+        assert not a.any() and bool(((b.float() - want.float()).abs() <= 2.02 * HALF[dtype] * want.float().abs() + 1e-9).all())

@@ -175,9 +175,10 @@ def _distill(logits, top, idx, weights, tau, reduction, need):
 class _DistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, top, idx, weights, tau, reduction):
-        loss, keep, ctx.d = _distill(logits, top, idx, weights, tau, reduction, ctx.needs_input_grad[0])
-        ctx.save_for_backward(logits, top, idx, weights, keep)
+        loss, keep, d = _distill(logits, top, idx, weights, tau, reduction, ctx.needs_input_grad[0])
+        ctx.save_for_backward(logits, top, idx, weights, keep, d)
         ctx.meta = (tau, reduction)
+        ctx.fresh = d is not None
         return loss
 
     @staticmethod
@@ -185,17 +186,17 @@ class _DistillFn(torch.autograd.Function):
         """Where the forward pass left the gradient for an upstream gradient of 1, that is it; for another one the gradient is computed
         again from the logits (one rounding), not scaled after its own."""
         who = "distillation_loss"
-        logits, top, idx, weights, keep = ctx.saved_tensors
+        logits, top, idx, weights, keep, d = ctx.saved_tensors
         if torch.is_grad_enabled():
             with torch.no_grad():
                 grads = _DistillFn.backward(ctx, g)
             return (L.not_twice(who, grads[0], g, logits), *grads[1:])
         tau, reduction = ctx.meta
         V, K = logits.shape[-1], top.shape[-1]
-        d, ctx.d = ctx.d, None                     # the buffer is the caller's now: a second backward pass fills one of its own
-        ready = d is not None
-        if not ready:
-            d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        # the buffer is the caller's from here on, who may change it: a second backward pass fills one of its own (and does not mind the
+        # change: what goes out counts its versions for itself)
+        ready, ctx.fresh = ctx.fresh, False
+        d = d.data if ready else torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         z, ld = L.rows_2d(logits, V)
         g = L.plain_f32(g)
         L.launch("sx_distill_backward", logits.device, L.dtype_code(logits, who), z.shape[0], V, K, L.addr(z), ld, L.dtype_code(top, who), L.addr(top),
