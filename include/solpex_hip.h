@@ -52,6 +52,8 @@ typedef enum sx_conv_mode {
 
 int sx_version(void);
 const char* sx_last_error(void);
+/* 0 while `stream` is not capturing, else a positive number of its own for each capture; negative: the runtime would not say */
+int64_t sx_stream_capture_id(void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Weight packing.  Replaces nothing in the reference (ATen consumes (Cout,Cin,kh,kw) directly);

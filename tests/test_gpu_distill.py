@@ -471,3 +471,61 @@ def test_saved_tensor_hooks_see_the_gradient_buffer():
         a.zero_()
         (b,) = torch.autograd.grad(loss, (z,))
         assert not a.any() and bool(((b.float() - want.float()).abs() <= 2.02 * HALF[dtype] * want.float().abs() + 1e-9).all())
+
+
+def test_a_captured_backward_pass_takes_every_factor():
+    """The gradient pass alone in a graph, of a loss that was computed before on the stream of the capture (an autograd node runs on its
+    forward pass's stream): replays with other upstream gradients, and after the gradient of the replay before was changed in place."""
+    from unet_amd.losses import distillation_loss
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        z, top, idx = _inputs((20,), 901, 7)
+        g = torch.ones((), device="cuda")
+        want = torch.autograd.grad(distillation_loss(z, top, idx), (z,))[0].clone()
+        loss = distillation_loss(z, top, idx)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            (grad,) = torch.autograd.grad(loss, (z,), g, retain_graph=True)
+        for f in (1.0, 2.0, 1.0, 0.0, 1.0):
+            g.fill_(f)
+            graph.replay()
+            torch.cuda.synchronize()
+            # both round gs * exp2(.) and, at the teacher's indices, gs * exp2(.) - gc * p: a factor of 1, 2 or 0 scales every term exactly
+            assert bool(((grad - f * want).abs() <= 8 * U * (f * want).abs() + 1e-9).all()), f
+            grad.zero_()
+
+
+def test_forward_and_backward_captured_in_graphs_of_their_own():
+    from unet_amd import _lib as L
+    from unet_amd.losses import distillation_loss
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        z, top, idx = _inputs((20,), 901, 7)
+        g = torch.ones((), device="cuda")
+        torch.autograd.grad(distillation_loss(z, top, idx), (z,), g)      # (first launches outside of a capture)
+        one, two, both = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        ids = [L.capture_id(z.device)]
+        with torch.cuda.graph(one, stream=side):
+            ids.append(L.capture_id(z.device))
+            loss = distillation_loss(z, top, idx)
+        with torch.cuda.graph(two, stream=side):
+            ids.append(L.capture_id(z.device))
+            (grad,) = torch.autograd.grad(loss, (z,), g)
+        with torch.cuda.graph(both, stream=side):
+            ids.append(L.capture_id(z.device))
+            (grad2,) = torch.autograd.grad(distillation_loss(z, top, idx), (z,), g)
+            assert L.capture_id(z.device) == ids[3]
+        assert ids[0] == 0 == L.capture_id(z.device) and len(set(ids)) == 4 and min(ids) == 0
+        for seed in range(3):
+            with torch.no_grad():
+                z.copy_(_inputs((20,), 901, 7, seed=seed + 3)[0])
+            for f in (1.0, 3.0, 1.0):
+                g.fill_(f)
+                want = torch.autograd.grad(distillation_loss(z, top, idx), (z,), g)[0]
+                if f == 1.0:
+                    one.replay()
+                two.replay()
+                both.replay()
+                torch.cuda.synchronize()
+                assert bool(((grad - want).abs() <= 8 * U * want.abs() + 1e-9).all()) and torch.equal(grad2, want), (seed, f)
+                grad.zero_()

@@ -49,6 +49,7 @@ _D = C.POINTER(UNetDesc)
 SIGNATURES = {
     "sx_version": (_i, []),
     "sx_last_error": (C.c_char_p, []),
+    "sx_stream_capture_id": (_l, [_p]),
     "sx_packed_weight_elems": (_l, [_i, _i, _i, _i]),
     "sx_set_fp32_exact": (_i, [_i]),
     "sx_set_fp32_planes": (_i, [_i]),
@@ -221,6 +222,11 @@ def launch(name, device, *args):
         with torch.cuda.device(i):
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     return rc if rc >= 0 else check(rc, name)
+
+
+def capture_id(device):
+    """0 where the current stream of `device` is not capturing, else the number of the capture."""
+    return (_lib or lib()).sx_stream_capture_id(torch._C._cuda_getCurrentRawStream(device.index))
 
 
 @functools.lru_cache(maxsize=1024)

@@ -68,5 +68,15 @@ extern "C" int sx_set_fp32_exact(int on) {
   if (on >= 0) sx::g_fp32_planes.store(on ? 0 : 2, std::memory_order_relaxed);      // on < 0: query only
   return was;
 }
+extern "C" int64_t sx_stream_capture_id(void* stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  const hipError_t e = hipStreamGetCaptureInfo((hipStream_t)stream, &status, &id);
+  if (e != hipSuccess) {
+    (void)hipGetLastError();                     // not for the next launch's check to find
+    return sx::hip_fail(e, "hipStreamGetCaptureInfo");
+  }
+  return status == hipStreamCaptureStatusNone ? 0 : (int64_t)(id + 1);
+}
 extern "C" int sx_version(void) { return SX_VERSION; }
 extern "C" const char* sx_last_error(void) { return sx::g_err; }

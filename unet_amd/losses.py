@@ -178,7 +178,7 @@ class _DistillFn(torch.autograd.Function):
         loss, keep, d = _distill(logits, top, idx, weights, tau, reduction, ctx.needs_input_grad[0])
         ctx.save_for_backward(logits, top, idx, weights, keep, d)
         ctx.meta = (tau, reduction)
-        ctx.fresh = d is not None
+        ctx.made = None if d is None else L.capture_id(d.device)
         return loss
 
     @staticmethod
@@ -193,9 +193,11 @@ class _DistillFn(torch.autograd.Function):
             return (L.not_twice(who, grads[0], g, logits), *grads[1:])
         tau, reduction = ctx.meta
         V, K = logits.shape[-1], top.shape[-1]
-        # the buffer is the caller's from here on, who may change it: a second backward pass fills one of its own (and does not mind the
-        # change: what goes out counts its versions for itself)
-        ready, ctx.fresh = ctx.fresh, False
+        # The buffer is the caller's from here on, who may change it: a second backward pass fills one of its own (and does not mind the
+        # change: what goes out counts its versions for itself).  So does one in a graph of its own: replayed without the forward pass, it
+        # would find what the replay before or the caller left.
+        made, ctx.made = ctx.made, None
+        ready = made is not None and made >= 0 and made == L.capture_id(logits.device)
         d = d.data if ready else torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         z, ld = L.rows_2d(logits, V)
         g = L.plain_f32(g)
