@@ -139,3 +139,19 @@ def test_what_looks_into_calls_is_seen():
     torch.func.jvp(f, (t,), (t,))
     f(t)
     assert seen == [False, True, False, True, True, True, True, False]
+
+
+def test_embedding_workspace_holds_the_runs_there_are():
+    """Two partial rows for each run of sorted ids, of which there are 1024 at most (4096 of rows that groups of 16 threads may take), however
+    many ids; beside them a place and a bucket per id and two numbers per row of the table."""
+    from unet_amd import _lib as L
+    lib = L.lib()
+    for n in (0, 16, 17, 1000, 65536, 70000, 1 << 24, (1 << 31) - 2048):
+        for rows, dim in ((50, 1), (50, 128), (50, 129), (1 << 24, 1024), (7, 5000)):
+            need, base, runs = lib.sx_embedding_workspace_bytes(n, rows, dim), 8 * n + 8 * (rows + 1), 4096 if dim <= 128 else 1024
+            assert base <= need <= base + runs * 8 * dim + 5 * 256, (n, rows, dim)
+            if n > 16:
+                used = 16
+                while used * runs < n:
+                    used *= 2
+                assert need >= base + (8 * dim * -(-n // used) if n > used else 0), (n, rows, dim)

@@ -22,6 +22,13 @@ static inline int embed_run(int64_t n, int group) {
   while ((int64_t)run * (group >= 64 ? 1024 : 4096) < n) run *= 2;
   return run;
 }
+// pieces of 16 bytes at most in a row that a group of 16 threads may take (embed_bwd_pick): longer ones have groups of 64 and more
+constexpr int kSmallPieces = 16;
+// runs, whatever the width of the loads: small groups, which a row of few pieces may have, have the most
+static inline int64_t embed_max_runs(int64_t n, int dim) {
+  const int run = embed_run(n, dim <= kSmallPieces * 8 ? 16 : 64);
+  return n > run ? cdiv64(n, run) : 0;
+}
 constexpr int64_t kMaxRows = 1 << 24;      // the gradient's grid gives every row of the table up to 128 threads of a 2^32 limit
 
 // E elements as one load or store
@@ -250,7 +257,7 @@ static EmbedWs embed_ws(int64_t n, int64_t rows, int dim) {
   w.key = o; o = align_up(o + (size_t)n * 4, 256);
   w.start = o; o = align_up(o + (size_t)(rows + 1) * 4, 256);
   w.end = o; o = align_up(o + (size_t)(rows + 1) * 4, 256);
-  w.part = o; o = align_up(o + (n > kMinRun ? (size_t)cdiv64(n, kMinRun) * 2 * (size_t)dim * 4 : 0), 256);
+  w.part = o; o = align_up(o + (size_t)embed_max_runs(n, dim) * 2 * (size_t)dim * 4, 256);
   w.total = o;
   return w;
 }
@@ -276,7 +283,7 @@ static int embed_bwd_launch(EmbedBwdArgs q, hipStream_t st) {
 template <typename T, int E>
 static int embed_bwd_pick(const EmbedBwdArgs& q, hipStream_t st) {
   const int pieces = q.dim / E;
-  if (pieces <= 16) return embed_bwd_launch<T, E, 16, 1>(q, st);
+  if (pieces <= kSmallPieces) return embed_bwd_launch<T, E, 16, 1>(q, st);
   if (pieces <= 64) return embed_bwd_launch<T, E, 64, 1>(q, st);
   if (pieces <= 128) return embed_bwd_launch<T, E, 128, 1>(q, st);
   return embed_bwd_launch<T, E, 128, 4>(q, st);
