@@ -110,3 +110,24 @@ def test_gradients_that_depend_on_nothing_are_constants():
     t = torch.randn(4, 3, device="cuda", requires_grad=True)
     (g,) = torch.autograd.grad(scaled_embedding(torch.tensor([0, 2, 2], device="cuda"), t).sum(), (t,), create_graph=True)
     assert not g.requires_grad and torch.equal(g[2], torch.full((3,), 2.0, device="cuda"))
+
+
+def test_sizes_beyond_a_c_int_are_refused():
+    """2^32 + 8 columns must not become 8 on their way into the library.  Views of one element: nothing of that size is allocated."""
+    from unet_amd import adapter_linear, distillation_loss, scaled_embedding
+    w = (1 << 32) + 8
+    one, zero = torch.ones(1, 1, device="cuda"), torch.zeros(1, 1, dtype=torch.int64, device="cuda")
+    before = torch.cuda.memory_allocated()
+    with pytest.raises(ValueError, match="too long"):
+        scaled_embedding(zero[0], one.expand(1, w))
+    with pytest.raises(ValueError, match="too large"):
+        adapter_linear(one.expand(1, w), one.expand(1, w), None, one[None].expand(1, 1, w), one[None], zero[0])
+    with pytest.raises(ValueError, match="too large"):
+        adapter_linear(one, one.expand(w, 1), None, one[None], one[None].expand(1, w, 1), zero[0])
+    with pytest.raises(ValueError, match="at most"):
+        adapter_linear(one, one, None, one[None].expand(w, 1, 1), one[None].expand(w, 1, 1), zero[0])
+    with pytest.raises(ValueError, match="too long"):
+        distillation_loss(one.expand(1, w), one, zero)
+    with pytest.raises(ValueError, match="too long"):
+        distillation_loss(one, one.expand(1, w), zero.expand(1, w))
+    assert torch.cuda.memory_allocated() == before

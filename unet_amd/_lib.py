@@ -28,6 +28,7 @@ SX_T_HEAD_BIAS_SUMS, SX_HEAD_BIAS_SLOTS = 9, 64
 SX_NORM_LOG, SX_NORM_LINEAR, SX_NORM_SYMLOG = 0, 1, 2
 SX_WGRAD_STATIC_BYTES = 32 << 20
 SX_GN_BWD_SUMS_READY = 4
+MAX_WIDTH = (1 << 31) - 1        # sizes that a C int carries: ctypes cuts larger numbers off without a word
 SX_ADAPTER_FORWARD, SX_ADAPTER_BACKWARD, SX_ADAPTER_ALONE = 0, 1, 2
 PX_KINDS = {"huber": 0, "l1": 1, "mse": 2}
 

@@ -13,7 +13,7 @@ from torch import nn
 
 from . import _lib as L
 
-MAX_RANK = 128
+MAX_RANK, MAX_ADAPTERS = 128, 65535
 
 
 def _project(x, weight, bias, A, B, ids, scales, keep):
@@ -91,8 +91,10 @@ def adapter_linear(x, weight, bias, A, B, ids, *, scales=None):
     if A.dim() != 3 or B.dim() != 3 or A.shape[2] != K or tuple(B.shape) != (A.shape[0], N, A.shape[1]):
         raise ValueError(f"{who}: A must be (G, r, {K}) and B (G, {N}, r), got {tuple(A.shape)} / {tuple(B.shape)}")
     G, r = A.shape[:2]
-    if not (1 <= r <= MAX_RANK and G >= 1):
-        raise ValueError(f"{who}: rank {r} must be 1..{MAX_RANK} and there must be an adapter, got {G}")
+    if not (1 <= r <= MAX_RANK and 1 <= G <= MAX_ADAPTERS):
+        raise ValueError(f"{who}: rank {r} must be 1..{MAX_RANK} and there must be an adapter, at most {MAX_ADAPTERS}, got {G}")
+    if max(N, K) > L.MAX_WIDTH:
+        raise ValueError(f"{who}: a projection of {K} to {N} is too large")
     if bias is not None and tuple(bias.shape) != (N,):
         raise ValueError(f"{who}: bias must be ({N},), got {tuple(bias.shape)}")
     if scales is not None and tuple(scales.shape) != (G,):

@@ -57,6 +57,8 @@ def scaled_embedding(ids, table, scale=1.0):
         raise RuntimeError(f"{who}: the HIP path needs CUDA (ROCm) tensors; this build has no CPU path")
     if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
         raise ValueError(f"{who}: table must be (rows, dim) with at least one of each, got {tuple(table.shape)}")
+    if table.shape[1] > L.MAX_WIDTH:
+        raise ValueError(f"{who}: rows of {table.shape[1]} are too long")
     if ids.device != table.device:
         raise ValueError(f"{who}: ids are on {ids.device}, the table on {table.device}")
     L.ids_flag(ids, who)

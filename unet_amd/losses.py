@@ -228,6 +228,8 @@ def distillation_loss(logits, top_logits, top_idx, *, temperature=1.0, weights=N
     lead = tuple(logits.shape[:-1])
     if top_logits.dim() < 1 or top_logits.shape[-1] < 1 or tuple(top_logits.shape) != tuple(top_idx.shape) or tuple(top_logits.shape[:-1]) != lead:
         raise ValueError(f"{who}: top_logits and top_idx must both be {lead + ('K',)}, got {tuple(top_logits.shape)} / {tuple(top_idx.shape)}")
+    if max(logits.shape[-1], top_logits.shape[-1]) > L.MAX_WIDTH:
+        raise ValueError(f"{who}: rows of {logits.shape[-1]} logits with {top_logits.shape[-1]} of the teacher's are too long")
     if top_logits.device != logits.device or top_idx.device != logits.device:
         raise ValueError(f"{who}: logits, top_logits and top_idx must be on one device")
     L.dtype_code(logits, who), L.dtype_code(top_logits, who), L.ids_flag(top_idx, who)
