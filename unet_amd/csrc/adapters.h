@@ -48,7 +48,7 @@ struct ProjectArgs {
   const void* bias;                           // [N] or null
   const void* q; int64_t q_g; int q_ld;       // Q(g, n, j) = q[g * q_g + n * q_ld + j], the adapter's second factor; zeros for j in [r, q_ld)
   const void* h; int rp;                      // sorted rows: fp32 [T][rp], or bf16 [T][rp / 16][16 hi, 16 lo]
-  const int* perm; const int* key; const int* start; const int* end;
+  const int* perm; const int* key; const int* end;
   int64_t T; int K, N, r, G;
   void* y; int64_t ldy;
   int parts, part_stages;                     // K in parts of that many stages, summed by a second launch; 0: in one

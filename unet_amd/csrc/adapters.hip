@@ -114,7 +114,7 @@ struct ShrinkArgs {
   const void* x; int64_t ldx;                 // rows of C elements
   const void* p; int64_t p_g; int p_ld;       // P(g, j, c) = p[g * p_g + j * p_ld + c]
   const float* scales;
-  const int* perm; const int* key; const int* start; const int* end;
+  const int* perm; const int* key;
   int64_t T; int C, r, G, rp;
   void* h;                                    // see ProjectArgs
   bf16* ht; int64_t ldt;                      // bf16: [2][rp][ldt], hi and lo parts with the rows along memory; or null
@@ -702,12 +702,12 @@ static int adapter_forward(const AdapterCall& c, const void* ids, int ids64, voi
   SX_TRY(pk.launch<T>(st));
   SX_TRY(launch_sort_ids(ids, ids64, c.T, c.G, perm, key, start, end, st));
   ShrinkArgs s = {};
-  s.x = x; s.ldx = ldx; s.p = A; s.p_g = (int64_t)c.r * Kp; s.p_ld = Kp; s.scales = c.scales; s.perm = perm; s.key = key; s.start = start; s.end = end;
+  s.x = x; s.ldx = ldx; s.p = A; s.p_g = (int64_t)c.r * Kp; s.p_ld = Kp; s.scales = c.scales; s.perm = perm; s.key = key;
   s.T = c.T; s.C = Kp; s.r = c.r; s.G = c.G; s.rp = k.rp; s.h = kept + k.h; s.ht = sizeof(T) == 2 ? (bf16*)(kept + k.ht) : nullptr; s.ldt = k.ldt;
   SX_TRY(shrink_launch<T>(s, st));
   ProjectArgs p = {};
   p.x = x; p.ldx = ldx; p.w = w; p.ldw = ldw; p.bias = c.bias; p.q = B; p.q_g = (int64_t)c.N * r8; p.q_ld = r8; p.h = kept + k.h; p.rp = k.rp;
-  p.perm = perm; p.key = key; p.start = start; p.end = end; p.T = c.T; p.K = Kp; p.N = c.N; p.r = c.r; p.G = c.G; p.y = y; p.ldy = ldy;
+  p.perm = perm; p.key = key; p.end = end; p.T = c.T; p.K = Kp; p.N = c.N; p.r = c.r; p.G = c.G; p.y = y; p.ldy = ldy;
   return project_launch<T>(p, ws + o.part, st);
 }
 
@@ -734,14 +734,14 @@ static int adapter_backward(const AdapterCall& c, const void* dy, int64_t lddy, 
   bf16* dht = sizeof(T) == 2 ? (bf16*)(ws + o.dht) : nullptr;
   if (dx || dA) {
     ShrinkArgs s = {};
-    s.x = d; s.ldx = ldd; s.p = ws + o.bt; s.p_g = (int64_t)c.r * Np; s.p_ld = Np; s.scales = c.scales; s.perm = perm; s.key = key; s.start = start; s.end = end;
+    s.x = d; s.ldx = ldd; s.p = ws + o.bt; s.p_g = (int64_t)c.r * Np; s.p_ld = Np; s.scales = c.scales; s.perm = perm; s.key = key;
     s.T = c.T; s.C = Np; s.r = c.r; s.G = c.G; s.rp = k.rp; s.h = ws + o.dh; s.ht = dht; s.ldt = k.ldt;
     SX_TRY(shrink_launch<T>(s, st));
   }
   if (dx) {
     ProjectArgs p = {};
     p.x = d; p.ldx = ldd; p.w = ws + o.wt; p.ldw = Np; p.q = ws + o.at; p.q_g = (int64_t)c.K * r8; p.q_ld = r8; p.h = ws + o.dh; p.rp = k.rp;
-    p.perm = perm; p.key = key; p.start = start; p.end = end; p.T = c.T; p.K = Np; p.N = c.K; p.r = c.r; p.G = c.G; p.y = dx; p.ldy = c.K;
+    p.perm = perm; p.key = key; p.end = end; p.T = c.T; p.K = Np; p.N = c.K; p.r = c.r; p.G = c.G; p.y = dx; p.ldy = c.K;
     SX_TRY(project_launch<T>(p, ws + o.part, st));
   }
   OuterArgs q = {};
