@@ -387,3 +387,67 @@ def test_parts_have_the_same_bits_in_a_replayed_graph(K, N, G):
             torch.cuda.synchronize()
             assert torch.equal(y, want)
             torch.randn(1 << 20, device="cuda").sum()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,K,N,r,used", [(5, 96, 80, 4, 2), (64, 260, 128, 8, 5), (300, 517, 65, 8, 1), (2100, 520, 264, 8, 5), (700, 64, 1100, 20, 40)])
+def test_many_registered_adapters_few_of_them_in_the_batch(T, K, N, r, used, dtype):
+    """1500 adapters, rows of a few of them together or mixed: the same results whatever is registered besides; zeros for the others."""
+    from unet_amd.adapters import adapter_linear
+    i = _inputs(T, K, N, r, 1500, dtype, seed=T)
+    g = torch.Generator().manual_seed(used)
+    some = torch.randperm(1500, generator=g)[:used]
+    for ids in (some[torch.arange(T) * used // T], some[torch.randint(0, used, (T,), generator=g)]):
+        i["ids"] = ids.cuda()
+        y, _, dA, dB = _check(i)
+        others = torch.ones(1500, dtype=torch.bool)
+        others[some] = False
+        assert not dA[others.cuda()].any() and not dB[others.cuda()].any()
+        with torch.no_grad():
+            alone = adapter_linear(i["x"], i["w"], i["b"], i["A"], i["B"], i["ids"], scales=i["sc"])
+        ref, tol = _ref(i)[0]
+        assert bool(((alone.double().cpu() - ref).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype,K,N", [(torch.float32, 23304, 23205), (torch.bfloat16, 32872, 32801)])
+def test_a_projection_beyond_two_gib(dtype, K, N):
+    """W (and its transpose in the backward pass) of 2 GiB and more: 32-bit offsets end inside of it.  References in 64 bits by pieces of W, the
+    tolerances of the top of this file."""
+    T, r, G = 70, 3, 2
+    i = _inputs(T, 8, 8, r, G, dtype, "random")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    w = torch.empty(N, K, dtype=dtype, device="cuda")
+    assert w.numel() * w.element_size() >= 1 << 31
+    for a in range(0, N, 4096):
+        w[a:a + 4096] = (torch.randn(min(4096, N - a), K, generator=g, device="cuda") / K ** 0.5).to(dtype)
+    rand = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    i.update(w=w, x=rand(T, K).to(dtype).requires_grad_(True), b=rand(N).to(dtype), dy=rand(T, N).to(dtype),
+             A=(rand(G, r, K) / K ** 0.5).to(dtype).requires_grad_(True), B=(rand(G, N, r) / r ** 0.5).to(dtype).requires_grad_(True))
+    y, dx, dA, dB = _call(i)
+    d = lambda t: t.detach().double()
+    x, dy, A, B, sc, ids = d(i["x"]), d(i["dy"]), d(i["A"]), d(i["B"]), d(i["sc"]), i["ids"]
+    ry, by = torch.empty(T, N, dtype=torch.float64, device="cuda"), torch.empty(T, N, dtype=torch.float64, device="cuda")
+    rx, bx = torch.zeros(T, K, dtype=torch.float64, device="cuda"), torch.zeros(T, K, dtype=torch.float64, device="cuda")
+    for a in range(0, N, 4096):
+        wa = w[a:a + 4096].double()
+        ry[:, a:a + 4096], by[:, a:a + 4096] = x @ wa.t(), x.abs() @ wa.abs().t()
+        rx += dy[:, a:a + 4096] @ wa
+        bx += dy[:, a:a + 4096].abs() @ wa.abs()
+    b = d(i["b"])
+    ry, ty, tx = ry + b, (K + r + 3) * U * (by + b.abs()), (N + r + 3) * U * bx
+    rA, rB, tA, tB = (torch.zeros_like(t) for t in (A, B, A, B))
+    s = SPLIT[dtype]
+    for k in range(G):
+        t = (ids == k).nonzero().view(-1)
+        Ak, Bk, xa, da = A[k], B[k], x[t], dy[t]
+        hh, ha = sc[k] * (xa @ Ak.t()), sc[k] * (xa.abs() @ Ak.abs().t())
+        dh, dha = sc[k] * (da @ Bk), sc[k] * (da.abs() @ Bk.abs())
+        ry[t] += hh @ Bk.t()
+        rx[t] += dh @ Ak
+        rA[k], rB[k] = dh.t() @ xa, da.t() @ hh
+        ty[t] += ((2 * K + 2 * r + 8) * U + s) * (ha @ Bk.abs().t())
+        tx[t] += ((2 * N + 2 * r + 8) * U + s) * (dha @ Ak.abs())
+        e = (t.numel() + K + N + 8) * U + s
+        tA[k], tB[k] = e * (dha.t() @ xa.abs()), e * (da.abs().t() @ ha)
+    for name, got, ref, tol in (("y", y, ry, ty), ("dx", dx, rx, tx), ("dA", dA, rA, tA), ("dB", dB, rB, tB)):
+        assert bool(((got.double() - ref).abs() <= tol + 1.01 * HALF[dtype] * ref.abs()).all()), name
