@@ -529,3 +529,28 @@ def test_forward_and_backward_captured_in_graphs_of_their_own():
                 torch.cuda.synchronize()
                 assert bool(((grad - want).abs() <= 8 * U * want.abs() + 1e-9).all()) and torch.equal(grad2, want), (seed, f)
                 grad.zero_()
+
+
+@pytest.mark.parametrize("V,K", [(300, 4), (300, 300), (9000, 4)])
+@pytest.mark.parametrize("N", [5, 5000])
+def test_a_nan_weight_reaches_the_mean(N, V, K):
+    """A NaN among the weights: their sum is NaN and with it the mean and every gradient of a live row, as in 64 bits; rows of weight 0 keep
+    theirs, and "sum" and "none" keep it in its row."""
+    from unet_amd.losses import distillation_loss
+    if N * V > 10_000_000:
+        N = 1000
+    z, top, idx = _inputs((N,), V, K)
+    w = torch.ones(N, device="cuda")
+    w[1], w[3] = float("nan"), 0.0
+    live = torch.ones(N, dtype=torch.bool, device="cuda")
+    live[3] = False
+    loss = distillation_loss(z, top, idx, weights=w)
+    (grad,) = torch.autograd.grad(loss, (z,))
+    assert torch.isnan(loss) and torch.isnan(grad[live]).all() and not grad[3].any()
+    (grad,) = torch.autograd.grad(distillation_loss(z, top, idx, weights=w), (z,), torch.tensor(0.5, device="cuda"))
+    assert torch.isnan(grad[live]).all() and not grad[3].any()
+    live[1] = False
+    for red in ("sum", "none"):
+        loss = distillation_loss(z, top, idx, weights=w, reduction=red)
+        (grad,) = torch.autograd.grad(loss, (z,), torch.ones_like(loss))
+        assert torch.isnan(grad[1]).all() and torch.isfinite(grad[live]).all()

@@ -71,6 +71,9 @@ __device__ __forceinline__ float all_sum(float v, float* red) {
   return v;
 }
 
+// the mean's divisor: the sum of the weights, at least 1e-8 (the masked losses' floor); NaN stays NaN
+__device__ __forceinline__ float divisor(float sum) { return sum < 1e-8f ? 1e-8f : sum; }
+
 __device__ __forceinline__ int64_t pair_idx(const DistillArgs& a, int64_t at) {
   return a.idx64 ? ((const int64_t*)a.idx)[at] : (int64_t)((const int32_t*)a.idx)[at];
 }
@@ -152,7 +155,7 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
     float s = 0.f;
     for (int64_t i = tid; i < a.N; i += NT) s += a.weights[i];
     s = all_sum<NT>(s, red_kl);
-    den = fmaxf(s, 1e-8f);
+    den = divisor(s);
     if (blockIdx.x == 0 && tid == 0) *a.den_out = den;
   } else if (a.den) {
     den = *a.den;
@@ -468,11 +471,10 @@ __device__ __forceinline__ float sum_all(const float* __restrict__ p, int64_t n,
   return all_sum<1024>((s[0] + s[1]) + (s[2] + s[3]), red);
 }
 
-// den = max(sum of weights, 1e-8) (the masked losses' floor)
 __global__ __launch_bounds__(1024) void distill_den_kernel(const float* __restrict__ w, int64_t n, float* __restrict__ den) {
   __shared__ float red[16];
   const float s = sum_all(w, n, red);
-  if (threadIdx.x == 0) *den = fmaxf(s, 1e-8f);
+  if (threadIdx.x == 0) *den = divisor(s);
 }
 
 __global__ __launch_bounds__(1024) void distill_total_kernel(const float* __restrict__ rows, int64_t n, const float* __restrict__ den, float den_host,
