@@ -260,12 +260,20 @@ def wants_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+_tracing_state, _transforms_active, _grad_enabled = torch._C._get_tracing_state, torch._C._are_functorch_transforms_active, torch.is_grad_enabled
+
+
 def by_autograd(*tensors):
     """Whether a call has to go through its autograd Function: one of its inputs wants a gradient, or something is at work that only sees
     what passes through one -- forward mode (a Function without a jvp refuses a tangent, a plain call would drop it), a trace (a plain
     call leaves nothing but the allocation of its output in it), a function transform."""
-    return (wants_grad(*tensors) or forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None
-            or torch._C._are_functorch_transforms_active())
+    if forward_ad._current_level >= 0 or _tracing_state() is not None or _transforms_active():
+        return True
+    if _grad_enabled():
+        for t in tensors:                        # (a generator would cost half a microsecond of a lookup's nine)
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def ptr_table(tensors):
