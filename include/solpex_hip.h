@@ -425,7 +425,8 @@ int sx_adapter_backward(int dtype, int64_t T, int K, int N, int r, int G, const 
  *                         d loss / d logits (for mean = 0: of the plain sum).  row_stats (nullable) [4][N]: kept for the call below.
  *   sx_distill_backward : dlogits = g[t * g_stride] * (the same gradient), from the logits and row_stats of the forward call.
  *                         ready != 0: dlogits still is what that forward call wrote; rows with g = 1 are then left as they are.
- * 2^-126 <= tau < inf; N < 2^22; V, K <= 2^30.
+ * 2^-126 <= tau < inf; N < 2^22; V, K <= 2^30.  Beyond 512 pairs the time grows with N * K * K (pairs that name one index are found by
+ * comparing all of a row's): 512 rows of 8000 logits take 0.17 ms with K = 1000, 8.5 ms with K = 8000.
  * --------------------------------------------------------------------------------------------- */
 int sx_distill_forward(int dtype, int64_t N, int V, int K, const void* logits, int64_t ld, int top_dtype, const void* top,
                        const void* idx, int idx64, float tau, const float* weights, int mean, float* row_loss,

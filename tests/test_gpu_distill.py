@@ -554,3 +554,28 @@ def test_a_nan_weight_reaches_the_mean(N, V, K):
         loss = distillation_loss(z, top, idx, weights=w, reduction=red)
         (grad,) = torch.autograd.grad(loss, (z,), torch.ones_like(loss))
         assert torch.isnan(grad[1]).all() and torch.isfinite(grad[live]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V,K", [(700, 513), (3000, 768), (3000, 2500), (40, 1500), (9001, 1025)])
+def test_very_many_pairs(V, K, dtype):
+    """More pairs than a block has threads, most of them naming an index that others name too."""
+    for red, g in (("mean", None), ("none", torch.tensor([0.5, 1.0, -3.0, 2.0]).cuda())):
+        z, top, idx = _inputs((4,), V, K, dtype, torch.float32, torch.int32, seed=K)
+        idx[1, ::3] = -1
+        idx[2] = idx[2] % 7
+        _check(z, top, idx, 1.25, None, red, g)
+    z, top, idx = _inputs((4100,), 33, 600, dtype, seed=3)
+    _check_rows_bf16_or_fp32(z, top, idx)
+
+
+def _check_rows_bf16_or_fp32(z, top, idx):
+    """Rows enough for a wave each: against the same loss of a few of them."""
+    from unet_amd.losses import distillation_loss
+    loss = distillation_loss(z, top, idx, reduction="none")
+    (grad,) = torch.autograd.grad(loss, (z,), torch.ones_like(loss))
+    for a in (0, 2000, 4096):
+        zs = z.detach()[a:a + 4].clone().requires_grad_(True)
+        rl, rg, lt, gt = _ref(zs, top[a:a + 4], idx[a:a + 4], 1.0, None, "none", torch.ones(4))
+        assert bool(((loss.detach()[a:a + 4].double().cpu() - rl).abs() <= lt + U * rl.abs()).all())
+        assert bool(((grad[a:a + 4].double().cpu() - rg).abs() <= gt + 1.01 * (HALF[z.dtype] + U) * rg.abs() + 1e-38).all())

@@ -317,7 +317,8 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
   if (fix_at) *fix_at = from_f32<T>(fix);
 }
 
-// any row length, the logits read once for the maximum and the sum and once for the gradient; with GRAD_ONLY, the gradient alone, from
+// any row length and any number of pairs (each compared with every other: the time grows with K * K beyond the few hundred that a block of
+// threads holds), the logits read once for the maximum and the sum and once for the gradient; with GRAD_ONLY, the gradient alone, from
 // the maxima and sums of an earlier pass.  fmaxf drops a NaN; the sum brings it back
 template <typename T, int NT, bool GRAD_ONLY>
 __global__ __launch_bounds__(NT) void distill_wide_kernel(DistillArgs a) {
@@ -506,6 +507,10 @@ template <typename T>
 static int wide_launch(const DistillArgs& a, int grad_only, hipStream_t st) {
   // a wave for a short row, more for a long one, most of them where there are few rows.  Gradient of 256 MB of bf16 logits with K = 16: rows of
   // 4000 by one wave 160 us, by four 222; of 50000 by four 122, by sixteen 137; of 131072 113 and 114
+  // Many pairs: K * K comparisons of a row (distill_wide_kernel) over as many threads as there are, unless rows enough for a wave each to fill
+  // the card have few of them.  fp32, loss and gradient, by one wave and by sixteen: 16 rows with K = 513 0.40 ms and 0.12, 1000 1.28 and 0.11,
+  // 8000 76 and 4.2; 8192 rows with K = 513 1.05 and 1.4, 1000 3.0 and 2.4
+  if (a.K > 768 || (a.K > 512 && a.N < 4096)) return wide_start<T, 1024>(a, grad_only, st);
   if (a.V <= 8192) return wide_start<T, 64>(a, grad_only, st);
   if (a.N >= 512) return wide_start<T, 256>(a, grad_only, st);
   return wide_start<T, 1024>(a, grad_only, st);
