@@ -378,7 +378,8 @@ int sx_inverse_adam_step(int N, int P, float* p, const float* grad, float* m, fl
  *   sx_embedding_backward : dtable[v] = scale * sum_{t: ids[t] = v} dout[t]; every row is written (zeros where no id points);
  *                           fp32 sums over the tokens in their order, rounded once: the same bits on every run.
  *                           workspace: sx_embedding_workspace_bytes, 16-byte aligned, contents irrelevant before and after.
- * rows <= 2^24, n < 2^31 - 1024.  n = 0 is allowed.
+ * rows <= 2^24, n < 2^31 - 1024.  n = 0 is allowed.  The gradient is made for up to 2^18 rows; beyond, the order of the ids costs
+ * n * rows / 1024 reads (2^20 ids: 0.4 ms of 2^18 rows, 10 ms of 2^24).
  * --------------------------------------------------------------------------------------------- */
 int64_t sx_embedding_workspace_bytes(int64_t n, int64_t rows, int dim);
 int sx_embedding_forward(int dtype, int64_t n, int64_t rows, int dim, const void* table, int64_t ld, const void* ids, int ids64,
@@ -390,7 +391,8 @@ int sx_embedding_backward(int dtype, int64_t n, int64_t rows, int dim, const voi
  * Low-rank adapters of many requests beside one shared projection.  Row t belongs to adapter a = ids[t] (outside [0, G): none).
  *   y[t] = W x[t] + bias + scales[a] * B_a (A_a x[t]);  gradients with respect to x, A and B (W, bias and scales are constants)
  * x (T, K), w (N, K), y / dy (T, N) with row strides in elements; A (G, r, K), B (G, N, r), dx (T, K), dA, dB contiguous; all of
- * `dtype`.  bias [N] and scales [G] (fp32) may be NULL.  Sums in fp32, one rounding; the same bits on every run.
+ * `dtype`.  bias [N] and scales [G] (fp32) may be NULL.  Sums in fp32, one rounding; the same bits on every run.  In bf16 A x and B^T dy
+ * are multiplied on as two bf16 parts (2^-17; an infinity that meets them may come out as NaN); other rows and adapters never see a NaN.
  *   kept      : sx_adapter_kept_bytes, written by the forward call (rows in the order of their adapter, A x), read by the backward call.
  *               NULL: no backward call will follow; up to 64 rows then take a path of their own (two launches).
  *   workspace : sx_adapter_workspace_bytes for the call's mode, contents irrelevant before and after.  Both 16-byte aligned.

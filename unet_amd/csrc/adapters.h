@@ -36,7 +36,8 @@ __device__ __forceinline__ typename Elem<T>::Vec load_piece(const T* __restrict_
 }
 
 // h in fp32 as the MFMA's operand.  fp32: as it is.  bf16: 16 ranks are 16 hi parts, then 16 lo parts (h - hi): one K block of 32, whose
-// other side holds the 16 factors twice.  h loses 2^-17 of itself where one bf16 would cost 2^-9.
+// other side holds the 16 factors twice.  h loses 2^-17 of itself where one bf16 would cost 2^-9: a third part would take another MFMA per 16
+// ranks.  An infinity among the factors meets both parts, lo may be 0 or of the other sign: what should be infinite may come out as NaN.
 __device__ __forceinline__ bf16 h_lo(float v) {
   const float hi = (float)(bf16)v;
   return fabsf(hi) == INFINITY ? (bf16)0.f : (bf16)(v - hi);

@@ -1,6 +1,7 @@
 """Learned rows for discrete conditions (machine, scenario, parameter bin): a scaled table lookup and its gradient on the HIP
 kernels of `csrc/embedding.hip`.  No counterpart in the reference, whose conditions are all continuous (`params`); the rows
-feed the same places, e.g. `UNet(..., P=dim)(x, params=scaled_embedding(ids, table))`.  No CPU fallback."""
+feed the same places, e.g. `UNet(..., P=dim)(x, params=scaled_embedding(ids, table))` with dim <= 64, the most that the U-Net
+takes, or the latent MLPs' input.  No CPU fallback."""
 from __future__ import annotations
 
 import torch
@@ -49,7 +50,7 @@ class _EmbeddingFn(torch.autograd.Function):
 def scaled_embedding(ids, table, scale=1.0):
     """out[..., :] = scale * table[ids[...], :] in the table's dtype (fp32 or bf16; one rounding).
 
-    ids: int64 / int32 of any shape, on the table's device.  An id outside [0, rows) -- -1 by convention -- is padding: a row of
+    table (rows, dim), at most 2^24 rows.  ids: int64 / int32 of any shape, on the table's device.  An id outside [0, rows) -- -1 by convention -- is padding: a row of
     zeros, no gradient.  The table's gradient sums the tokens of a row in their order, in fp32: the same bits on every run.
     Not differentiable twice.  `scale` is a number."""
     who = "scaled_embedding"
