@@ -6,7 +6,7 @@
  * Python module API solpex.models / solpex.losses / solpex.train / solpex.predict, which dispatches
  * to ATen ops.  Each entry point below therefore cites the reference *Python call site* whose ATen
  * work it replaces (paths relative to the reference root).  The host-side mirror of that Python API
- * lives in unet_amd/ and binds these symbols with ctypes (see INTEGRATION.md).
+ * lives in unet_amd/ and binds these symbols with ctypes.
  *
  * Conventions
  *  - Plain pointers and sizes only; no torch types.  All pointers are DEVICE pointers unless a
@@ -240,7 +240,7 @@ int sx_global_avg_pool(int dtype, int B, int HW, int C, const void* x, int ld, f
 int sx_zero_border(int dtype, int B, int H, int W, int Hin, int Win, int C, void* t, int ld, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
- * Latent MLPs (SURVEY 8f-2; latent.py:14-48 ParamToZ / ZToParam and their SmoothL1 trainers, latent.py:51-310), fp32.
+ * Latent MLPs (latent.py:14-48 ParamToZ / ZToParam and their SmoothL1 trainers, latent.py:51-310), fp32.
  *   sx_gemm_f32 : C[m][n] (+)= epilogue( sum_k A(m,k) * B(n,k) + bias[n] ), A(m,k) = A[m*a_sm + k*a_sk],
  *                 B(n,k) = B[n*b_sn + k*b_sk].  One kernel for nn.Linear forward (A = x, B = W), its input gradient
  *                 (A = dy, B = W^T by strides) and its weight gradient (A = dy^T, B = x^T).  Epilogue, in this order:
@@ -263,7 +263,7 @@ int sx_smooth_l1(int64_t n, const float* pred, const float* target, float beta, 
 int sx_mul(int64_t n, const float* x, const float* m, float* y, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
- * Device-resident dataset (SURVEY 8f-3; replaces the per-item host path of SOLPSDataset.__getitem__ + default collate,
+ * Device-resident dataset (replaces the per-item host path of SOLPSDataset.__getitem__ + default collate,
  * data.py:359-391, for tensors that already live in HBM).
  *   sx_gather_rows : dst[r][0..row_elems) = src[idx[r]][0..row_elems) for r < n_rows; idx is a DEVICE int64 array,
  *                    strides in elements; out-of-range indices are skipped (the host wrapper raises IndexError first).

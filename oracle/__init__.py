@@ -9,8 +9,8 @@ product package `unet_amd` (which must fail loudly without its HIP library).
 Parity pin: every function here is checked against golden vectors captured
 from the live reference (`/root/reference/solpex`, imported in the build
 container by `tools/make_golden.py`; vectors committed under `tests/golden/`).
-The reference itself ships no tests or golden vectors for this path
-(SURVEY.md section 4), so those captured vectors are the only pin.
+The reference itself ships no tests or golden vectors for this path,
+so those captured vectors are the only pin.
 """
 from .unet_ref import UNetCfg, init_state_dict, unet_forward, unet_encode, unet_decode, film_generator  # noqa: F401
 from .loss_ref import masked_weighted_loss, masked_mean, mae_norm, batch_error_sums_ev, edge_weights, sobel_xy  # noqa: F401

@@ -131,7 +131,7 @@ def weighted_masked_mse(pred, target, mask, cw):
 
 
 def weighted_masked_mse_per_sample(pred, target, mask, cw):
-    """Per-sample form of the above (B independent problems; SURVEY 3.5)."""
+    """Per-sample form of the above (B independent problems)."""
     m = mask.expand_as(pred)
     w = cw.view(1, -1, 1, 1).to(pred.dtype)
     num = ((pred - target) ** 2 * m * w).sum(dim=(1, 2, 3))

@@ -1,5 +1,5 @@
 #!/usr/bin/env python3
-"""BASELINE config 5 (plasma-to-sources: in 10, out 4, base 64, depth 3, no FiLM, 256x128): training step time.
+"""Plasma-to-sources network (in 10, out 4, base 64, depth 3, no FiLM, 256x128): training step time.
 usage: cfg5_bench.py [batch] [steps] [bf16|fp32]"""
 import os, sys, time
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))

@@ -8,7 +8,7 @@ import torch
 import bench
 from unet_amd import _lib as L
 
-arch = bench.ARCH_B if os.environ.get("CFG") == "5" else bench.ARCH_A       # CFG=5: BASELINE configs[4] (batch 32)
+arch = bench.ARCH_B if os.environ.get("CFG") == "5" else bench.ARCH_A       # CFG=5: the plasma-to-sources network (batch 32)
 B = int(sys.argv[1]) if len(sys.argv) > 1 else (32 if arch is bench.ARCH_B else 64)
 make = bench.conv_launch_maker(B, L.SX_BF16)
 st = torch.cuda.current_stream()

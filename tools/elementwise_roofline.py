@@ -1,8 +1,8 @@
 #!/usr/bin/env python3
-"""Achieved HBM bandwidth of the element-wise / pooling / loss / optimizer kernels of one training step (
-batch 64, 128x64, base 32, depth 3, bf16) from a rocprofv3 kernel trace of bench.py.
+"""Achieved HBM bandwidth of the element-wise / pooling / loss / optimizer kernels of one training step:
+batch 64, 128x64, base 32, depth 3, bf16, from a rocprofv3 kernel trace of bench.py.
 usage: python tools/elementwise_roofline.py results.db > profiles/xxx.txt
-Algorithmic bytes = every tensor the kernel must read once + write once (SURVEY 8d), T(level) = B*H*W*C*2 bytes."""
+Algorithmic bytes = every tensor the kernel must read once + write once, T(level) = B*H*W*C*2 bytes."""
 import re, sqlite3, sys
 
 B, PEAK = 64, 8000.0

@@ -1,5 +1,5 @@
 #!/usr/bin/env python3
-"""Which kernels carry the split-bf16 error at BASELINE configs[4]'s full grid?  Worst per-tensor gradient error (smooth loss)
+"""Which kernels carry the split-bf16 error at the full 256x128 grid of the 512-channel network?  Worst per-tensor gradient error (smooth loss)
 of one training step against the CPU oracle for: everything split / weight gradients exact / convolutions exact / all exact.
 Also the step time of each mix at batch 32."""
 import os, sys, time

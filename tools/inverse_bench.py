@@ -1,5 +1,5 @@
 #!/usr/bin/env python3
-"""BASELINE config 4 shape: batched inverse (cfg A, 128x64), problem-steps/s on one GPU.  usage: inverse_bench.py [N] [steps]"""
+"""Batched inverse (cfg A, 128x64), problem-steps/s on one GPU.  usage: inverse_bench.py [N] [steps]"""
 import os, sys, time
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 import torch

@@ -13,7 +13,7 @@ st = torch.cuda.current_stream()
 C = [32, 64, 128, 256]
 HW = [(128, 64), (64, 32), (32, 16), (16, 8)]
 CIN0, COUT = 8, 8
-if os.environ.get("CFG") == "5":           # BASELINE configs[4]: base 64, 256x128, in 10 (padded 16), out 4 (padded 8)
+if os.environ.get("CFG") == "5":           # base 64, 256x128, in 10 (padded 16), out 4 (padded 8)
     C = [64, 128, 256, 512]
     HW = [(256, 128), (128, 64), (64, 32), (32, 16)]
     CIN0 = 16

@@ -22,7 +22,7 @@ namespace sx {
 // (measured: cfg 5 fp32 step 31.1 ms with 32-channel tiles).
 template <int PL> struct X3Row { static constexpr int BYTES = PL * 64 + 32; static constexpr int WBYTES = PL == 3 ? 192 : BYTES; };
 
-// THREE planes ("x6", round 3): v = hi + mid + lo + r, |r| <= 2^-27 |v|, and a product keeps the six terms down to 2^-18
+// THREE planes ("x6"): v = hi + mid + lo + r, |r| <= 2^-27 |v|, and a product keeps the six terms down to 2^-18
 // (hi*hi, hi*mid, mid*hi, mid*mid, hi*lo, lo*hi; the dropped mid*lo, lo*mid, lo*lo are <= 2^-27): fp32-grade products at six
 // bf16 MFMAs per block (96 matrix-core cycles against 256 of the exact kernels).  Used where two planes were measured outside
 // the 1e-4 contract: networks whose widest layer reaches 512 channels (unet_plan.hip).

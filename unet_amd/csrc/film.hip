@@ -301,7 +301,7 @@ __global__ __launch_bounds__(256) void film_bwd_b_kernel(const FilmArgs) { film_
 
 // Training tail: rows y < ngen are the generators (dW2 rows and fused dW1 rows), the rows behind them run the GroupNorm affine /
 // bias gradient reductions of the same backward half.
-// ... and behind those, the slab reduction of the same half's weight gradients (round 3): it is independent of the generators,
+// ... and behind those, the slab reduction of the same half's weight gradients: it is independent of the generators,
 // and as a launch of its own (16 us) it ran while this one's 40 latency-bound blocks (33 us) had the chip to themselves.
 // Table sizes are what fits the 4 KB kernel-argument segment next to FilmArgs; larger halves take the separate launches.
 static constexpr int TAIL_GN = 20, TAIL_RED = 15;

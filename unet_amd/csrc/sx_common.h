@@ -106,7 +106,7 @@ __device__ __forceinline__ void store8(bf16* p, const f32x8& r) {
 
 // ------------------------------------------------------------------ math
 // v_exp_f32 + v_rcp_f32 (1 ulp each): an IEEE division here costs ~10 extra VALU instructions per element, and the
-// element-wise GroupNorm / SiLU passes sit close to their VALU floor (measured: see DESIGN.md, "element-wise passes")
+// element-wise GroupNorm / SiLU passes sit close to their VALU floor
 __device__ __forceinline__ float sigmoidf_(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f)); }
 __device__ __forceinline__ float siluf_(float z) { return z * sigmoidf_(z); }
 __device__ __forceinline__ float dsiluf_(float z) {
@@ -158,7 +158,7 @@ int env_int(const char* name, int dflt);
 // 1: fp32 convolutions and weight gradients run as three bf16 MFMAs on split operands (default; conv_x3.hip); 0: exact
 // fp32 MFMA (SX_FP32_EXACT=1 or sx_set_fp32_exact).  The packed fp32 weights differ between the two: repack after a switch.
 int fp32_split();
-// the process-wide mode alone, whatever scope is active: the WEIGHT GRADIENTS follow it (measured at BASELINE configs[4], full
+// the process-wide mode alone, whatever scope is active: the WEIGHT GRADIENTS follow it (measured on the 512-channel network, full
 // grid, tools/fp32_mix.py: the split arithmetic's error comes from the forward / data-gradient convolutions alone --
 // convolutions split 3.95e-4 with exact or split weight gradients, convolutions exact 3.31e-5 with either)
 int fp32_split_process();

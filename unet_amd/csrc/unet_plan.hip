@@ -205,7 +205,7 @@ static int build_plan(const sx_unet_desc* dp, Plan& p) {
 
 // fp32 tier, arithmetic per architecture.  Two-plane split products carry ~4e-6 per convolution; through the whole network and
 // its GroupNorm backward (differences of large sums) that came to a worst per-tensor gradient error of 8e-5 at cfg A
-// (bottleneck 256 channels) and 4.1e-4 at BASELINE configs[4] (bottleneck 512, 256x128; smooth loss, so this is arithmetic,
+// (bottleneck 256 channels) and 4.1e-4 with twice the width (bottleneck 512, 256x128; smooth loss, so this is arithmetic,
 // not a loss kink: tests/test_gpu_fullsize.py) against 3.3e-5 with exact fp32 MFMA -- all of it from the forward / data-gradient
 // convolutions (tools/fp32_mix.py), none from the weight gradients.  The contract is 1e-4, so networks whose widest layer
 // reaches 512 channels run their convolutions on THREE planes (conv_x3.hip, six MFMAs per block, fp32-grade products).

@@ -5,8 +5,8 @@ Two kinds of code live here:
     loop and inference (solpex/train.py:284, solpex/predict.py:134).  On CUDA tensors they run the fused
     HIP kernel `sx_norm_apply` (one pass for all channels instead of slice/map/cat per channel);
   * host-side dataset preparation (npz loading, fitting, parameter transforms, DataLoaders), which the
-    reference runs once on the CPU and which is deliberately plain Python/numpy here too (SURVEY 2.1 #5:
-    out of scope as kernels, kept for drop-in).  CPU tensors handed to a normalizer by that pipeline
+    reference runs once on the CPU and which is deliberately plain Python/numpy here too:
+    out of scope as kernels, kept for drop-in.  CPU tensors handed to a normalizer by that pipeline
     (`SOLPSDataset.__getitem__`) are mapped with the same formulas in torch on the host.
 """
 from __future__ import annotations
@@ -425,7 +425,7 @@ def rank_share(global_batch, rank, world, pad):
 
 
 class ResidentLoader:
-    """Device-resident replacement of `DataLoader(Subset(SOLPSDataset, indices), batch_size, shuffle)` (SURVEY 8f-3).
+    """Device-resident replacement of `DataLoader(Subset(SOLPSDataset, indices), batch_size, shuffle)`.
 
     The reference re-normalises every sample on the host every epoch (solpex/data.py:359-366) and collates item by
     item; at the HIP path's step time that host loop is the bottleneck.  Here the subset is uploaded ONCE, normalised

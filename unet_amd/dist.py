@@ -1,5 +1,5 @@
 """Data-parallel helpers: one process per GPU, torch.distributed (backend "nccl" = RCCL over xGMI on
-ROCm; "gloo" in the CPU tests).  The reference is single-device (SURVEY 2.2); what DP must preserve is
+ROCm; "gloo" in the CPU tests).  The reference is single-device; what DP must preserve is
 its batch-GLOBAL loss denominators (solpex/losses.py:77-79):
 
     1. every rank computes its local raw denominators  sum(m), sum(m*w), sum(m_g)       (sx_loss_prepare)

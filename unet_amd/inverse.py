@@ -2,7 +2,7 @@
 
 Reference: scripts/eval_inverse_cycle_conditional_unet.py:105-162 (losses, forward_from_scaled) and :316-444 (the per-case
 optimisation loop and the forward-cycle metrics).  The reference solves one case at a time (B = 1: mask (1,1,H,W),
-p (1,P)); here N cases run as one batch per call (SURVEY 8 row a20 / BASELINE config 4) with every per-case quantity kept
+p (1,P)); here N cases run as one batch per call with every per-case quantity kept
 per SAMPLE: loss denominators, the L2 regulariser, Adam state, clamp and early stopping.  Only the data gradient of the
 network is computed (`SX_BWD_WEIGHT_GRADS` off): the reference's `loss.backward()` also fills every weight gradient and
 throws it away.
@@ -245,7 +245,7 @@ def inverse_with_restarts(model, mask, y_true_norm, p0_restarts, **kw):
 
 def batched_inverse_sharded(model, mask, y_true_norm, p0, **kw):
     """config 4 across ranks: cases are independent, so each rank takes a contiguous slice and the rows are all-gathered at the end
-    (no data-path collective; SURVEY 8e)."""
+    (no data-path collective)."""
     rank, world = sxdist.rank(), sxdist.world_size()
     lo, hi = sxdist.shard_range(p0.shape[0], rank, world)
     res = batched_inverse(model, mask[lo:hi], y_true_norm[lo:hi], p0[lo:hi], **kw)

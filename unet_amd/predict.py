@@ -1,7 +1,7 @@
 """MI355X-native mirror of `solpex.predict` (reference: solpex/predict.py).
 
 `load_checkpoint`, `predict_fields`, `predict_te`, `scale_params` keep the reference signatures, return
-values, printed warnings and exceptions.  New (SURVEY 8f rank 1): `predict_fields_batch` runs N
+values, printed warnings and exceptions.  New: `predict_fields_batch` runs N
 (mask, params) pairs in one HIP forward and de-normalises on the device.
 """
 from __future__ import annotations

@@ -1,10 +1,10 @@
-"""Trial-level parallelism for hyper-parameter / ablation sweeps (SURVEY 8f-4).
+"""Trial-level parallelism for hyper-parameter / ablation sweeps.
 
 Reference: scripts/run_ablation_sweep.py:257-271 runs its experiments one after the other on one device; each is a small
 model (base 16-64, batch 4-16) that cannot fill an MI355X, let alone eight.  The trials are independent, so the natural
 partition is one trial per GPU at a time: every rank of a `torch.distributed.run` job takes a share of the trial list,
 trains each of its trials as a single-rank job (`dist.local_mode()`: no gradient all-reduce, its own checkpoint file) and
-the result rows are gathered on every rank at the end -- no data-path collective, like the batched inverse (SURVEY 8e).
+the result rows are gathered on every rank at the end -- no data-path collective, like the batched inverse.
 """
 from __future__ import annotations
 

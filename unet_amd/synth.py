@@ -1,4 +1,4 @@
-"""Seeded synthetic SOLPS-shaped inputs (SURVEY.md 8d): annular mask, standardised
+"""Seeded synthetic SOLPS-shaped inputs: annular mask, standardised
 control parameters, masked normalised targets.  Host-side torch only; used by
 bench.py, the golden-vector tool and the tests so that all three see the same data.
 

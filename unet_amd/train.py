@@ -183,7 +183,7 @@ class TrainEngine:
             # (single scale: phase 1 keeps this rank's own pixel count in the loss workspace and phase 2 reports it as out[3];
             # the multi-scale path has no such slot: copy den[0] aside before the all-reduce)
             px_local = bufs.den[0].clone() if int(o["multiscale"]) != 0 else None
-            handle = sxdist.all_reduce_sum(bufs.den, async_op=True)        # batch-global denominators (SURVEY 8e)
+            handle = sxdist.all_reduce_sum(bufs.den, async_op=True)        # batch-global denominators
         return m, px_local, handle
 
     def _loss_end(self, sess, bufs, y, begun, lam_grad, want_grad, grad_scale):
