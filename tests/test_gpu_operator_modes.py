@@ -131,3 +131,20 @@ def test_sizes_beyond_a_c_int_are_refused():
     with pytest.raises(ValueError, match="too long"):
         distillation_loss(one, one.expand(1, w), zero.expand(1, w))
     assert torch.cuda.memory_allocated() == before
+
+
+@pytest.mark.parametrize("name", NAMES[:5])
+def test_recomputed_forward_passes(name):
+    """Non-reentrant checkpoints hand each saved tensor out once, with and without create_graph; all through offloaded ones too."""
+    from torch.utils.checkpoint import checkpoint
+    fn, args = _calls()[name]
+    leaves = [a.clone().requires_grad_(True) for a in args]
+    want = torch.autograd.grad(fn(*leaves).square().sum(), leaves)
+    for create in (False, True):
+        y = checkpoint(fn, *leaves, use_reentrant=False)
+        got = torch.autograd.grad(y.square().sum(), leaves, create_graph=create)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        with torch.autograd.graph.save_on_cpu():
+            y = fn(*leaves)
+        got = torch.autograd.grad(y.square().sum(), leaves, create_graph=create)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -44,12 +44,19 @@ class _AdapterFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        x, weight, A, B, scales, kept = ctx.saved_tensors
-        if torch.is_grad_enabled():
-            who = "adapter_linear"
+        saved = ctx.saved_tensors                  # once: recomputed ones are handed out a single time
+        if not torch.is_grad_enabled():
+            dx, dA, dB = _AdapterFn.gradients(ctx, saved, dy)
+        else:
+            who, (x, _, A, B, _, _) = "adapter_linear", saved
             with torch.no_grad():
-                dx, _, _, dA, dB, _, _ = _AdapterFn.backward(ctx, dy)
-            return (L.not_twice(who, dx, dy, A, B), None, None, L.not_twice(who, dA, dy, x, B), L.not_twice(who, dB, dy, x, A), None, None)
+                dx, dA, dB = _AdapterFn.gradients(ctx, saved, dy)
+            dx, dA, dB = L.not_twice(who, dx, dy, A, B), L.not_twice(who, dA, dy, x, B), L.not_twice(who, dB, dy, x, A)
+        return dx, None, None, dA, dB, None, None
+
+    @staticmethod
+    def gradients(ctx, saved, dy):
+        x, weight, A, B, scales, kept = saved
         need_x, _, _, need_a, need_b = ctx.needs_input_grad[:5]
         N, K = weight.shape
         G, r = A.shape[:2]
@@ -63,7 +70,7 @@ class _AdapterFn(torch.autograd.Function):
             for g in (dA, dB):
                 if g is not None:
                     g.zero_()
-            return dx, None, None, dA, dB, None, None
+            return dx, dA, dB
         w, ldw = L.rows_2d(weight, K)
         d2, ldd = L.rows_2d(dy, N, aligned=True)
         Ad, Bd = L.packed(A), L.packed(B)
@@ -71,7 +78,7 @@ class _AdapterFn(torch.autograd.Function):
         ws = torch.empty(nw, dtype=torch.uint8, device=dev)
         L.launch("sx_adapter_backward", dev, dt, T, K, N, r, G, L.addr(x2), ldx, L.addr(w), ldw, L.addr(Ad), L.addr(Bd), L.addr(scales), L.addr(d2), ldd,
                  L.addr(kept), kept.numel(), L.addr(dx), L.addr(dA), L.addr(dB), L.addr(ws), nw)
-        return dx, None, None, dA, dB, None, None
+        return dx, dA, dB
 
 
 def adapter_linear(x, weight, bias, A, B, ids, *, scales=None):

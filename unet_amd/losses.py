@@ -183,14 +183,21 @@ class _DistillFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g):
+        saved = ctx.saved_tensors                  # once: recomputed ones are handed out a single time
+        if not torch.is_grad_enabled():
+            d = _DistillFn.gradient(ctx, saved, g)
+        else:
+            with torch.no_grad():
+                d = _DistillFn.gradient(ctx, saved, g)
+            d = L.not_twice("distillation_loss", d, g, saved[0])
+        return d, None, None, None, None, None
+
+    @staticmethod
+    def gradient(ctx, saved, g):
         """Where the forward pass left the gradient for an upstream gradient of 1, that is it; for another one the gradient is computed
         again from the logits (one rounding), not scaled after its own."""
         who = "distillation_loss"
-        logits, top, idx, weights, keep, d = ctx.saved_tensors
-        if torch.is_grad_enabled():
-            with torch.no_grad():
-                grads = _DistillFn.backward(ctx, g)
-            return (L.not_twice(who, grads[0], g, logits), *grads[1:])
+        logits, top, idx, weights, keep, d = saved
         tau, reduction = ctx.meta
         V, K = logits.shape[-1], top.shape[-1]
         # The buffer is the caller's from here on, who may change it: a second backward pass fills one of its own (and does not mind the
@@ -204,7 +211,7 @@ class _DistillFn(torch.autograd.Function):
         L.launch("sx_distill_backward", logits.device, L.dtype_code(logits, who), z.shape[0], V, K, L.addr(z), ld, L.dtype_code(top, who), L.addr(top),
                  L.addr(idx), L.ids_flag(idx, who), tau, L.addr(weights), 1 if reduction == "mean" else 0, L.addr(keep) + 4, L.addr(keep), L.addr(g),
                  1 if reduction == "none" else 0, 1 if ready else 0, L.addr(d), V)
-        return d, None, None, None, None, None
+        return d
 
 
 def distillation_loss(logits, top_logits, top_idx, *, temperature=1.0, weights=None, reduction="mean"):
