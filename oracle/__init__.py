@@ -3,7 +3,7 @@
 TEST INFRASTRUCTURE ONLY.  This package is a fresh, plain-PyTorch (CPU, fp32)
 restatement of the reference algorithm.  It may be imported only by `tests/`,
 by `__graft_entry__.smoke()` and by the `cpu_baseline` leg of `bench.py`,
-and there only as the checker / the timed CPU baseline -- never by the
+and there only as the oracle and the timed CPU baseline -- never by the
 product package `unet_amd` (which must fail loudly without its HIP library).
 
 Parity pin: every function here is checked against golden vectors captured
